@@ -302,6 +302,142 @@ NOOR_MOE_API int noor_moe_route_static(const void* x, const void* gate, const fl
                                        int64_t T, int32_t d, int32_t E, int32_t top_k, int32_t dtype,
                                        int32_t* idx, float* w, int64_t* counts, void* stream);
 
+/* ---- the attention half of a block, served from an 8-bit cache ---- */
+
+/* The reference's GQAAttention (attention.rs:67-191) and RoPE (rope.rs:5-90)
+ * run on f32 host tensors with an f32 cache; these entry points are the
+ * device form of the same steps over a paged cache held in 8 bits.  They need
+ * no handle: all pointers are device pointers, the work is enqueued on
+ * `stream` (NULL = the legacy default stream) of `device`, nothing is
+ * allocated and nothing synchronises, so every call can be captured into a
+ * CUDA graph.  Activations are F32 or BF16 (NOOR_DTYPE_*).  Host-visible
+ * mistakes return a status; mistakes in device metadata (lengths, row offsets,
+ * page numbers) set the cache's status word and never touch memory outside
+ * the buffers. */
+
+/* A [tokens][heads][head_dim] tensor: element strides of a token and of a
+ * head; a head's head_dim elements are contiguous.  Strides may be 0
+ * (broadcast inputs) or any order; an output's heads must not overlap. */
+typedef struct {
+  const void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} noor_heads;
+
+#define NOOR_ROPE_INTERLEAVED 0 /* pairs (2i, 2i + 1), RoPE::apply (rope.rs:49-90) */
+#define NOOR_ROPE_HALF 1        /* pairs (i, i + rotate_dim / 2) */
+
+/* Rotary positions: pair i of the first rotate_dim dims (even, 0 rotates
+ * nothing) turns by position * inv_freq[i]; the rest of the head passes
+ * unchanged.  factor scales the rotated dims (1, or the attention factor of a
+ * table stretched for long contexts).  The angle is formed and reduced in
+ * 64 bits, so far positions lose nothing. */
+typedef struct {
+  const float* inv_freq; /* [rotate_dim / 2] device */
+  int32_t rotate_dim;
+  int32_t layout;        /* NOOR_ROPE_* */
+  float factor;
+} noor_rotary;
+
+/* Rotate q and, if k is not NULL, k beside it: token t of both is at
+ * positions[t] (int32).  inverse != 0 turns the other way, which with the
+ * same factor is the gradient.  Outputs may be the inputs (same strides) or
+ * not overlap them; q_out / k_out are written whole.  head_dim even, at most
+ * 1024. */
+NOOR_MOE_API int noor_rope_apply(const noor_rotary* r, const noor_heads* q, const noor_heads* q_out, int32_t q_heads,
+                                 const noor_heads* k, const noor_heads* k_out, int32_t k_heads,
+                                 const int32_t* positions, int64_t tokens, int32_t head_dim, int32_t dtype,
+                                 int32_t inverse, int32_t device, void* stream);
+
+#define NOOR_KV_INT8 0 /* codes -127..127 */
+#define NOOR_KV_E4M3 1 /* 8-bit floating point, largest value 448 */
+
+/* A paged cache of keys and values.  Page p holds `block` tokens of every kv
+ * head: k_codes [num_blocks][n_kv_heads][block][head_dim] and v_codes
+ * [num_blocks][n_kv_heads][head_dim][block] (a value's tokens side by side,
+ * as the product with the probabilities reads them), one byte a code;
+ * k_scale / v_scale [num_blocks][n_kv_heads] f32; value = code * scale.
+ * noor_kv_append chooses the scale as the smallest power of two (at least
+ * 2^-126) that holds the block's largest magnitude, so growing it later is an
+ * exact shift.  block 16, 32 or 64; head_dim a multiple of 16 up to 256; the
+ * four arrays 16-byte aligned.
+ * status (one device int32, zero at first, nullable) takes the first mistake
+ * that a kernel found in device metadata: NOOR_KV_BAD_*. */
+typedef struct {
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int32_t* status;
+  int64_t num_blocks;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t block;
+  int32_t format; /* NOOR_KV_INT8 / NOOR_KV_E4M3 */
+  int32_t device;
+} noor_kv_cache;
+
+#define NOOR_KV_BAD_ROWS 1    /* cu_rows not ascending within 0 .. n_rows */
+#define NOOR_KV_BAD_LENGTH 2  /* kv_lens below 0, below the sequence's rows, or past its pages */
+#define NOOR_KV_BAD_PAGE 3    /* a page number outside 0 .. num_blocks - 1 */
+#define NOOR_KV_TIMEOUT 4     /* a bounded wait gave up */
+
+/* A ragged batch of sequences over the cache: rows cu_rows[b] .. cu_rows[b+1]-1
+ * belong to sequence b, whose token j lives in page
+ * block_table[b * table_stride + j / block], slot j % block.  n_rows is the
+ * number of rows the row tensors hold; rows at or past cu_rows[batch] are
+ * padding and are left as they were.  A sequence may have no rows.  One whose
+ * offsets or length are wrong is skipped, and a page that cannot be read reads
+ * as NaN; both set the status word. */
+typedef struct {
+  const int32_t* block_table; /* [batch][max_blocks], entries past a sequence's pages are not read */
+  int64_t table_stride;
+  const int32_t* kv_lens;     /* [batch] tokens of each sequence, this call's new ones included */
+  const int32_t* cu_rows;     /* [batch + 1] */
+  int64_t n_rows;
+  int32_t batch;
+  int32_t max_blocks;
+} noor_kv_batch;
+
+/* Write the batch's new tokens into the cache: row i of sequence b is its
+ * token kv_lens[b] - rows(b) + i.  With r, keys are rotated to that position
+ * first (in 64 bits, so the codes are those of the exact rotation); with q as
+ * well, q is rotated into q_out in the same launch (q [n_rows][q_heads],
+ * ignored without r).  k, v [n_rows][n_kv_heads].
+ * A block whose first token is new starts over (old contents ignored); a
+ * block that held tokens keeps its scale, or grows it and rounds its old codes
+ * again (ties to even).  A value that is not finite makes its block's scale
+ * NaN: every read of the block is NaN until it starts over.
+ * A page is written by one sequence at a time: two sequences of a batch, or
+ * two overlapping calls, must not append to the same page. */
+NOOR_MOE_API int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_heads* k,
+                                const noor_heads* v, const noor_rotary* r, const noor_heads* q,
+                                const noor_heads* q_out, int32_t q_heads, int32_t dtype, void* stream);
+
+/* Read tokens back: row i of sequence b is its token starts[b] + i (starts
+ * NULL: 0), k_out / v_out [n_rows][n_kv_heads][head_dim] contiguous.  Tokens
+ * must lie below kv_lens[b] (kv_lens NULL: within the sequence's pages). */
+NOOR_MOE_API int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* starts, void* k_out,
+                              void* v_out, int32_t dtype, void* stream);
+
+/* Causal attention of the batch's rows over the cache: row i of sequence b is
+ * a query at position p = kv_lens[b] - rows(b) + i and sees the tokens j <= p
+ * (window > 0: only p - j <= window, as attention.rs:133-136), query head h
+ * over kv head h / (q_heads / n_kv_heads).  out = softmax(scale q.k) v; a row
+ * that sees nothing gets zeros.  q, out [n_rows][q_heads] (they may be the
+ * same); lse [n_rows][q_heads] f32 contiguous, nullable: the natural
+ * logarithm of the sum of exponentials, -inf for a row that sees nothing.
+ * max_rows: the most rows of any sequence, a hint that picks the kernels (a
+ * wrong value costs time, not results).  The workspace, 16-byte aligned, of
+ * at least noor_kv_attention_workspace bytes for the same arguments, is free
+ * again when the call's work is done. */
+NOOR_MOE_API int noor_kv_attention_workspace(const noor_kv_cache* c, const noor_kv_batch* b, int32_t q_heads,
+                                             int32_t max_rows, int32_t dtype, int64_t* bytes);
+NOOR_MOE_API int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor_heads* q,
+                                   const noor_heads* out, float* lse, int32_t q_heads, int32_t max_rows, float scale,
+                                   int32_t window, int32_t dtype, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -44,6 +44,7 @@ EXPORTED_SYMBOLS = (
     "noor_moe_utilization", "noor_moe_smebu_update", "noor_moe_smebu_momentum", "noor_moe_get_bias",
     "noor_moe_ffn_sublayer_forward", "noor_moe_set_sandwich", "noor_moe_load_gguf", "noor_gguf_tensor_info",
     "noor_gguf_read_f32", "noor_moe_peer_plan",
+    "noor_rope_apply", "noor_kv_append", "noor_kv_read", "noor_kv_attention_workspace", "noor_kv_attention",
 )
 
 EP_TRANSPORTS = {0: "none", 1: "nccl", 2: "peer"}
@@ -63,6 +64,32 @@ class Desc(ctypes.Structure):
         ("device", ctypes.c_int32), ("world_size", ctypes.c_int32), ("rank", ctypes.c_int32),
         ("max_tokens", ctypes.c_int64),
     ]
+
+
+class Heads(ctypes.Structure):
+    """noor_heads: a [tokens][heads][head_dim] tensor with element strides."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """noor_rotary."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rotate_dim", ctypes.c_int32), ("layout", ctypes.c_int32),
+                ("factor", ctypes.c_float)]
+
+
+class KVCacheDesc(ctypes.Structure):
+    """noor_kv_cache."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("status", ctypes.c_void_p), ("num_blocks", ctypes.c_int64),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("block", ctypes.c_int32),
+                ("format", ctypes.c_int32), ("device", ctypes.c_int32)]
+
+
+class KVBatch(ctypes.Structure):
+    """noor_kv_batch."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("kv_lens", ctypes.c_void_p),
+                ("cu_rows", ctypes.c_void_p), ("n_rows", ctypes.c_int64), ("batch", ctypes.c_int32),
+                ("max_blocks", ctypes.c_int32)]
 
 
 _lib = None
@@ -115,6 +142,12 @@ def lib() -> ctypes.CDLL:
     L.noor_moe_peer_plan.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [_vp] * 7
     L.noor_moe_route_static.argtypes = [_vp, _vp, _vp, _vp, _i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                         ctypes.c_int32, _vp, _vp, _vp, _vp]
+    _i32 = ctypes.c_int32
+    L.noor_rope_apply.argtypes = [_vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _vp]
+    L.noor_kv_append.argtypes = [_vp] * 7 + [_i32, _i32, _vp]
+    L.noor_kv_read.argtypes = [_vp] * 5 + [_i32, _vp]
+    L.noor_kv_attention_workspace.argtypes = [_vp, _vp, _i32, _i32, _i32, _vp]
+    L.noor_kv_attention.argtypes = [_vp] * 5 + [_i32, _i32, ctypes.c_float, _i32, _i32, _vp, _i64, _vp]
     _lib = L
     return L
 

@@ -1,0 +1,366 @@
+"""The attention half of a block served from an 8-bit cache: rotary positions,
+the paged cache (write, read back) and attention over it.
+
+Torch tensors in and out over the C ABI's noor_rope_apply, noor_kv_append,
+noor_kv_read and noor_kv_attention (include/noor_moe.h states what each
+computes).  Every call runs on the tensors' device and on that device's
+current torch stream, allocates only through torch (so it can be captured into
+a CUDA graph) and never synchronises.  The reference's counterparts are
+RoPE::apply (crates/noor-core/src/layers/rope.rs:49-90) and
+GQAAttention::forward with its KV cache (attention.rs:67-191).
+
+There is no CPU fallback: tensors must be on a CUDA device.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import numpy as np
+
+from . import api
+
+LAYOUTS = {"interleaved": 0, "half": 1}
+FORMATS = {"int8": 0, "e4m3": 1}
+STATUS = {1: "row offsets are not ascending within the rows given",
+          2: "a length is negative, below the sequence's rows, or past its pages",
+          3: "a page number is outside the cache",
+          4: "a bounded wait on the device gave up"}
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _code_dtype(fmt: str):
+    torch = _torch()
+    return torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+
+
+def _dtype_code(t) -> int:
+    torch = _torch()
+    if t.dtype == torch.bfloat16:
+        return api.DTYPE_BF16
+    if t.dtype == torch.float32:
+        return api.DTYPE_F32
+    raise ValueError(f"expected bfloat16 or float32, got {t.dtype}")
+
+
+def _heads(t, what: str, dim: Optional[int] = None) -> api.Heads:
+    """noor_heads of a CUDA tensor [tokens, heads, head_dim]."""
+    if t.dim() != 3 or not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor [tokens, heads, head_dim], got {tuple(t.shape)} on {t.device}")
+    if dim is not None and t.shape[2] != dim:
+        raise ValueError(f"{what} has head_dim {t.shape[2]}, expected {dim}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{what}: a head's elements must be contiguous")
+    return api.Heads(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _int32(t, what: str, shape: Sequence[Optional[int]], device) -> int:
+    """Data pointer of an int32 tensor on `device`, its shape checked."""
+    torch = _torch()
+    if t.dtype != torch.int32 or t.device != device:
+        raise ValueError(f"{what} must be an int32 tensor on {device}, got {t.dtype} on {t.device}")
+    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.numel() > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what} must be contiguous along its last dimension")
+    return t.data_ptr()
+
+
+def _stream(device) -> int:
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
+
+
+# ------------------------------------------------------------ rotary
+
+
+def rotary_frequencies(head_dim: int, theta: float = 10000.0, fraction: Optional[float] = None, *,
+                       linear: float = 1.0, ntk: float = 1.0,
+                       yarn: Optional[dict] = None) -> Tuple[np.ndarray, float]:
+    """Inverse frequencies (f32) of the rotated pairs and the attention factor.
+
+    theta and fraction as RoPE::new / new_proportional (rope.rs:17-45).  For
+    contexts longer than the trained one, at most one of
+      linear  s: positions are divided by s;
+      ntk     s: theta grows by s^(rot / (rot - 2)), which leaves the fastest
+              pair as it is and divides the slowest by s;
+      yarn    {"scale": s, "original": trained context, "fast": 32, "slow": 1}:
+              pairs that turn more than `fast` times over the trained context
+              keep their frequency, those below `slow` turns are divided by s,
+              a linear ramp between (Peng et al., "YaRN", 2023); the factor is
+              0.1 ln s + 1.
+    """
+    rot = head_dim if fraction is None else max(2, (int(head_dim * fraction) // 2) * 2)
+    if rot > head_dim or rot % 2:
+        raise ValueError(f"cannot rotate {rot} of {head_dim} dims")
+    if sum((linear != 1.0, ntk != 1.0, yarn is not None)) > 1:
+        raise ValueError("at most one of linear, ntk and yarn")
+    if linear <= 0 or ntk <= 0 or (yarn is not None and yarn["scale"] <= 0):
+        raise ValueError("a scale must be positive")
+    if ntk != 1.0 and rot > 2:
+        theta = theta * ntk ** (rot / (rot - 2.0))
+    inv = theta ** (-2.0 * np.arange(rot // 2, dtype=np.float64) / rot) / linear
+    factor = 1.0
+    if yarn is not None:
+        s = float(yarn["scale"])
+        fast, slow = float(yarn.get("fast", 32.0)), float(yarn.get("slow", 1.0))
+        turns = float(yarn["original"]) * inv / (2.0 * math.pi)
+        keep = np.clip((turns - slow) / (fast - slow), 0.0, 1.0)
+        inv = inv / s * (1.0 - keep) + inv * keep
+        factor = 0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0
+    return inv.astype(np.float32), factor
+
+
+class Rotary:
+    """A table of inverse frequencies on a device, its layout and factor.
+
+    inv_freq: f32 tensor (or numpy array, uploaded to `device`) of rotate_dim / 2
+    frequencies; layout "interleaved" (pairs 2i, 2i + 1, the reference's) or
+    "half" (pairs i, i + rotate_dim / 2)."""
+
+    def __init__(self, inv_freq, layout: str = "interleaved", factor: float = 1.0, device: Union[int, str] = 0):
+        torch = _torch()
+        if layout not in LAYOUTS:
+            raise ValueError(f"unknown rotary layout {layout!r}")
+        if isinstance(inv_freq, np.ndarray):
+            inv_freq = torch.from_numpy(np.ascontiguousarray(inv_freq, np.float32)).to(torch.device("cuda", device) if isinstance(
+                device, int) else device)
+        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_cuda:
+            raise ValueError("inv_freq must be a 1-D float32 CUDA tensor")
+        self.inv_freq = inv_freq.contiguous()
+        self.rotate_dim = 2 * inv_freq.numel()
+        self.layout, self.factor = layout, float(factor)
+        self.desc = api.RotaryDesc(self.inv_freq.data_ptr(), self.rotate_dim, LAYOUTS[layout], self.factor)
+
+    @classmethod
+    def create(cls, head_dim: int, theta: float = 10000.0, fraction: Optional[float] = None,
+               layout: str = "interleaved", device: Union[int, str] = 0, **scaling) -> "Rotary":
+        inv, factor = rotary_frequencies(head_dim, theta, fraction, **scaling)
+        return cls(inv, layout, factor, device)
+
+
+def _rope_call(q, k, positions, rotary: Rotary, inverse: bool):
+    torch = _torch()
+    dt = _dtype_code(q)
+    D = q.shape[-1]
+    hq = _heads(q, "q")
+    if rotary.inv_freq.device != q.device:
+        raise ValueError(f"the rotary table is on {rotary.inv_freq.device}, q on {q.device}")
+    pos = _int32(positions, "positions", (q.shape[0],), q.device)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = hk = hk_out = None
+    if k is not None:
+        if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0]:
+            raise ValueError("k must have q's tokens, type and device")
+        hk = _heads(k, "k", D)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        hk_out = ctypes.byref(_heads(k_out, "k"))
+    api.check(api.lib().noor_rope_apply(
+        ctypes.byref(rotary.desc), ctypes.byref(hq), ctypes.byref(_heads(q_out, "q")), q.shape[1],
+        ctypes.byref(hk) if hk is not None else None, hk_out, k.shape[1] if k is not None else 0, pos, q.shape[0], D,
+        dt, int(inverse), q.device.index, _stream(q.device)))
+    return q_out, k_out
+
+
+_rope_function = None
+
+
+def _rope_autograd():
+    """The autograd function, made on first use (torch is imported lazily)."""
+    global _rope_function
+    if _rope_function is None:
+        torch = _torch()
+
+        class RopeFunction(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, q, k, positions, rotary):
+                ctx.rotary = rotary
+                ctx.set_materialize_grads(False)
+                ctx.save_for_backward(positions)
+                q_out, k_out = _rope_call(q, k, positions, rotary, False)
+                return q_out if k is None else (q_out, k_out)
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, gq, gk=None):
+                # the rotation's transpose; gradients may come broadcast
+                (positions,) = ctx.saved_tensors
+                gs = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (gq, gk)]
+                need = [g is not None and n for g, n in zip(gs, ctx.needs_input_grad)]
+                dq = dk = None
+                if need[0] and need[1]:
+                    dq, dk = _rope_call(gs[0], gs[1], positions, ctx.rotary, True)
+                elif need[0]:
+                    dq, _ = _rope_call(gs[0], None, positions, ctx.rotary, True)
+                elif need[1]:
+                    dk, _ = _rope_call(gs[1], None, positions, ctx.rotary, True)
+                return dq, dk, None, None
+
+        _rope_function = RopeFunction
+    return _rope_function
+
+
+def rope_apply(q, positions, rotary: Rotary, k=None):
+    """Rotate q [tokens, heads, head_dim] (and k beside it, in one launch) to
+    positions [tokens] (int32).  Differentiable in q and k; returns new tensors
+    q', or (q', k')."""
+    torch = _torch()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _rope_autograd().apply(q, k, positions, rotary)
+    q_out, k_out = _rope_call(q, k, positions, rotary, False)
+    return q_out if k is None else (q_out, k_out)
+
+
+# ------------------------------------------------------------ cache
+
+
+class KVCache:
+    """A paged cache of keys and values in 8 bits (noor_kv_cache).
+
+    A page holds `block` tokens of every kv head; k_codes [pages, kv heads,
+    block, head_dim], v_codes [pages, kv heads, head_dim, block], int8 or
+    float8_e4m3fn; k_scale and v_scale [pages, kv heads] f32.  The caller owns
+    the pages: block_table [batch, max_blocks] int32 names those of each
+    sequence, kv_lens [batch] int32 its tokens (a call's new ones included),
+    cu_rows [batch + 1] int32 the rows of each sequence in the row tensors;
+    all three stay on the device, so one captured graph serves changing
+    lengths.  Mistakes in them never reach memory outside the buffers: the
+    rows concerned are skipped or come back NaN, and check() raises."""
+
+    def __init__(self, num_blocks: int, n_kv_heads: int, head_dim: int, block: int = 64, fmt: str = "int8",
+                 device: int = 0):
+        torch = _torch()
+        if fmt not in FORMATS:
+            raise ValueError(f"unknown cache format {fmt!r}")
+        dev = torch.device("cuda", device)
+        z = lambda shape: torch.zeros(shape, dtype=torch.int8, device=dev).view(_code_dtype(fmt))
+        self._bind(z((num_blocks, n_kv_heads, block, head_dim)), z((num_blocks, n_kv_heads, head_dim, block)),
+                   torch.zeros((num_blocks, n_kv_heads), device=dev), torch.zeros((num_blocks, n_kv_heads), device=dev))
+
+    @classmethod
+    def from_tensors(cls, k_codes, v_codes, k_scale, v_scale) -> "KVCache":
+        """A cache over tensors the caller holds (kept, not copied)."""
+        c = cls.__new__(cls)
+        c._bind(k_codes, v_codes, k_scale, v_scale)
+        return c
+
+    def _bind(self, k_codes, v_codes, k_scale, v_scale) -> None:
+        torch = _torch()
+        if k_codes.dim() != 4 or not k_codes.is_cuda:
+            raise ValueError("k_codes must be a CUDA tensor [pages, kv heads, block, head_dim]")
+        P, H, blk, D = k_codes.shape
+        fmt = {torch.int8: "int8", torch.float8_e4m3fn: "e4m3"}.get(k_codes.dtype)
+        if fmt is None or v_codes.dtype != k_codes.dtype:
+            raise ValueError(f"codes must both be int8 or float8_e4m3fn, got {k_codes.dtype} and {v_codes.dtype}")
+        for name, t, shape in (("v_codes", v_codes, (P, H, D, blk)), ("k_scale", k_scale, (P, H)),
+                               ("v_scale", v_scale, (P, H))):
+            if tuple(t.shape) != shape or t.device != k_codes.device:
+                raise ValueError(f"{name} must have shape {shape} on {k_codes.device}")
+        for name, t in (("k_codes", k_codes), ("v_codes", v_codes), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if name.endswith("scale") and t.dtype != torch.float32:
+                raise ValueError(f"{name} must be float32")
+        self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
+        self.num_blocks, self.n_kv_heads, self.block, self.head_dim = P, H, blk, D
+        self.format, self.device = fmt, k_codes.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.desc = api.KVCacheDesc(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                    self.status.data_ptr(), P, H, D, blk, FORMATS[fmt], self.device.index)
+
+    def check(self) -> None:
+        """Wait for the device and raise NoorMoEError if a kernel found a
+        mistake in device metadata since the last check; clears it."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            raise api.NoorMoEError(6 if code == 4 else 1, f"cache: {STATUS.get(code, code)}")
+
+    def _batch(self, block_table, kv_lens, cu_rows, rows: int) -> api.KVBatch:
+        table = _int32(block_table, "block_table", (None, None), self.device)
+        B = block_table.shape[0]
+        lens = _int32(kv_lens, "kv_lens", (B,), self.device) if kv_lens is not None else None
+        cu = _int32(cu_rows, "cu_rows", (B + 1,), self.device)
+        return api.KVBatch(table, block_table.stride(0), lens, cu, rows, B, block_table.shape[1])
+
+    def _rows(self, t, what: str, like=None) -> api.Heads:
+        if t.device != self.device:
+            raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
+        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
+            raise ValueError(f"{what} must have the other rows' number and type")
+        return _heads(t, what, self.head_dim)
+
+    def append(self, k, v, block_table, kv_lens, cu_rows, rotary: Optional[Rotary] = None, q=None):
+        """Write the new tokens' k and v [rows, kv heads, head_dim]; row i of
+        sequence b is its token kv_lens[b] - rows(b) + i.  With `rotary`, keys
+        are rotated to their positions first, and q [rows, heads, head_dim]
+        beside them: the rotated q is returned (rows past the last sequence's are
+        undefined), else None."""
+        torch = _torch()
+        dt = _dtype_code(k)
+        hk, hv = self._rows(k, "k"), self._rows(v, "v", k)
+        if k.shape[1] != self.n_kv_heads or v.shape[1] != self.n_kv_heads:
+            raise ValueError(f"k and v must have {self.n_kv_heads} heads")
+        if q is not None and rotary is None:
+            raise ValueError("q is rotated beside the write: it needs `rotary`")
+        if rotary is not None and rotary.inv_freq.device != self.device:
+            raise ValueError(f"the rotary table is on {rotary.inv_freq.device}, the cache on {self.device}")
+        batch = self._batch(block_table, kv_lens, cu_rows, k.shape[0])
+        q_out = hq = hq_out = None
+        if q is not None:
+            hq = ctypes.byref(self._rows(q, "q", k))
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            hq_out = ctypes.byref(_heads(q_out, "q"))
+        api.check(api.lib().noor_kv_append(
+            ctypes.byref(self.desc), ctypes.byref(batch), ctypes.byref(hk), ctypes.byref(hv),
+            ctypes.byref(rotary.desc) if rotary is not None else None, hq, hq_out, q.shape[1] if q is not None else 0,
+            dt, _stream(self.device)))
+        return q_out
+
+    def read(self, block_table, starts, cu_rows, rows: int, dtype=None, kv_lens=None):
+        """Tokens read back: row i of sequence b is its token starts[b] + i
+        (starts None: from 0).  rows: rows of the result, at least cu_rows[-1].
+        kv_lens bounds the tokens (None: the tables' whole width).  Returns k, v
+        [rows, kv heads, head_dim] in `dtype` (bfloat16 by default)."""
+        torch = _torch()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        out = [torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
+        dt = _dtype_code(out[0])
+        batch = self._batch(block_table, kv_lens, cu_rows, rows)
+        st = _int32(starts, "starts", (batch.batch,), self.device) if starts is not None else None
+        api.check(api.lib().noor_kv_read(ctypes.byref(self.desc), ctypes.byref(batch), st, out[0].data_ptr(),
+                                         out[1].data_ptr(), dt, _stream(self.device)))
+        return out[0], out[1]
+
+    def attention(self, q, block_table, kv_lens, cu_rows, max_rows: int, scale: Optional[float] = None,
+                  window: int = 0, out=None, return_lse: bool = False):
+        """Causal attention of q [rows, heads, head_dim] over the cache: row i
+        of sequence b is at position kv_lens[b] - rows(b) + i.  max_rows: the
+        most rows of a sequence (a hint).  window > 0: keys at most `window`
+        positions back.  scale: 1 / sqrt(head_dim) by default.  Returns out, or
+        (out, lse) with lse [rows, heads] f32.  `out` may be q."""
+        torch = _torch()
+        dt = _dtype_code(q)
+        hq = self._rows(q, "q")
+        if q.shape[1] % self.n_kv_heads != 0:
+            raise ValueError(f"{q.shape[1]} query heads over {self.n_kv_heads} kv heads")
+        batch = self._batch(block_table, kv_lens, cu_rows, q.shape[0])
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        ho = self._rows(out, "out", q)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        need = ctypes.c_int64()
+        args = (ctypes.byref(self.desc), ctypes.byref(batch))
+        api.check(api.lib().noor_kv_attention_workspace(*args, q.shape[1], max_rows, dt, ctypes.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        api.check(api.lib().noor_kv_attention(
+            *args, ctypes.byref(hq), ctypes.byref(ho), lse.data_ptr() if lse is not None else None, q.shape[1], max_rows,
+            float(self.head_dim) ** -0.5 if scale is None else float(scale), window, dt, ws.data_ptr(), need.value,
+            _stream(self.device)))
+        return (out, lse) if return_lse else out

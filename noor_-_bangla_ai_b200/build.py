@@ -21,7 +21,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnoor_moe.so")
 LIB_CHECK = os.path.join(HERE, "libnoor_moe_check.so")
-SOURCES = ["noor_moe.cu"]
+SOURCES = ["noor_moe.cu", "noor_attention.cu"]
 
 
 def headers() -> list:

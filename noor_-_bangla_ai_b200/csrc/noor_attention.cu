@@ -1,0 +1,399 @@
+// noor_attention.cu -- C ABI of the attention half of a block: rotary
+// positions, the paged 8-bit cache (write, read back) and attention over it.
+// Every entry point checks its host arguments, sets the device for the call,
+// enqueues on the caller's stream and allocates nothing.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <exception>
+
+#include "noor_moe.h"
+
+#include "common.cuh"
+#include "host.h"
+#include "kv_attention.cuh"
+#include "kv_cache.cuh"
+#include "rope.cuh"
+
+using namespace noor;
+
+namespace {
+
+// C callers never see an exception.
+template <typename F>
+int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return NOOR_MOE_ERR_OOM;
+  } catch (...) {
+    return NOOR_MOE_ERR_OOM;
+  }
+}
+
+int check_device(int dev) {
+  int n = 0;
+  CK(cudaGetDeviceCount(&n));
+  if (dev < 0 || dev >= n) return fail(NOOR_MOE_ERR_INVALID, "device %d not in 0 .. %d", dev, n - 1);
+  return NOOR_MOE_OK;
+}
+
+// Streaming multiprocessors of a device (looked up once).
+int sm_count(int dev, int* out) {
+  static std::mutex mu;
+  static int known[64] = {0};
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 64 && known[dev]) {
+    *out = known[dev];
+    return NOOR_MOE_OK;
+  }
+  CK(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev] = *out;
+  return NOOR_MOE_OK;
+}
+
+int check_dtype(int dtype) {
+  if (dtype != NOOR_DTYPE_F32 && dtype != NOOR_DTYPE_BF16) return fail(NOOR_MOE_ERR_INVALID, "unknown dtype %d", dtype);
+  return NOOR_MOE_OK;
+}
+
+size_t esize(int dtype) { return dtype == NOOR_DTYPE_BF16 ? 2 : 4; }
+
+int check_rotary(const noor_rotary* r, int D) {
+  if (r->rotate_dim < 0 || r->rotate_dim % 2 != 0 || r->rotate_dim > D)
+    return fail(NOOR_MOE_ERR_INVALID, "rotate_dim %d is not an even number in 0 .. %d", r->rotate_dim, D);
+  if (r->layout != NOOR_ROPE_INTERLEAVED && r->layout != NOOR_ROPE_HALF)
+    return fail(NOOR_MOE_ERR_INVALID, "unknown rotary layout %d", r->layout);
+  if (r->rotate_dim > 0 && !r->inv_freq) return fail(NOOR_MOE_ERR_INVALID, "null inv_freq");
+  return NOOR_MOE_OK;
+}
+
+int check_view(const noor_heads* v, int dtype, const char* what) {
+  if (!v || !v->data) return fail(NOOR_MOE_ERR_INVALID, "null %s", what);
+  if (reinterpret_cast<uintptr_t>(v->data) % esize(dtype) != 0)
+    return fail(NOOR_MOE_ERR_INVALID, "%s is not aligned to its elements", what);
+  return NOOR_MOE_OK;
+}
+
+rope::View view(const noor_heads* v) {
+  return v ? rope::View{v->data, v->token_stride, v->head_stride} : rope::View{nullptr, 0, 0};
+}
+
+bool vector_rows(const rope::View& v, int dtype) {
+  const size_t e = esize(dtype);
+  return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.st * (int64_t)e % 16 == 0 && v.sh * (int64_t)e % 16 == 0;
+}
+
+// 16-byte vectors fit the heads of `views` and the rotary layout.
+bool vector_heads(const rope::Args& a, int dtype, std::initializer_list<rope::View> views) {
+  const int n = 16 / (int)esize(dtype);
+  if (a.D % n != 0 || (a.layout == rope::HALF && a.rot / 2 % n != 0)) return false;
+  for (const auto& v : views)
+    if (v.p && !vector_rows(v, dtype)) return false;
+  return true;
+}
+
+template <typename F>
+int by_dtype(int dtype, F&& f) {
+  return dtype == NOOR_DTYPE_BF16 ? f(bf16{}) : f(float{});
+}
+
+int check_cache(const noor_kv_cache* c) {
+  if (!c) return fail(NOOR_MOE_ERR_INVALID, "null cache");
+  CKR(check_device(c->device));
+  if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale) return fail(NOOR_MOE_ERR_INVALID, "null cache array");
+  for (const void* p : {(const void*)c->k_codes, (const void*)c->v_codes, (const void*)c->k_scale, (const void*)c->v_scale})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return fail(NOOR_MOE_ERR_INVALID, "cache arrays must be 16-byte aligned");
+  if (c->block != 16 && c->block != 32 && c->block != 64)
+    return fail(NOOR_MOE_ERR_UNSUPPORTED, "block %d is not 16, 32 or 64", c->block);
+  if (c->head_dim <= 0 || c->head_dim % 16 != 0 || c->head_dim > 256)
+    return fail(NOOR_MOE_ERR_UNSUPPORTED, "head_dim %d is not a multiple of 16 up to 256", c->head_dim);
+  if (c->format != NOOR_KV_INT8 && c->format != NOOR_KV_E4M3)
+    return fail(NOOR_MOE_ERR_INVALID, "unknown cache format %d", c->format);
+  if (c->num_blocks <= 0 || c->num_blocks > INT32_MAX || c->n_kv_heads <= 0 || c->n_kv_heads > 4096)
+    return fail(NOOR_MOE_ERR_INVALID, "num_blocks or n_kv_heads out of range");
+  return NOOR_MOE_OK;
+}
+
+int check_batch(const noor_kv_cache* c, const noor_kv_batch* b, bool need_lens = true) {
+  if (!b || !b->block_table || (need_lens && !b->kv_lens) || !b->cu_rows) return fail(NOOR_MOE_ERR_INVALID, "null batch argument");
+  if (b->batch <= 0 || b->batch > (1 << 20)) return fail(NOOR_MOE_ERR_INVALID, "batch %d out of range", b->batch);
+  if (b->n_rows < 0 || b->n_rows > (1 << 28)) return fail(NOOR_MOE_ERR_INVALID, "n_rows out of range");
+  if (b->max_blocks <= 0 || (int64_t)b->max_blocks * c->block > (1 << 30) || b->table_stride < 0)
+    return fail(NOOR_MOE_ERR_INVALID, "max_blocks or table_stride out of range");
+  return NOOR_MOE_OK;
+}
+
+kv::Cache cache_of(const noor_kv_cache* c) {
+  return kv::Cache{static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->v_codes), c->k_scale, c->v_scale,
+                   c->status, c->num_blocks, c->n_kv_heads, c->head_dim, c->block};
+}
+
+kv::Batch batch_of(const noor_kv_batch* b) {
+  return kv::Batch{b->block_table, b->table_stride, b->kv_lens, b->cu_rows, b->n_rows, b->batch, b->max_blocks};
+}
+
+// The most blocks that a batch's rows can touch: each sequence with n rows
+// touches at most (n - 1) / block + 2 of them and at most n.
+int64_t most_tasks(const noor_kv_cache* c, const noor_kv_batch* b) {
+  return std::min<int64_t>(b->n_rows, b->n_rows / c->block + 2 * std::min<int64_t>(b->batch, b->n_rows));
+}
+
+}  // namespace
+
+extern "C" {
+
+int noor_rope_apply(const noor_rotary* r, const noor_heads* q, const noor_heads* q_out, int32_t q_heads,
+                    const noor_heads* k, const noor_heads* k_out, int32_t k_heads, const int32_t* positions,
+                    int64_t tokens, int32_t head_dim, int32_t dtype, int32_t inverse, int32_t device, void* stream) {
+  return guarded([&]() -> int {
+    if (!r) return fail(NOOR_MOE_ERR_INVALID, "null rotary");
+    CKR(check_dtype(dtype));
+    if (head_dim <= 0 || head_dim % 2 != 0 || head_dim > 1024)
+      return fail(NOOR_MOE_ERR_UNSUPPORTED, "head_dim %d is not an even number up to 1024", head_dim);
+    CKR(check_rotary(r, head_dim));
+    if (tokens < 0 || tokens > (1 << 28) || q_heads <= 0 || q_heads > 4096 || (k && (k_heads <= 0 || k_heads > 4096)))
+      return fail(NOOR_MOE_ERR_INVALID, "tokens or heads out of range");
+    if (tokens == 0) return NOOR_MOE_OK;
+    CKR(check_view(q, dtype, "q"));
+    CKR(check_view(q_out, dtype, "q_out"));
+    if (k) CKR(check_view(k, dtype, "k"));
+    if (k) CKR(check_view(k_out, dtype, "k_out"));
+    if (!positions) return fail(NOOR_MOE_ERR_INVALID, "null positions");
+    CKR(check_device(device));
+    DeviceGuard g(device);
+    rope::Args a{r->inv_freq, r->rotate_dim, r->layout, r->factor, inverse ? -1.f : 1.f, view(q), view(q_out),
+                 view(k), view(k ? k_out : nullptr), q_heads, k ? k_heads : 0, head_dim, positions, tokens};
+    const int tok = 4;
+    const unsigned grid = (unsigned)((tokens + tok - 1) / tok);
+    const size_t smem = (size_t)tok * (r->rotate_dim / 2) * sizeof(float2);
+    const bool vec = vector_heads(a, dtype, {a.q, a.q_out, a.k, a.k_out});
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return by_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      if (vec)
+        rope::rope_kernel<T, true><<<grid, 256, smem, s>>>(a, tok);
+      else
+        rope::rope_kernel<T, false><<<grid, 256, smem, s>>>(a, tok);
+      CK(cudaGetLastError());
+      return NOOR_MOE_OK;
+    });
+  });
+}
+
+int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_heads* k, const noor_heads* v,
+                   const noor_rotary* r, const noor_heads* q, const noor_heads* q_out, int32_t q_heads, int32_t dtype,
+                   void* stream) {
+  return guarded([&]() -> int {
+    CKR(check_cache(c));
+    CKR(check_batch(c, b));
+    CKR(check_dtype(dtype));
+    if (r) CKR(check_rotary(r, c->head_dim));
+    if (!r) q = nullptr;
+    if (b->n_rows == 0) return NOOR_MOE_OK;
+    CKR(check_view(k, dtype, "k"));
+    CKR(check_view(v, dtype, "v"));
+    if (q) {
+      CKR(check_view(q, dtype, "q"));
+      CKR(check_view(q_out, dtype, "q_out"));
+      if (q_heads <= 0 || q_heads > 4096) return fail(NOOR_MOE_ERR_INVALID, "q_heads %d out of range", q_heads);
+    }
+    DeviceGuard g(c->device);
+    kv::AppendArgs a{};
+    a.c = cache_of(c);
+    a.b = batch_of(b);
+    a.k = view(k);
+    a.v = view(v);
+    a.r.D = c->head_dim;
+    a.r.factor = 1.f;
+    if (r) {
+      a.r.inv_freq = r->inv_freq;
+      a.r.rot = r->rotate_dim;
+      a.r.layout = r->layout;
+      a.r.factor = r->factor;
+    }
+    a.r.q = view(q);
+    a.r.q_out = view(q ? q_out : nullptr);
+    a.r.hq = q ? q_heads : 0;
+    a.q_tok = 4;
+    const int64_t kvb = most_tasks(c, b) * c->n_kv_heads, qb = q ? (b->n_rows + a.q_tok - 1) / a.q_tok : 0;
+    if (kvb + qb > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
+    a.kv_blocks = (int32_t)kvb;
+    const bool vec = !q || vector_heads(a.r, dtype, {a.r.q, a.r.q_out});
+    const int smem = (int)std::max<size_t>((size_t)c->block * c->head_dim * (esize(dtype) + 1),
+                                           (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return by_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      auto go = [&](auto kern) -> int {
+        // the kernel's static arrays count against the 48 KB too
+        CKR(ensure_smem_limit(kern, smem > 47 * 1024 ? std::max(smem, 48 * 1024 + 1) : smem));
+        kern<<<(unsigned)(kvb + qb), kv::kAppendThreads, smem, s>>>(a);
+        CK(cudaGetLastError());
+        return NOOR_MOE_OK;
+      };
+      if (c->format == NOOR_KV_INT8)
+        return vec ? go(kv::append_kernel<T, kv::INT8, true>) : go(kv::append_kernel<T, kv::INT8, false>);
+      return vec ? go(kv::append_kernel<T, kv::E4M3, true>) : go(kv::append_kernel<T, kv::E4M3, false>);
+    });
+  });
+}
+
+int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* starts, void* k_out, void* v_out,
+                 int32_t dtype, void* stream) {
+  return guarded([&]() -> int {
+    CKR(check_cache(c));
+    CKR(check_batch(c, b, false));
+    CKR(check_dtype(dtype));
+    if (b->n_rows == 0) return NOOR_MOE_OK;
+    if (!k_out || !v_out) return fail(NOOR_MOE_ERR_INVALID, "null output");
+    if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
+      return fail(NOOR_MOE_ERR_INVALID, "outputs must be 16-byte aligned");
+    DeviceGuard g(c->device);
+    const kv::ReadArgs a{cache_of(c), batch_of(b), starts, k_out, v_out};
+    const int64_t grid = most_tasks(c, b) * c->n_kv_heads;
+    if (grid > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return by_dtype(dtype, [&](auto t) -> int {
+      using T = decltype(t);
+      if (c->format == NOOR_KV_INT8)
+        kv::read_kernel<T, kv::INT8><<<(unsigned)grid, 256, 0, s>>>(a);
+      else
+        kv::read_kernel<T, kv::E4M3><<<(unsigned)grid, 256, 0, s>>>(a);
+      CK(cudaGetLastError());
+      return NOOR_MOE_OK;
+    });
+  });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------- attention
+
+namespace {
+
+struct StreamPlan {
+  int grid = 0, warps = 0;
+  int64_t off_ml = 0, off_desc = 0, bytes = 0;
+};
+
+int warps_per_block(int D, int dtype) {
+  const bool f32 = dtype == NOOR_DTYPE_F32;
+  if (D <= 64) return f32 ? attn::Shape<64, 2>::kWarps : attn::Shape<64, 1>::kWarps;
+  if (D <= 128) return f32 ? attn::Shape<128, 2>::kWarps : attn::Shape<128, 1>::kWarps;
+  return f32 ? attn::Shape<256, 2>::kWarps : attn::Shape<256, 1>::kWarps;
+}
+
+// Grid of the streamed kernel: one block per SM, fewer where the batch cannot
+// have that many tiles.
+int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int dtype, StreamPlan* p) {
+  int sms = 0;
+  CKR(sm_count(c->device, &sms));
+  const int64_t g = Hq / c->n_kv_heads, per = warps_per_block(c->head_dim, dtype);
+  const int64_t rtiles = std::min(b->n_rows * g, b->n_rows * g / 16 + b->batch);
+  const int64_t tiles = ((int64_t)b->max_blocks * c->block + attn::kTile - 1) / attn::kTile;
+  const double most = (double)rtiles * c->n_kv_heads * tiles;
+  p->grid = (int)std::min<double>(sms, std::max(1.0, most));
+  p->warps = p->grid * (int)per;
+  p->off_ml = (int64_t)p->warps * 2 * 16 * c->head_dim * 4;
+  p->off_desc = p->off_ml + (int64_t)p->warps * 2 * 32 * 4;
+  p->bytes = p->off_desc + (int64_t)p->warps * 16;
+  return NOOR_MOE_OK;
+}
+
+int check_heads(const noor_kv_cache* c, int Hq) {
+  if (Hq <= 0 || Hq > 65536 || Hq % c->n_kv_heads != 0)
+    return fail(NOOR_MOE_ERR_INVALID, "%d query heads over %d kv heads", Hq, c->n_kv_heads);
+  return NOOR_MOE_OK;
+}
+
+template <int DP, int FMT, int PARTS>
+int launch_stream(const attn::Args& a, int grid, cudaStream_t s) {
+  using Sh = attn::Shape<DP, PARTS>;
+  auto kern = attn::stream_kernel<DP, FMT, PARTS>;
+  const int smem = Sh::smem_bytes(a.c.D);
+  CKR(ensure_smem_limit(kern, smem));
+  kern<<<grid, Sh::kWarps * 32, smem, s>>>(a);
+  CK(cudaGetLastError());
+  return NOOR_MOE_OK;
+}
+
+template <int FMT, int PARTS>
+int launch_stream_d(const attn::Args& a, int grid, cudaStream_t s) {
+  if (a.c.D <= 64) return launch_stream<64, FMT, PARTS>(a, grid, s);
+  if (a.c.D <= 128) return launch_stream<128, FMT, PARTS>(a, grid, s);
+  return launch_stream<256, FMT, PARTS>(a, grid, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int noor_kv_attention_workspace(const noor_kv_cache* c, const noor_kv_batch* b, int32_t q_heads, int32_t max_rows,
+                                int32_t dtype, int64_t* bytes) {
+  return guarded([&]() -> int {
+    CKR(check_cache(c));
+    CKR(check_batch(c, b));
+    CKR(check_dtype(dtype));
+    CKR(check_heads(c, q_heads));
+    if (!bytes || max_rows < 0) return fail(NOOR_MOE_ERR_INVALID, "null bytes or negative max_rows");
+    StreamPlan p;
+    CKR(stream_plan(c, b, q_heads, dtype, &p));
+    *bytes = p.bytes;
+    return NOOR_MOE_OK;
+  });
+}
+
+int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor_heads* q, const noor_heads* out,
+                      float* lse, int32_t q_heads, int32_t max_rows, float scale, int32_t window, int32_t dtype,
+                      void* workspace, int64_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    CKR(check_cache(c));
+    CKR(check_batch(c, b));
+    CKR(check_dtype(dtype));
+    CKR(check_heads(c, q_heads));
+    if (max_rows < 0 || window < 0) return fail(NOOR_MOE_ERR_INVALID, "negative max_rows or window");
+    if (!std::isfinite(scale)) return fail(NOOR_MOE_ERR_INVALID, "scale is not finite");
+    if (b->n_rows == 0) return NOOR_MOE_OK;
+    CKR(check_view(q, dtype, "q"));
+    CKR(check_view(out, dtype, "out"));
+    StreamPlan p;
+    CKR(stream_plan(c, b, q_heads, dtype, &p));
+    if (!workspace || workspace_bytes < p.bytes)
+      return fail(NOOR_MOE_ERR_INVALID, "workspace of %lld bytes, needs %lld", (long long)workspace_bytes,
+                  (long long)p.bytes);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+      return fail(NOOR_MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+    DeviceGuard g(c->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    attn::Args a{};
+    a.c = cache_of(c);
+    a.b = batch_of(b);
+    a.q = view(q);
+    a.out = view(out);
+    a.lse = lse;
+    a.Hq = q_heads;
+    a.g = q_heads / c->n_kv_heads;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.window = window;
+    a.warps = p.warps;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + p.off_ml);
+    a.desc = reinterpret_cast<int4*>(ws + p.off_desc);
+    if (dtype == NOOR_DTYPE_BF16)
+      CKR((c->format == NOOR_KV_INT8 ? launch_stream_d<kv::INT8, 1>(a, p.grid, s) : launch_stream_d<kv::E4M3, 1>(a, p.grid, s)));
+    else
+      CKR((c->format == NOOR_KV_INT8 ? launch_stream_d<kv::INT8, 2>(a, p.grid, s) : launch_stream_d<kv::E4M3, 2>(a, p.grid, s)));
+    return by_dtype(dtype, [&](auto t) -> int {
+      const int64_t rows = std::min<int64_t>(16, b->n_rows * a.g);
+      attn::combine_kernel<decltype(t)><<<dim3((unsigned)p.warps, (unsigned)rows), 128, 0, s>>>(a);
+      CK(cudaGetLastError());
+      return NOOR_MOE_OK;
+    });
+  });
+}
+
+}  // extern "C"

@@ -40,6 +40,7 @@
 #include "common.cuh"
 #include "gguf.h"
 #include "dispatch.cuh"
+#include "host.h"
 #include "nccl_dyn.h"
 #include "norm.cuh"
 #include "peer_ep.cuh"
@@ -56,7 +57,7 @@ using namespace noor;
 
 static thread_local std::string g_last_error;
 
-static int fail(int code, const char* fmt, ...) {
+int noor::fail(int code, const char* fmt, ...) {
   char buf[1024];
   va_list ap;
   va_start(ap, fmt);
@@ -66,19 +67,6 @@ static int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-// A failed runtime call is reported by the call that made it; the runtime's
-// last-error state is cleared so that it does not resurface as the launch
-// error of a later, unrelated call (faults that poison the context stay).
-#define CK(call)                                                                                       \
-  do {                                                                                                 \
-    cudaError_t e_ = (call);                                                                           \
-    if (e_ != cudaSuccess) {                                                                           \
-      (void)cudaGetLastError();                                                                        \
-      return fail(e_ == cudaErrorMemoryAllocation ? NOOR_MOE_ERR_OOM : NOOR_MOE_ERR_CUDA,              \
-                  "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__);                \
-    }                                                                                                  \
-  } while (0)
-
 #define CKN(call)                                                                                      \
   do {                                                                                                 \
     if (!noor::nccl().ok) return fail(NOOR_MOE_ERR_NCCL, "libnccl.so.2 could not be loaded");          \
@@ -86,12 +74,6 @@ static int fail(int code, const char* fmt, ...) {
     if (r_ != ncclSuccess)                                                                             \
       return fail(NOOR_MOE_ERR_NCCL, "%s: %s (%s:%d)", #call, noor::nccl().GetErrorString(r_),         \
                   __FILE__, __LINE__);                                                                 \
-  } while (0)
-
-#define CKR(call)               \
-  do {                          \
-    int rc_ = (call);           \
-    if (rc_ != NOOR_MOE_OK) return rc_; \
   } while (0)
 
 // ============================================================== device buffers
@@ -329,19 +311,6 @@ extern "C" int noor_moe_ep_plan(const int64_t* counts_local, const int64_t* coun
 
 namespace {
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
 // Launch wrapper: names the launch with an NVTX range (seen by ncu / nsys;
 // a no-op without a tool attached), brackets it with profile events when
 // enabled and counts it.
@@ -534,36 +503,6 @@ void set_peer_out(tc::Params& p, const PeerOut* po) {
   if (po->bases)
     for (int r = 0; r < noor::peer::kMaxRanks; ++r) p.out_peer[r] = po->bases[r];
   p.out_rowmap = po->rowmap;
-}
-
-// Raise a kernel's dynamic shared-memory limit to at least `bytes`.  Up to
-// 48 KB needs no attribute; above it the limit set so far for each
-// (kernel, device) is remembered, so the slow host call runs only when a
-// launch needs more than before.
-template <typename K>
-int ensure_smem_limit(K kern, int bytes) {
-  if (bytes <= 48 * 1024) return NOOR_MOE_OK;
-  static std::mutex mu;
-  struct Entry {
-    const void* kern;
-    int dev;
-    int bytes;
-  };
-  static std::vector<Entry> done;
-  int dev = 0;
-  CK(cudaGetDevice(&dev));
-  const void* key = reinterpret_cast<const void*>(kern);
-  std::lock_guard<std::mutex> lock(mu);
-  for (auto& e : done)
-    if (e.kern == key && e.dev == dev) {
-      if (e.bytes >= bytes) return NOOR_MOE_OK;
-      CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-      e.bytes = bytes;
-      return NOOR_MOE_OK;
-    }
-  CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.push_back({key, dev, bytes});
-  return NOOR_MOE_OK;
 }
 
 // c_rows: rows the output buffer(s) hold, for the bounds checks of the

@@ -1,0 +1,352 @@
+"""GPU: the attention half served from the 8-bit cache (attention.py over
+noor_rope_apply, noor_kv_append, noor_kv_read, noor_kv_attention) against its
+plain 64-bit form (tests/attention_ref.py).
+
+Tolerances, fixed before the first run:
+  rotary      own rounding (BF16 2^-8, F32 2^-24 of the value) + 10 * 2^-24 (|x0| + |x1|) |factor|:
+              the angle's fraction in f32 (3.2 units), sine and cosine (2), products and sum (3)
+  cache       scales and codes equal; values read back equal (BF16 holds 8-bit codes times a power of two)
+  attention   attention_ref.attend_tolerance
+"""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+i32 = lambda xs: torch.tensor(xs, dtype=torch.int32, device="cuda")
+
+
+def cu_of(counts):
+    return i32([0] + np.cumsum(counts).tolist())
+
+
+def randn(shape, seed, dtype=torch.float32, gain=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * gain).to(dtype)
+
+
+# ---------------------------------------------------------------- rotary
+
+
+def check_rope(got, x, pos, inv, layout, factor, sign=1.0):
+    want = ref.rotate(x, pos, inv, layout, factor, sign)
+    own = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+    half = inv.numel()
+    pair = torch.zeros_like(want)
+    if half:
+        i0, i1 = ((torch.arange(half) * 2, torch.arange(half) * 2 + 1) if layout == "interleaved" else
+                  (torch.arange(half), torch.arange(half) + half))
+        pair[..., i0] = pair[..., i1] = x.double()[..., i0].abs() + x.double()[..., i1].abs()
+    tol = own * want.abs() + 10 * 2.0 ** -24 * pair * abs(factor) * (1 + own) + 1e-38
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+    assert torch.equal(got.cpu()[..., 2 * half:], x[..., 2 * half:].to(got.dtype))  # the rest passes unchanged
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("T,Hq,Hk,D,rot,start", [(1, 1, 0, 2, 2, 0), (1, 32, 8, 128, 128, 2 ** 31 - 1), (7, 4, 2, 64, 16, 10 ** 6),
+                                                 (5, 3, 1, 80, 20, 77), (33, 2, 2, 48, 0, 5), (130, 9, 3, 256, 256, 131072),
+                                                 (3, 2, 1, 18, 6, -9), (64, 1, 1, 1024, 1024, 4)])
+def test_rope(pkg, cuda_device, dtype, layout, T, Hq, Hk, D, rot, start):
+    A = pkg.attention
+    inv = torch.from_numpy((10000.0 ** (-2.0 * np.arange(rot // 2) / max(rot, 1))).astype(np.float32))
+    r = A.Rotary(inv.cuda(), layout, 1.25)
+    pos = torch.clamp(torch.arange(T) + start, max=2 ** 31 - 1).to(torch.int32)
+    q, k = randn((T, Hq, D), 1, DT[dtype]), randn((T, max(Hk, 1), D), 2, DT[dtype])
+    if Hk:
+        gq, gk = A.rope_apply(q.cuda(), pos.cuda(), r, k=k.cuda())
+        check_rope(gk, k, pos, inv, layout, 1.25)
+    else:
+        gq = A.rope_apply(q.cuda(), pos.cuda(), r)
+    check_rope(gq, q, pos, inv, layout, 1.25)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rope_views_and_unaligned(pkg, cuda_device, dtype):
+    """q and k as slices of one fused tensor, heads outermost, a broadcast
+    token and a base off by one element."""
+    A = pkg.attention
+    inv, _ = A.rotary_frequencies(64, 10000.0, 0.5)
+    inv = torch.from_numpy(inv)
+    r = A.Rotary(inv.numpy(), "half", device=0)
+    T = 9
+    pos = torch.randint(0, 50000, (T,), generator=torch.Generator().manual_seed(3)).to(torch.int32)
+    fused = randn((T, 7, 64), 4, DT[dtype])
+    f = fused.cuda()
+    gq, gk = A.rope_apply(f[:, :4], pos.cuda(), r, k=f[:, 4:6])
+    check_rope(gq, fused[:, :4], pos, inv, "half", 1.0)
+    check_rope(gk, fused[:, 4:6], pos, inv, "half", 1.0)
+    heads_first = f.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(A.rope_apply(heads_first, pos.cuda(), r), A.rope_apply(f, pos.cuda(), r))
+    one = f[:1].expand(T, 7, 64)
+    check_rope(A.rope_apply(one, pos.cuda(), r), fused[:1].expand(T, 7, 64), pos, inv, "half", 1.0)
+    flat = torch.empty(T * 7 * 64 + 1, dtype=DT[dtype], device="cuda")
+    off = flat[1:].view(T, 7, 64)
+    off.copy_(f)
+    check_rope(A.rope_apply(off, pos.cuda(), r), fused, pos, inv, "half", 1.0)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_gradient(pkg, cuda_device, layout):
+    """The gradient is the transposed rotation; checked against the formula,
+    against differences, and for gradients that arrive broadcast."""
+    A = pkg.attention
+    inv, factor = A.rotary_frequencies(32, 10000.0, 0.75, yarn={"scale": 4.0, "original": 2048})
+    r = A.Rotary(inv, layout, factor)
+    inv = torch.from_numpy(inv)
+    pos = i32([5, 0, 4096])
+    q, k = randn((3, 2, 32), 5).cuda().requires_grad_(), randn((3, 1, 32), 6).cuda().requires_grad_()
+    wq, wk = randn((3, 2, 32), 7), randn((3, 1, 32), 8)
+    oq, ok = A.rope_apply(q, pos, r, k=k)
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (wq.cuda(), wk.cuda()))
+    check_rope(dq, wq, pos.cpu(), inv, layout, factor, -1.0)
+    check_rope(dk, wk, pos.cpu(), inv, layout, factor, -1.0)
+    # differences of sum(w . rope(q)): linear in q, so a step of 1/2 is exact but for rounding
+    e = randn((3, 2, 32), 9)
+    f = lambda x: float((ref.rotate(x, pos.cpu(), inv, layout, factor) * wq.double()).sum())
+    slope = (f(q.detach().cpu().double() + 0.5 * e.double()) - f(q.detach().cpu().double() - 0.5 * e.double()))
+    assert abs(slope - float((dq.cpu().double() * e.double()).sum())) <= 1e-5 * 3 * 2 * 32
+    (g,) = torch.autograd.grad(A.rope_apply(q, pos, r).sum(), q)  # an expanded gradient
+    check_rope(g, torch.ones((3, 2, 32)), pos.cpu(), inv, layout, factor, -1.0)
+    (g,) = torch.autograd.grad(A.rope_apply(q, pos, r, k=k)[1].sum(), k)  # q's output unused
+    check_rope(g, torch.ones((3, 1, 32)), pos.cpu(), inv, layout, factor, -1.0)
+
+
+# ---------------------------------------------------------------- the cache
+
+
+def make_cache(pkg, P, H, blk, D, fmt, junk=True):
+    """A cache whose unused memory holds anything (NaN codes for e4m3)."""
+    c = pkg.attention.KVCache(P, H, D, blk, fmt)
+    if junk:
+        for t in (c.k_codes, c.v_codes):
+            t.view(torch.uint8).fill_(0x7F)
+        c.k_scale.fill_(float("nan"))
+        c.v_scale.fill_(float("nan"))
+    return c, ref.RefCache(P, H, blk, D, fmt), ref.RefCache(P, H, blk, D, fmt)
+
+
+def cache_equal(c, rk, rv, pages_lens, blk):
+    """Codes and scales of every written token equal the reference's."""
+    kc, vc = c.k_codes.cpu().float().double(), c.v_codes.cpu().float().double()
+    for pages, n in pages_lens:
+        for j in range(-(-n // blk)):
+            p, m = int(pages[j]), min(blk, n - j * blk)
+            for got, want in ((c.k_scale[p].cpu().double(), rk.scale[p]), (c.v_scale[p].cpu().double(), rv.scale[p])):
+                assert torch.equal(torch.isnan(got), torch.isnan(want))
+                assert torch.equal(got.nan_to_num(), want.nan_to_num()), (got, want)
+            assert torch.equal(kc[p][:, :m], rk.vals[p][:, :m]), (p, (kc[p][:, :m] - rk.vals[p][:, :m]).abs().max())
+            assert torch.equal(vc[p][:, :, :m].transpose(1, 2), rv.vals[p][:, :m])
+
+
+def tables(lens_max, blk, P, seed):
+    """Shuffled pages for sequences of up to lens_max tokens; -1 past the end."""
+    need = [max(1, -(-n // blk)) for n in lens_max]
+    perm = np.random.default_rng(seed).permutation(P)
+    t = np.full((len(need), max(need) + 1), -1, np.int64)
+    at = 0
+    for b, n in enumerate(need):
+        t[b, :n] = perm[at:at + n]
+        at += n
+    return t
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,D,blk,layout,rot", [(2, 128, 64, "interleaved", 128), (3, 80, 16, "half", 40), (1, 16, 32, "interleaved", 4),
+                                                (2, 256, 64, "half", 256), (2, 48, 16, "interleaved", 0)])
+def test_append_and_read(pkg, cuda_device, fmt, dtype, H, D, blk, layout, rot):
+    """Four appends (prompts, then a few tokens at a time, growing blocks) into
+    ragged sequences: codes and scales after each equal the reference's, as do
+    the values read back; q is rotated beside."""
+    A = pkg.attention
+    steps = [[1, blk + 3, 0, 2 * blk], [1, 1, 1, 1], [3, 0, blk, 5], [1, 1, 1, 0]]
+    lens_max = [sum(s[b] for s in steps) for b in range(4)]
+    P = sum(-(-n // blk) for n in lens_max) + 2
+    c, rk, rv = make_cache(pkg, P, H, blk, D, fmt)
+    tab = tables(lens_max, blk, P, 1)
+    td = i32(tab.tolist())
+    inv = torch.from_numpy((10000.0 ** (-2.0 * np.arange(rot // 2) / max(rot, 1))).astype(np.float32))
+    r = A.Rotary(inv.cuda(), layout, 1.0)
+    lens = np.zeros(4, int)
+    for si, n in enumerate(steps):
+        N = sum(n)
+        gain = 1.0 + 3.0 * si  # later tokens are larger: scales grow
+        k, v = randn((N + 2, H, D), 10 + si, DT[dtype], gain), randn((N + 2, H, D), 20 + si, DT[dtype], gain)
+        q = randn((N + 2, 2 * H, D), 30 + si, DT[dtype])
+        lens = lens + np.array(n)
+        cu = np.concatenate([[0], np.cumsum(n)])
+        pos = torch.tensor([p for b in range(4) for p in range(lens[b] - n[b], lens[b])], dtype=torch.int64)
+        kr = ref.rotate(k[:N], pos, inv, layout)
+        for b in range(4):
+            rk.append(kr, int(cu[b]), n[b], int(lens[b]), tab[b])
+            rv.append(v[:N].double(), int(cu[b]), n[b], int(lens[b]), tab[b])
+        q_out = c.append(k.cuda(), v.cuda(), td, i32(lens.tolist()), cu_of(n), rotary=r, q=q.cuda())
+        c.check()
+        cache_equal(c, rk, rv, [(tab[b], int(lens[b])) for b in range(4)], blk)
+        check_rope(q_out[:N], q[:N], pos, inv, layout, 1.0)
+    starts = [0, 2, int(lens[2]), 17]
+    counts = [int(lens[b]) - starts[b] for b in range(4)]
+    for out in ("bf16", "f32"):
+        gk, gv = c.read(td, i32(starts), cu_of(counts), sum(counts), dtype=DT[out], kv_lens=i32(lens.tolist()))
+        wk = torch.cat([rk.tokens(tab[b], int(lens[b]))[starts[b]:] for b in range(4)])
+        wv = torch.cat([rv.tokens(tab[b], int(lens[b]))[starts[b]:] for b in range(4)])
+        assert torch.equal(gk.cpu().double(), wk) and torch.equal(gv.cpu().double(), wv)
+    gk, _ = c.read(td[:1], None, i32([0, 2]), 2)
+    assert torch.equal(gk.cpu().double(), rk.tokens(tab[0], 2))
+    c.check()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_append_values_at_the_edges(pkg, cuda_device, fmt):
+    """Zeros, subnormals, values at the scale's border, the largest floats, and
+    values that are not finite; a poisoned block reads NaN until it starts over."""
+    D, blk, q = 16, 16, ref.QMAX[fmt]
+    c, rk, rv = make_cache(pkg, 12, 1, blk, D, fmt)
+    rows = [torch.zeros(D), torch.full((D,), 1e-42), torch.full((D,), q), torch.full((D,), q * (1 + 2.0 ** -20)),
+            torch.full((D,), 3.4e38), torch.linspace(-q, q, D), torch.full((D,), -2.0 ** -120)]
+    tab = i32([[i] for i in range(len(rows))])
+    x = torch.stack(rows)[:, None]
+    n = len(rows)
+    for b in range(n):
+        rk.append(x.double(), b, 1, 1, [b])
+        rv.append(x.double(), b, 1, 1, [b])
+    c.append(x.cuda(), x.cuda(), tab, i32([1] * n), cu_of([1] * n))
+    cache_equal(c, rk, rv, [([b], 1) for b in range(n)], blk)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        y = torch.ones((3, 1, D))
+        y[1, 0, 3] = bad
+        t = i32([[9]])
+        c.append(y.cuda(), torch.ones_like(y).cuda(), t, i32([3]), i32([0, 3]))
+        assert math.isnan(float(c.k_scale[9, 0])) and not math.isnan(float(c.v_scale[9, 0]))
+        assert torch.isfinite(c.k_codes[9].float()).all() or fmt == "e4m3"
+        c.append(torch.ones((1, 1, D), device="cuda"), torch.ones((1, 1, D), device="cuda"), t, i32([4]), i32([0, 1]))
+        gk, gv = c.read(t, None, i32([0, 4]), 4, dtype=torch.float32)
+        assert torch.isnan(gk).all() and torch.equal(gv.cpu(), torch.ones((4, 1, D)))
+        c.append(torch.ones((1, 1, D), device="cuda"), torch.ones((1, 1, D), device="cuda"), t, i32([1]), i32([0, 1]))
+        gk, _ = c.read(t, None, i32([0, 1]), 1, dtype=torch.float32)
+        assert torch.equal(gk.cpu(), torch.ones((1, 1, D)))
+    c.check()
+
+
+# ---------------------------------------------------------------- attention
+
+
+def fill(c, seed, gain=1.0):
+    """Random finite codes and power-of-two scales; returns the reference pools."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for codes, scale, trans in ((c.k_codes, c.k_scale, False), (c.v_codes, c.v_scale, True)):
+        P, H = scale.shape
+        x = torch.randn(codes.shape, generator=g) * (40 if c.format == "int8" else 100)
+        x = x.round().clamp(-127, 127).to(torch.int8) if c.format == "int8" else x.clamp(-448, 448).to(ref.F8)
+        s = 2.0 ** torch.randint(-8, -4, (P, H), generator=g).float() * gain
+        codes.copy_(x.cuda())
+        scale.copy_(s.cuda())
+        r = ref.RefCache(P, H, c.block, c.head_dim, c.format)
+        r.vals = (x.float().double().transpose(2, 3) if trans else x.float().double()).contiguous()
+        r.scale = s.double()
+        out.append(r)
+    return out
+
+
+def check_attention(pkg, c, rk, rv, tab, lens, news, Hq, dtype, window=0, seed=0, qgain=1.0, scale=None, max_rows=None,
+                    strided=False):
+    N, D = sum(news), c.head_dim
+    q = randn((N, Hq, D), seed, DT[dtype], qgain)
+    qd = q.cuda()
+    if strided:
+        wide = torch.zeros((N, Hq + 3, D), dtype=DT[dtype], device="cuda")
+        wide[:, 1:1 + Hq] = qd
+        qd = wide[:, 1:1 + Hq]
+    pad = 3
+    qp = torch.cat([qd, torch.full((pad, Hq, D), float("nan"), dtype=DT[dtype], device="cuda")])
+    out = torch.full_like(qp, 7.5)
+    got, lse = c.attention(qp, i32(tab.tolist()), i32(lens), cu_of(news), max(news) if max_rows is None else max_rows, scale=scale,
+                           window=window, out=out, return_lse=True)
+    c.check()
+    assert torch.all(got[N:] == 7.5)  # rows behind the last sequence
+    row = 0
+    sc = scale if scale is not None else D ** -0.5
+    for b, (L, n) in enumerate(zip(lens, news)):
+        if n == 0:
+            continue
+        pos = torch.arange(L - n, L)
+        o, ls, mag, smax = ref.attend(q[row:row + n].double(), rk.tokens(tab[b], L), rv.tokens(tab[b], L), pos, sc, window)
+        g = got[row:row + n].cpu().double()
+        tol = ref.attend_tolerance(DT[dtype], o, mag, smax, D, L)
+        bad = torch.isnan(g) | ((g - o).abs() > tol)
+        assert not bool(bad.any()), (b, L, n, float(((g - o).abs() / tol).max()))
+        gl = lse[row:row + n].cpu().double()
+        lt = 2 * (D + 8) * 2.0 ** -23 * smax + (L + 64) * 2.0 ** -23 + 2.0 ** -22 * ls.abs()
+        assert bool(((gl - ls).abs() <= lt)[~torch.isinf(ls)].all()) and torch.equal(torch.isinf(gl), torch.isinf(ls))
+        row += n
+    return got
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("Hkv,g,D,blk", [(2, 4, 128, 64), (1, 1, 64, 16), (2, 5, 80, 32), (1, 16, 256, 64), (3, 2, 16, 16),
+                                         (1, 33, 48, 32), (2, 8, 128, 16), (1, 8, 144, 32)])
+def test_attention(pkg, cuda_device, fmt, dtype, Hkv, g, D, blk):
+    """Ragged batch: one token, block borders, idle sequences, many rows."""
+    lens = [1, blk, blk + 1, 0, 63, 64, 65, 700, 129, 5]
+    news = [1, 1, 2, 0, 1, 3, 65, 1, 17, 5]
+    P = sum(max(1, -(-n // blk)) for n in lens) + 3
+    c, _, _ = make_cache(pkg, P, Hkv, blk, D, fmt)
+    rk, rv = fill(c, 5)
+    tab = tables(lens, blk, P, 2)
+    check_attention(pkg, c, rk, rv, tab, lens, news, Hkv * g, dtype, seed=3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window", [1, 16, 63, 64, 200])
+def test_attention_window(pkg, cuda_device, dtype, window):
+    lens, news, blk = [300, 64, 1, 555, 210], [1, 64, 1, 40, 9], 32
+    P = sum(-(-n // blk) for n in lens)
+    c, _, _ = make_cache(pkg, P, 2, blk, 64, "int8")
+    rk, rv = fill(c, 6)
+    check_attention(pkg, c, rk, rv, tables(lens, blk, P, 4), lens, news, 8, dtype, window=window, seed=4, strided=True)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("B,L,Hkv", [(1, 20000, 1), (1, 9000, 8), (300, 90, 2), (3, 4000, 2)])
+def test_attention_split(pkg, cuda_device, fmt, B, L, Hkv):
+    """Long contexts cut between warps and joined; many short sequences."""
+    rng = np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(max(1, L // 2), L + 1, B)]
+    blk = 64
+    P = sum(-(-n // blk) for n in lens)
+    c, _, _ = make_cache(pkg, P, Hkv, blk, 128, fmt)
+    rk, rv = fill(c, 7)
+    check_attention(pkg, c, rk, rv, tables(lens, blk, P, 5), lens, [1] * B, 4 * Hkv, "bf16", seed=5, qgain=3.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_prompt_from_nothing(pkg, cuda_device, dtype):
+    """A whole prompt (its own rows are all the context), with and without a window."""
+    lens, blk = [333, 1, 128, 200], 64
+    P = sum(-(-n // blk) for n in lens)
+    c, _, _ = make_cache(pkg, P, 2, blk, 128, "int8")
+    rk, rv = fill(c, 8)
+    for w in (0, 50):
+        check_attention(pkg, c, rk, rv, tables(lens, blk, P, 6), lens, lens, 8, dtype, window=w, seed=6)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("qgain,gain", [(1e-30, 1.0), (1e30, 2.0 ** -100), (60.0, 1.0), (0.0, 1.0), (1.0, 2.0 ** 60), (1.0, 2.0 ** -60)])
+def test_attention_magnitudes(pkg, cuda_device, dtype, qgain, gain):
+    """Queries and scales far from one, peaked and flat softmax."""
+    lens, blk = [150, 64], 16
+    P = 14
+    c, _, _ = make_cache(pkg, P, 1, blk, 64, "e4m3")
+    rk, rv = fill(c, 9, gain)
+    s = 0.125 if gain == 1.0 or qgain != 1.0 else 0.125 / gain
+    check_attention(pkg, c, rk, rv, tables(lens, blk, P, 7), lens, [1, 2], 4, dtype, seed=7, qgain=qgain, scale=s)
