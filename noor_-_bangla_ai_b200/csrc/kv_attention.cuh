@@ -6,30 +6,32 @@
 //
 // For few query rows the time is that of reading the codes once, so the work
 // is cut by bytes: the batch's visible 64-token tiles of every (sequence, kv
-// head, 16-row tile of queries) form one list, and every warp of the grid
-// takes an equal contiguous share of it, whatever the sequences' lengths.  A
-// warp works alone, with no barrier to the others: it streams its tiles through its own ring
-// in shared memory with bulk copies and keeps o, m and l in registers.  A unit
-// (sequence, head, row tile) cut between warps leaves partial (m, l, o), which
-// combine_kernel joins in a fixed order.
+// head, tile of query rows) form one list, and every warp pair of the grid takes an
+// equal contiguous share of it, whatever the sequences' lengths.  A pair works
+// alone: its first warp streams the tiles into the pair's own ring in
+// shared memory with bulk copies, each warp takes 32 of a tile's 64 tokens and
+// keeps its o, m and l in registers, and the two are joined when a unit
+// (sequence, head, row tile) ends.  A unit cut between pairs leaves partial
+// (m, l, o), which combine_kernel joins in a fixed order.
 //
-// The products run on mma.sync m16n8k16 in f16 with f32 sums: the query rows
-// of a kv head's group fill the 16 rows, which tcgen05's 128-row tiles would
-// leave empty, and at one pass per byte the tensor work is far below the
-// memory time.  Codes (|int8| <= 127, e4m3) are exact in f16.  Queries are
+// The products run on mma.sync m16n8k16 in f16 with f32 sums, with tokens (and
+// for p v, head dims) as the 16 rows and 8 query rows as the columns: a decode
+// step has 1 to 8 query rows for a kv head, which tcgen05's 128-row tiles would
+// leave nearly empty, and at one pass per byte the tensor work is far below
+// the memory time.  More rows (NB = 4: 32) share each widened code.
+// Codes (|int8| <= 127, e4m3) are exact in f16.  Queries are
 // scaled by a power of two for each row so that f16 holds them: exactly for BF16
 // (elements under 2^-38 of the row's largest aside), and for F32 as a sum of
-// two f16 parts (22 bits).  Probabilities p are f16 as well, off by 2^-12
+// two f16 parts (22 bits).  Probabilities p are f16 as well, off by 2^-11
 // relative, an eighth of the BF16 output's half step (F32: two parts again),
 // scaled by 2^14 so that p down to 2^-38 counts in a long context.  A block's
 // v scale multiplies its p, relative to the largest scale so far.
 //
 // The contraction index of an mma may be permuted at will if both operands
-// agree: thread c of a quad takes 16 consecutive bytes of a key row and of a
-// value row and feeds them to four mma steps, so both operands come straight
-// from the stored layouts with 16-byte shared loads; a score tile's column n
-// is token 16 (n / 2) + 2 t + n % 2, which makes the thread that holds a
-// score the one that needs it for p v.
+// agree: thread c of a quad takes 16 consecutive bytes of a key row and feeds
+// them to four mma steps, so keys come straight from the stored layout with
+// 16-byte shared loads; token 8 (r / 2) + 2 G + r % 2 is row r of score group
+// G, which leaves thread c with 8 consecutive tokens of each value row.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -56,11 +58,13 @@ struct Args {
   int32_t Hq, g;   // query heads, query heads per kv head
   float scale2;    // scale * log2(e)
   int32_t window;
-  // partial results: [2 * warps] slots of 16 rows of (D o's), and [2 * warps][32] (m, l)
+  // partial results: [2 * pairs] slots of `rows` rows of D o's, and of `rows` (m, l)
   float* part_o;
   float* part_ml;
-  int4* desc;      // [warps] of the split units: (sequence, head | row tile << 12.., first warp, last warp)
-  int32_t warps;   // warps of the grid that share the work
+  int4* desc;      // [pairs] the cut unit that starts in a pair's share: (sequence or -1, head, row tile,
+                   // last pair << 1 | slot of its part)
+  int32_t pairs;   // warp pairs of the grid that share the work
+  int32_t rows;    // query rows of a row tile
 };
 
 // ------------------------------------------------------------ mma pieces
@@ -119,7 +123,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 
 struct SeqWork {
   kv::Seq s;
-  int32_t rtiles;    // 16-row tiles of (row, query head of the group)
+  int32_t rtiles;    // row tiles of (row, query head of the group)
   int32_t t0, tiles; // first visible 64-token tile and their number, over all rows
 };
 
@@ -127,7 +131,7 @@ __device__ __forceinline__ SeqWork seq_work(const Args& a, int i) {
   SeqWork w;
   w.s = kv::sequence(a.b, a.b.cu, a.b.lens, a.c.blk, i, a.c.status);
   if (w.s.n > 0 && w.s.len < w.s.n) kv::flag(a.c.status, NOOR_KV_BAD_LENGTH);
-  w.rtiles = (int)(((int64_t)w.s.n * a.g + 15) >> 4);
+  w.rtiles = (int)(((int64_t)w.s.n * a.g + a.rows - 1) / a.rows);
   // rows at negative positions see nothing; at least one tile, so that rows
   // which see nothing are written too
   const int32_t p0 = max(w.s.len - w.s.n, 0);
@@ -137,41 +141,63 @@ __device__ __forceinline__ SeqWork seq_work(const Args& a, int i) {
   return w;
 }
 
-// Warps per block and shared memory: a ring of two tiles (k and v) and the
-// query fragments for each warp.
-template <int DP, int PARTS>
+// Transpose the 8x8 f16 matrix whose row r, columns 2c, 2c + 1 thread (r, c) holds.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void pair_sync(int pair) {
+  asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory");
+}
+
+// Pairs per block and shared memory: a ring of two tiles (k and v) for each
+// pair, and the query fragments where they do not fit into registers.
+template <int DP, int PARTS, int NB>
 struct Shape {
-  static constexpr int kWarps = DP == 64 ? 8 : DP == 128 ? (PARTS == 1 ? 6 : 5) : (PARTS == 1 ? 3 : 2);
+  static constexpr int kRows = 8 * NB;
+  static constexpr bool kQShared = DP / 8 * NB * PARTS > 32;
+  static constexpr int kPairs = DP == 64 ? (NB == 1 ? 8 : 4)
+                                : DP == 128 ? (NB == 1 ? (PARTS == 1 ? 7 : 6) : 4)
+                                            : (NB == 1 ? 3 : 2);
   static constexpr int kStages = 2;
-  static constexpr int kQBytes = DP / 16 * 32 * 16 * PARTS;
+  static constexpr int kQBytes = kQShared ? DP / 16 * NB * PARTS * 32 * 8 : 0;
   // v pages of 16 or 32 tokens lie 32 or 64 bytes apart, so that the quads'
   // reads of different pages fall into different banks
   static constexpr int kVPad = 128;
-  static __host__ __device__ int warp_bytes(int D) { return kStages * (2 * kTile * D + kVPad) + kQBytes; }
-  static __host__ __device__ int smem_bytes(int D) { return kWarps * (warp_bytes(D) + 2 * kStages * 8) + 128; }
+  // bytes of the second warp's part when the pair joins (it reuses the ring)
+  static constexpr int kJoin = (DP / 16 * NB * 4 + 4 * NB + 1) * 32 * 4;
+  static __host__ __device__ int pair_bytes(int D) {
+    const int ring = kStages * (2 * kTile * D + kVPad);
+    return (ring > kJoin ? ring : kJoin) + kQBytes;
+  }
+  static constexpr int kBarBytes = (kPairs * 2 * kStages * 8 + 127) / 128 * 128;
+  static __host__ __device__ int smem_bytes(int D) { return kBarBytes + kPairs * pair_bytes(D); }
 };
 
-template <int DP, int FMT, int PARTS>
-__global__ void __launch_bounds__(Shape<DP, PARTS>::kWarps * 32, 1) stream_kernel(const Args a) {
-  using Sh = Shape<DP, PARTS>;
+template <int DP, int FMT, int PARTS, int NB>
+__global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_kernel(const Args a) {
+  using Sh = Shape<DP, PARTS, NB>;
   using T = typename std::conditional<PARTS == 1, bf16, float>::type;
-  constexpr int NST = Sh::kStages;
+  constexpr int NST = Sh::kStages, R = Sh::kRows;
   extern __shared__ __align__(128) uint8_t s_attn[];
   const int D = a.c.D, blk = a.c.blk;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, qc = lane & 3;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_attn) + warp * 2 * NST;  // k barriers, then v
-  uint8_t* mine = s_attn + (Sh::kWarps * 2 * NST * 8 + 127) / 128 * 128 + warp * Sh::warp_bytes(D);
+  const int pair = threadIdx.x >> 6, half = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31, gr = lane >> 2, qc = lane & 3;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_attn) + pair * 2 * NST;  // k barriers, then v
+  uint8_t* mine = s_attn + Sh::kBarBytes + pair * Sh::pair_bytes(D);
   const int kbytes = kTile * D, vbytes = kTile * D + Sh::kVPad;
   uint8_t* s_k = mine;
   uint8_t* s_v = mine + NST * kbytes;
-  uint4* s_q = reinterpret_cast<uint4*>(mine + NST * (kbytes + vbytes));  // [part][k step][lane]
-  if (lane < 2 * NST) tc::mbar_init(bars + lane, 1);
+  float* s_join = reinterpret_cast<float*>(mine);
+  uint2* s_q = reinterpret_cast<uint2*>(mine + Sh::pair_bytes(D) - Sh::kQBytes);  // [part][k step][nb][lane]
+  if (half == 0 && lane < 2 * NST) tc::mbar_init(bars + lane, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
+  pair_sync(pair);
 
-  // ---- this warp's share of the list
-  const int wid = warp * gridDim.x + blockIdx.x;
+  // ---- this pair's share of the list
+  const int wid = pair * gridDim.x + blockIdx.x;
   int64_t total = 0;
   for (int base = 0; base < a.b.B; base += 32) {
     int64_t n = 0;
@@ -183,12 +209,12 @@ __global__ void __launch_bounds__(Shape<DP, PARTS>::kWarps * 32, 1) stream_kerne
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     total += n;
   }
-  if (lane == 0) a.desc[wid] = make_int4(-1, 0, 0, 0);
-  // no more warps than tiles: every share has one, so a cut unit's parts lie
-  // in consecutive warps
-  const int64_t warps = min((int64_t)a.warps, total);
-  if (wid >= warps) return;
-  const int64_t beg = total * wid / warps, end = total * (wid + 1) / warps;
+  if (half == 0 && lane == 0) a.desc[wid] = make_int4(-1, 0, 0, 0);
+  // no more shares than tiles: every share has one, so a cut unit's parts lie
+  // in consecutive pairs
+  const int64_t pairs = min((int64_t)a.pairs, total);
+  if (wid >= pairs) return;
+  const int64_t beg = total * wid / pairs, end = total * (wid + 1) / pairs;
   // ---- find the sequence of `beg`
   int sb = 0;
   int64_t seq0 = 0;  // list position of sequence sb
@@ -222,7 +248,9 @@ __global__ void __launch_bounds__(Shape<DP, PARTS>::kWarps * 32, 1) stream_kerne
   bool dead = false;                // a wait gave up: nothing more is issued or waited for
   int64_t at = beg;
   SeqWork w = seq_work(a, sb);
-  int piece = 0;  // pieces of units left as partials by this warp
+  int piece = 0;  // pieces of units so far
+  const int my_tok = 8 * (gr >> 1) + (gr & 1);  // this lane's token of score group 0, within its warp's 32
+  const float nan = __uint_as_float(0x7FC00000u);
   while (at < end) {
     const int64_t unit_tiles = w.tiles, seq_units = (int64_t)w.rtiles * a.c.H;
     if (at - seq0 >= unit_tiles * seq_units) {  // next sequence (those without rows are passed over)
@@ -236,112 +264,57 @@ __global__ void __launch_bounds__(Shape<DP, PARTS>::kWarps * 32, 1) stream_kerne
     const int h = (int)(u / w.rtiles), rt = (int)(u % w.rtiles);
     const int64_t stop = min(end, u1);
 
-    // rows of the unit: index e = 16 rt + i is query row e / g, head h g + e % g
-    const int nrows = min(16, w.s.n * a.g - 16 * rt);
-    const int p_first = w.s.len - w.s.n + (16 * rt) / a.g;
-    const int p_last = w.s.len - w.s.n + (16 * rt + nrows - 1) / a.g;
-    int qpos[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = gr + 8 * i;
-      qpos[i] = r < nrows ? w.s.len - w.s.n + (16 * rt + r) / a.g : -1;
-    }
-    // the unit's own visible tiles, within this warp's share
+    // rows of the unit: index e = R rt + i is query row e / g, head h g + e % g
+    const int e0 = R * rt;
+    const int nrows = min(R, w.s.n * a.g - e0);
+    const int pos0 = w.s.len - w.s.n;
+    const int p_first = pos0 + e0 / a.g;
+    const int p_last = pos0 + (e0 + nrows - 1) / a.g;
+    // the unit's own visible tiles, within this pair's share
     const int lo_tok = a.window > 0 ? max(p_first - a.window, 0) : 0;
     const int hi_tok = p_last + 1;  // one past the last visible token
     const int tb = max(w.t0 + (int)(at - u0), lo_tok / kTile);
     const int te = min(w.t0 + (int)(stop - u0), (hi_tok + kTile - 1) / kTile);
 
-    // ---- query fragments
-    float qfac[2] = {0.f, 0.f};
-    {
-      const T* qp[2] = {nullptr, nullptr};
-      float mx[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = gr + 8 * i;
-        if (r < nrows) {
-          const int e = 16 * rt + r;
-          qp[i] = static_cast<const T*>(a.q.p) + (int64_t)(w.s.row0 + e / a.g) * a.q.st + (int64_t)(h * a.g + e % a.g) * a.q.sh;
-          for (int d = qc; d < D; d += 4) mx[i] = fmaxf(mx[i], fabsf(rope::to_f32(qp[i][d])));
-        }
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      }
-      float up[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // 2^e <= mx < 2^(e + 1) becomes 2^14: up = 2^(14 - e), within f32's exponents
-        int ex = (int)(__float_as_uint(mx[i]) >> 23) - 127;
-        ex = max(min(ex, 127), -112);
-        up[i] = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
-        qfac[i] = a.scale2 * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
-      }
-      __syncwarp();
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        // step ks = 4 j + s takes bytes 4 s .. 4 s + 3 of chunk 4 j + c
-        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
-        float v[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[i][x] = qp[i] != nullptr && d0 < D ? rope::to_f32(qp[i][d0 + x]) * up[i] : 0.f;
-        const uint4 hi = make_uint4(pack_half(v[0][0], v[0][1]), pack_half(v[1][0], v[1][1]), pack_half(v[0][2], v[0][3]),
-                                    pack_half(v[1][2], v[1][3]));
-        s_q[ks * 32 + lane] = hi;
-        if constexpr (PARTS == 2)
-          s_q[(DP / 16 + ks) * 32 + lane] =
-              make_uint4(pack_rest(v[0][0], v[0][1], hi.x), pack_rest(v[1][0], v[1][1], hi.y),
-                         pack_rest(v[0][2], v[0][3], hi.z), pack_rest(v[1][2], v[1][3], hi.w));
-      }
-      __syncwarp();
-    }
-
-    float o[DP / 8][4];
-#pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float vref = 1.17549435e-38f;
-
-    // Issue tile t into a stage: every quad lane knows its own page (16-token
-    // quarter qc of the tile) and the first quad's lanes issue one copy per
-    // page.  Returns the page's scales and whether it can be read.
+    // The first warp issues tile t into a stage: lane p one copy for page p of
+    // the tile.
     const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
-    const int per_page = blk / 16;  // quarters of a page
-    auto issue = [&](int t, int stage, float& ks, float& vs, bool& have) {
-      const int tok = t * kTile + 16 * qc;
-      have = false;
-      ks = vs = 0.f;
+    const int tile_pages = kTile / blk;
+    auto issue = [&](int t, int stage) {
       int32_t page = -1;
-      if (tok / blk * blk < hi_tok) {
-        page = __ldg(table + tok / blk);
-        have = page >= 0 && (int64_t)page < a.c.P;
-        if (!have) {
+      if (lane < tile_pages && t * kTile + lane * blk < hi_tok) {
+        page = __ldg(table + t * tile_pages + lane);
+        if (page < 0 || (int64_t)page >= a.c.P) {
           kv::flag(a.c.status, NOOR_KV_BAD_PAGE);
-          ks = vs = __uint_as_float(0x7FC00000u);
+          page = -1;
         }
       }
-      const int64_t ph = have ? (int64_t)page * a.c.H + h : 0;
-      const bool first = gr == 0 && qc % per_page == 0 && have && !dead;
-      const unsigned who = __ballot_sync(0xffffffffu, first);
+      if (dead) return;
+      const unsigned who = __ballot_sync(0xffffffffu, page >= 0);
       const uint32_t bytes = (uint32_t)blk * D;
-      if (!dead) {
-        if (lane == 0) {
-          tc::mbar_arrive_expect_tx(bars + stage, __popc(who) * bytes);
-          tc::mbar_arrive_expect_tx(bars + NST + stage, __popc(who) * bytes);
-        }
-        __syncwarp();
-        if (first) {
-          const int pg = qc / per_page;
-          bulk_load(s_k + stage * kbytes + pg * bytes, a.c.k + ph * bytes, bytes, bars + stage);
-          bulk_load(s_v + stage * vbytes + pg * (bytes + 2 * blk), a.c.v + ph * bytes, bytes, bars + NST + stage);
-        }
+      if (lane == 0) {
+        tc::mbar_arrive_expect_tx(bars + stage, __popc(who) * bytes);
+        tc::mbar_arrive_expect_tx(bars + NST + stage, __popc(who) * bytes);
       }
-      if (have) {
-        ks = __ldg(a.c.ks + ph);
-        vs = __ldg(a.c.vs + ph);
+      __syncwarp();
+      if (page >= 0) {
+        const int64_t ph = ((int64_t)page * a.c.H + h) * bytes;
+        bulk_load(s_k + stage * kbytes + lane * bytes, a.c.k + ph, bytes, bars + stage);
+        bulk_load(s_v + stage * vbytes + lane * (bytes + 2 * blk), a.c.v + ph, bytes, bars + NST + stage);
+      }
+    };
+    // Scales of the page that holds this lane's score tokens of tile t: NaN
+    // for a page that cannot be read, 0 past the visible tokens.
+    auto scales = [&](int t, float& ks, float& vs, bool& have) {
+      const int tok = t * kTile + 32 * half + 8 * (gr >> 1);
+      ks = vs = 0.f;
+      have = false;
+      if (tok / blk * blk < hi_tok) {
+        const int32_t page = __ldg(table + tok / blk);
+        have = page >= 0 && (int64_t)page < a.c.P;
+        const int64_t ph = (int64_t)page * a.c.H + h;
+        ks = have ? __ldg(a.c.ks + ph) : nan;
+        vs = have ? __ldg(a.c.vs + ph) : nan;
       }
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -358,235 +331,363 @@ __global__ void __launch_bounds__(Shape<DP, PARTS>::kWarps * 32, 1) stream_kerne
 
     float ks_s[NST], vs_s[NST];
     bool have_s[NST];
+    if (half == 0) {
+#pragma unroll
+      for (int i = 0; i < NST; ++i)
+        if (tb + i < te) issue(tb + i, i);
+    }
 #pragma unroll
     for (int i = 0; i < NST; ++i)
-      if (tb + i < te) issue(tb + i, i, ks_s[i], vs_s[i], have_s[i]);
+      if (tb + i < te) scales(tb + i, ks_s[i], vs_s[i], have_s[i]);
+
+    // ---- query fragments: this lane holds row gr of each group of 8, dims
+    // d0 .. d0 + 3 of step ks = 4 j + s, d0 = 16 (4 j + c) + 4 s
+    uint2 qreg[Sh::kQShared ? 1 : PARTS * DP / 16 * NB];
+    float qfac[NB][2];  // score factors of rows 2c, 2c + 1 of each group
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = 8 * nb + gr, e = e0 + r;
+      const T* qp = nullptr;
+      if (r < nrows)
+        qp = static_cast<const T*>(a.q.p) + (int64_t)(w.s.row0 + e / a.g) * a.q.st + (int64_t)(h * a.g + e % a.g) * a.q.sh;
+      float mx = 0.f;
+      if (qp != nullptr)
+        for (int d = qc; d < D; d += 4) mx = fmaxf(mx, fabsf(rope::to_f32(qp[d])));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // 2^e <= mx < 2^(e + 1) becomes 2^14: up = 2^(14 - e), within f32's exponents
+      const int ex = max(min((int)(__float_as_uint(mx) >> 23) - 127, 127), -112);
+      const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+      const float down = a.scale2 * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
+      qfac[nb][0] = __shfl_sync(0xffffffffu, down, 8 * qc);
+      qfac[nb][1] = __shfl_sync(0xffffffffu, down, 8 * qc + 4);
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
+        float v[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = qp != nullptr && d0 < D ? rope::to_f32(qp[d0 + x]) * up : 0.f;
+        const uint2 hi = make_uint2(pack_half(v[0], v[1]), pack_half(v[2], v[3]));
+        const uint2 lo = make_uint2(pack_rest(v[0], v[1], hi.x), pack_rest(v[2], v[3], hi.y));
+        if constexpr (Sh::kQShared) {
+          if (half == 0) {  // both warps use it
+            s_q[(ks * NB + nb) * 32 + lane] = hi;
+            if constexpr (PARTS == 2) s_q[((DP / 16 + ks) * NB + nb) * 32 + lane] = lo;
+          }
+        } else {
+          qreg[ks * NB + nb] = hi;
+          if constexpr (PARTS == 2) qreg[(DP / 16 + ks) * NB + nb] = lo;
+        }
+      }
+    }
+    if constexpr (Sh::kQShared) pair_sync(pair);
+    int qpos[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) qpos[nb][x] = pos0 + (e0 + 8 * nb + 2 * qc + x) / a.g;
+
+    float o[DP / 16][NB][4];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][nb][x] = 0.f;
+    float m[NB][2], l[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[nb][x] = -INFINITY;
+        l[nb][x] = 0.f;
+      }
+    float vref = 1.17549435e-38f;
 
     for (int t = tb; t < te; ++t) {
       const int stage = (t - tb) % NST;
       const float ks = ks_s[0], vs = vs_s[0];
       const bool have = have_s[0];
-      // ---- scores
+      const int tok0 = t * kTile + 32 * half;
+      // ---- scores of this warp's 32 tokens
       wait(bars + stage, (kphase >> stage) & 1);
       kphase ^= 1u << stage;
-      float sc[8][4];
+      float sc[2][NB][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[i][x] = 0.f;
-      const uint8_t* kt = s_k + stage * kbytes + (16 * (gr >> 1) + (gr & 1)) * D + 16 * qc;
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[i][nb][x] = 0.f;
+      const uint8_t* kt = s_k + stage * kbytes + (32 * half + my_tok) * D + 16 * qc;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j) {
         if (64 * j >= D) break;
         const bool in = 64 * j + 16 * qc < D;
-        uint4 qf[4 * PARTS];
+        uint4 kb[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          qf[s] = s_q[(4 * j + s) * 32 + lane];
-          if constexpr (PARTS == 2) qf[4 + s] = s_q[(DP / 16 + 4 * j + s) * 32 + lane];
+        for (int G = 0; G < 4; ++G) {
+          kb[G] = make_uint4(0, 0, 0, 0);
+          if (in) kb[G] = *reinterpret_cast<const uint4*>(kt + 2 * G * D + 64 * j);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint4 kb = make_uint4(0, 0, 0, 0);
-          if (in) kb = *reinterpret_cast<const uint4*>(kt + 2 * i * D + 64 * j);
-          const uint32_t w4[4] = {kb.x, kb.y, kb.z, kb.w};
+        for (int s = 0; s < 4; ++s) {
+          uint2 qf[PARTS][NB];
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            uint32_t b0, b1;
-            widen<FMT>(w4[s], b0, b1);
-            mma_f16(sc[i], qf[s].x, qf[s].y, qf[s].z, qf[s].w, b0, b1);
-            if constexpr (PARTS == 2) mma_f16(sc[i], qf[4 + s].x, qf[4 + s].y, qf[4 + s].z, qf[4 + s].w, b0, b1);
+          for (int pt = 0; pt < PARTS; ++pt)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const int qi = (pt * DP / 16 + 4 * j + s) * NB + nb;
+              qf[pt][nb] = Sh::kQShared ? s_q[qi * 32 + lane] : qreg[Sh::kQShared ? 0 : qi];
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 x0 = kb[2 * i], x1 = kb[2 * i + 1];
+            const uint32_t w0 = s == 0 ? x0.x : s == 1 ? x0.y : s == 2 ? x0.z : x0.w;
+            const uint32_t w1 = s == 0 ? x1.x : s == 1 ? x1.y : s == 2 ? x1.z : x1.w;
+            uint32_t a0, a1, a2, a3;
+            widen<FMT>(w0, a0, a2);
+            widen<FMT>(w1, a1, a3);
+#pragma unroll
+            for (int pt = 0; pt < PARTS; ++pt)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma_f16(sc[i][nb], a0, a1, a2, a3, qf[pt][nb].x, qf[pt][nb].y);
           }
         }
       }
       // ---- scale, mask, running maximum
-      const float f0 = qfac[0] * ks, f1 = qfac[1] * ks;
-      const int tok0 = t * kTile + 16 * qc;
-      const bool whole = t * kTile + kTile - 1 <= p_first && (a.window <= 0 || p_last - t * kTile <= a.window);
-      float tm[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float v = sc[i][x] * (x < 2 ? f0 : f1);
-          if (!whole) {
-            const int tok = tok0 + 2 * i + (x & 1), p = qpos[x >> 1];
-            if (tok > p || (a.window > 0 && p - tok > a.window)) v = -INFINITY;
-          }
-          sc[i][x] = v;
-          tm[x >> 1] = fmaxf(tm[x >> 1], v);
-        }
-      float alpha[2], mref[2];
-      const float vmax = fmaxf(fabsf(vs), __shfl_xor_sync(0xffffffffu, fabsf(vs), 1));
-      const float vnew = fmaxf(vref, fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2)));
+      const bool whole = tok0 + 31 <= p_first && (a.window <= 0 || p_last - tok0 <= a.window);
+      float alpha[NB][2], mref[NB][2];
+      const float vmax = fmaxf(fabsf(vs), __shfl_xor_sync(0xffffffffu, fabsf(vs), 16));
+      const float vnew = fmaxf(vref, vmax);
       const float vstep = vref / vnew, vrel = vs / vnew;
       vref = vnew;
+      bool moved = vstep != 1.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        tm[i] = fmaxf(tm[i], __shfl_xor_sync(0xffffffffu, tm[i], 1));
-        tm[i] = fmaxf(tm[i], __shfl_xor_sync(0xffffffffu, tm[i], 2));
-        const float mn = fmaxf(m[i], tm[i]);
-        mref[i] = mn == -INFINITY ? 0.f : mn - kPShift;
-        alpha[i] = mn == -INFINITY ? 1.f : exp2_approx(m[i] - mn);
-        m[i] = mn;
+      for (int nb = 0; nb < NB; ++nb) {
+        float tm[2] = {-INFINITY, -INFINITY};
+        const float f0 = qfac[nb][0] * ks, f1 = qfac[nb][1] * ks;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float v = sc[i][nb][x] * ((x & 1) ? f1 : f0);
+            if (!whole) {
+              const int tok = tok0 + my_tok + 2 * (2 * i + (x >> 1)), p = qpos[nb][x & 1];
+              if (tok > p || (a.window > 0 && p - tok > a.window)) v = -INFINITY;
+            }
+            sc[i][nb][x] = v;
+            tm[x & 1] = fmaxf(tm[x & 1], v);
+          }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          tm[x] = fmaxf(tm[x], __shfl_xor_sync(0xffffffffu, tm[x], 4));
+          tm[x] = fmaxf(tm[x], __shfl_xor_sync(0xffffffffu, tm[x], 8));
+          tm[x] = fmaxf(tm[x], __shfl_xor_sync(0xffffffffu, tm[x], 16));
+          const float mn = fmaxf(m[nb][x], tm[x]);
+          mref[nb][x] = mn == -INFINITY ? 0.f : mn - kPShift;
+          alpha[nb][x] = mn == -INFINITY ? 1.f : exp2_approx(m[nb][x] - mn);
+          m[nb][x] = mn;
+          moved |= alpha[nb][x] != 1.f;
+        }
       }
-      // ---- probabilities (f16 pairs are mma's first operand)
-      uint32_t pf[8][2 * PARTS];
-      float sum[2] = {0.f, 0.f};
+      // ---- probabilities, transposed into the second operand's layout
+      uint32_t pf[PARTS][NB][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int nb = 0; nb < NB; ++nb) {
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = exp2_approx(sc[i][x] - mref[x >> 1]);
-          sum[x >> 1] += p;
-          // a masked token's p is zero whatever its block's scale
-          sc[i][x] = sc[i][x] == -INFINITY ? 0.f : p * vrel;
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float p = exp2_approx(sc[i][nb][x] - mref[nb][x & 1]);
+            sum[x & 1] += p;
+            // a masked token's p is zero whatever its block's scale
+            sc[i][nb][x] = sc[i][nb][x] == -INFINITY ? 0.f : p * vrel;
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t hi = pack_half(sc[i][nb][2 * y], sc[i][nb][2 * y + 1]);
+            pf[0][nb][2 * i + y] = transpose8(hi);
+            if constexpr (PARTS == 2) pf[1][nb][2 * i + y] = transpose8(pack_rest(sc[i][nb][2 * y], sc[i][nb][2 * y + 1], hi));
+          }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          pf[i][r] = pack_half(sc[i][2 * r], sc[i][2 * r + 1]);
-          if constexpr (PARTS == 2) pf[i][2 + r] = pack_rest(sc[i][2 * r], sc[i][2 * r + 1], pf[i][r]);
+        for (int x = 0; x < 2; ++x) {
+          l[nb][x] = l[nb][x] * alpha[nb][x] + sum[x];
+          alpha[nb][x] *= vstep;
         }
       }
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] = l[i] * alpha[i] + sum[i];
-        alpha[i] *= vstep;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+        for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[i][x] *= alpha[x >> 1];
+            for (int x = 0; x < 4; ++x) o[i][nb][x] *= alpha[nb][x & 1];
       }
       // ---- values; codes past the last visible token (or of a page that
       // could not be read) are whatever the memory holds, and count as zero
       wait(bars + NST + stage, (vphase >> stage) & 1);
       vphase ^= 1u << stage;
-      const int nv = have ? min(max(hi_tok - tok0, 0), 16) : 0;
-      const bool clip = __any_sync(0xffffffffu, nv < 16);
-      uint32_t vm[4];
+      const bool vhave = __shfl_sync(0xffffffffu, (int)have, 8 * qc) != 0;  // of tokens 8c .. 8c + 7
+      const int nv = vhave ? min(max(hi_tok - (tok0 + 8 * qc), 0), 8) : 0;
+      const bool clip = __any_sync(0xffffffffu, nv < 8);
+      const uint32_t vm0 = nv >= 4 ? 0xFFFFFFFFu : (1u << (8 * nv)) - 1u;
+      const uint32_t vm1 = nv >= 8 ? 0xFFFFFFFFu : nv <= 4 ? 0u : (1u << (8 * (nv - 4))) - 1u;
+      const int vtok = 32 * half + 8 * qc;
+      const uint8_t* vt = s_v + stage * vbytes + (vtok / blk) * (blk * D + 2 * blk) + gr * blk + vtok % blk;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int n = min(max(nv - 4 * s, 0), 4);
-        vm[s] = n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
-      }
-      const uint8_t* vt = s_v + stage * vbytes + (qc / per_page) * (blk * D + 2 * blk) + gr * blk + 16 * (qc % per_page);
+      for (int i = 0; i < DP / 16; ++i) {
+        if (16 * i >= D) break;
+        uint2 v0 = *reinterpret_cast<const uint2*>(vt + 16 * i * blk);
+        uint2 v1 = *reinterpret_cast<const uint2*>(vt + (16 * i + 8) * blk);
+        if (clip) {
+          v0.x &= vm0; v0.y &= vm1; v1.x &= vm0; v1.y &= vm1;
+        }
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
-        if (8 * i >= D) break;
-        const uint4 vb = *reinterpret_cast<const uint4*>(vt + 8 * i * blk);
-        uint32_t w4[4] = {vb.x, vb.y, vb.z, vb.w};
-        if (clip)
+        for (int y = 0; y < 2; ++y) {
+          uint32_t a0, a1, a2, a3;
+          widen<FMT>(y ? v0.y : v0.x, a0, a2);
+          widen<FMT>(y ? v1.y : v1.x, a1, a3);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) w4[s] &= vm[s];
+          for (int pt = 0; pt < PARTS; ++pt)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint32_t b0, b1;
-          widen<FMT>(w4[s], b0, b1);
-          mma_f16(o[i], pf[2 * s][0], pf[2 * s][1], pf[2 * s + 1][0], pf[2 * s + 1][1], b0, b1);
-          if constexpr (PARTS == 2)
-            mma_f16(o[i], pf[2 * s][2], pf[2 * s][3], pf[2 * s + 1][2], pf[2 * s + 1][3], b0, b1);
+            for (int nb = 0; nb < NB; ++nb) mma_f16(o[i][nb], a0, a1, a2, a3, pf[pt][nb][2 * y], pf[pt][nb][2 * y + 1]);
         }
       }
-      __syncwarp();  // every lane has read the stage
 #pragma unroll
       for (int i = 0; i + 1 < NST; ++i) {
         ks_s[i] = ks_s[i + 1];
         vs_s[i] = vs_s[i + 1];
         have_s[i] = have_s[i + 1];
       }
-      if (t + NST < te) issue(t + NST, stage, ks_s[NST - 1], vs_s[NST - 1], have_s[NST - 1]);
+      pair_sync(pair);  // both warps have read the stage
+      if (t + NST < te) {
+        if (half == 0) issue(t + NST, stage);
+        scales(t + NST, ks_s[NST - 1], vs_s[NST - 1], have_s[NST - 1]);
+      }
     }
 
-    // ---- the unit's result, or this warp's part of it
+    // ---- join the pair: the second warp hands its part to the first through
+    // the ring, which no copy is filling now
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) l[nb][x] += __shfl_xor_sync(0xffffffffu, l[nb][x], s);
+    if (tb >= te) pair_sync(pair);  // no tile parted this piece from the last one's join
+    if (half == 1) {
+      float* j = s_join + lane;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          j[(4 * nb + 2 * x) * 32] = m[nb][x];
+          j[(4 * nb + 2 * x + 1) * 32] = l[nb][x];
+        }
+      j[4 * NB * 32] = vref;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) j[(4 * NB + 1 + (i * NB + nb) * 4 + x) * 32] = o[i][nb][x];
     }
-    if (at == u0 && stop == u1) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = gr + 8 * i;
-        if (r >= nrows) continue;
-        const int e = 16 * rt + r, row = w.s.row0 + e / a.g, head = h * a.g + e % a.g;
-        const float f = l[i] == 0.f ? 0.f : vref / l[i];
-        T* op = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
-#pragma unroll
-        for (int d = 0; d < DP / 8; ++d) {
-          if (8 * d >= D) break;
-          op[8 * d + 2 * qc] = rope::from_f32<T>(o[d][2 * i] * f);
-          op[8 * d + 2 * qc + 1] = rope::from_f32<T>(o[d][2 * i + 1] * f);
-        }
-        if (a.lse != nullptr && qc == 0)
-          a.lse[(int64_t)row * a.Hq + head] =
-              l[i] == 0.f ? -INFINITY : (m[i] - kPShift + log2f(l[i])) * 0.69314718055994531f;
-      }
-    } else {
+    pair_sync(pair);
+    if (half == 0) {
+      const float* j = s_join + lane;
+      const float vref1 = j[4 * NB * 32];
+      const bool done = at == u0 && stop == u1;
       const int64_t slot = 2 * (int64_t)wid + (piece > 0 ? 1 : 0);
-      float* po = a.part_o + slot * 16 * D;
-      float* pm = a.part_ml + slot * 32;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = gr + 8 * i;
-        if (r >= nrows) continue;
-        if (qc == 0) {
-          pm[2 * r] = l[i] == 0.f ? -INFINITY : m[i];
-          pm[2 * r + 1] = l[i];
-        }
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int d = 0; d < DP / 8; ++d) {
-          if (8 * d >= D) break;
-          po[r * D + 8 * d + 2 * qc] = o[d][2 * i] * vref;
-          po[r * D + 8 * d + 2 * qc + 1] = o[d][2 * i + 1] * vref;
+        for (int x = 0; x < 2; ++x) {
+          const float m1 = j[(4 * nb + 2 * x) * 32], l1 = j[(4 * nb + 2 * x + 1) * 32];
+          const float mm = fmaxf(m[nb][x], m1);
+          // a side without visible tokens has m = -inf, l = 0 and o = 0
+          const float f0 = l[nb][x] == 0.f ? 0.f : exp2_approx(m[nb][x] - mm), f1 = l1 == 0.f ? 0.f : exp2_approx(m1 - mm);
+          const float ll = l[nb][x] * f0 + l1 * f1;
+          const int r = 8 * nb + 2 * qc + x;
+          if (r >= nrows) continue;
+          const int e = e0 + r, row = w.s.row0 + e / a.g, head = h * a.g + e % a.g;
+          const float inv = !done ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
+          const float g0 = f0 * vref * inv, g1 = f1 * vref1 * inv;
+          if (gr == 0) {
+            if (!done) {
+              a.part_ml[(slot * R + r) * 2] = ll == 0.f ? -INFINITY : mm;
+              a.part_ml[(slot * R + r) * 2 + 1] = ll;
+            } else if (a.lse != nullptr) {
+              a.lse[(int64_t)row * a.Hq + head] =
+                  ll == 0.f ? -INFINITY : (mm - kPShift + log2f(ll)) * 0.69314718055994531f;
+            }
+          }
+          T* op = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
+          float* po = a.part_o + (slot * R + r) * D;
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {
+            if (16 * i >= D) break;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int d = 16 * i + 8 * y + gr;
+              const float v = o[i][nb][2 * y + x] * g0 + j[(4 * NB + 1 + (i * NB + nb) * 4 + 2 * y + x) * 32] * g1;
+              if (done)
+                op[d] = rope::from_f32<T>(v);
+              else
+                po[d] = v;
+            }
+          }
         }
-      }
-      if (at == u0 && lane == 0) {
-        // the unit goes on past this warp: warps wid .. last hold its parts
-        // (the first warp whose share ends at or past u1)
-        const int lw = (int)((u1 * warps + total - 1) / total) - 1;
+      if (!done && at == u0 && lane == 0) {
+        // the unit goes on past this pair: pairs wid .. lw hold its parts
+        // (the first pair whose share ends at or past u1)
+        const int lw = (int)((u1 * pairs + total - 1) / total) - 1;
         a.desc[wid] = make_int4(sb, h, rt, (lw << 1) | (piece > 0 ? 1 : 0));
       }
+      // the next piece's copies overwrite what ordinary stores wrote
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
     }
     ++piece;
     at = stop;
   }
 }
 
-// Join the parts of one cut unit's row: block (warp that holds the first
-// part, row).  The first warp's part may be its last piece (slot 1); every
-// later warp's is its first (slot 0).
+// Join the parts of one cut unit's row: block (pair that holds the first
+// part, row).  The first pair's part may be its last piece (slot 1); every
+// later pair's is its first (slot 0).
 template <typename T>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   const int wid = blockIdx.x, r = blockIdx.y;
   const int4 d = a.desc[wid];
   if (d.x < 0) return;
   const kv::Seq s = kv::sequence(a.b, a.b.cu, a.b.lens, a.c.blk, d.x, nullptr);
-  const int e = 16 * d.z + r;
-  if (e >= s.n * a.g) return;
+  const int64_t e = (int64_t)a.rows * d.z + r;
+  if (e >= (int64_t)s.n * a.g) return;
   const int D = a.c.D, last = d.w >> 1;
   const int64_t slot0 = 2 * (int64_t)wid + (d.w & 1);
   float m = -INFINITY;
   for (int i = wid + threadIdx.x; i <= last; i += blockDim.x)
-    m = fmaxf(m, a.part_ml[(i == wid ? slot0 : 2 * (int64_t)i) * 32 + 2 * r]);
+    m = fmaxf(m, a.part_ml[((i == wid ? slot0 : 2 * (int64_t)i) * a.rows + r) * 2]);
   __shared__ float s_m[4];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
   __syncthreads();
   m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const int row = s.row0 + e / a.g, head = d.y * a.g + e % a.g;
+  const int row = s.row0 + (int)(e / a.g), head = d.y * a.g + (int)(e % a.g);
   T* op = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
   for (int c = threadIdx.x; c < D; c += blockDim.x) {
     float acc = 0.f, l = 0.f;
     for (int i = wid; i <= last; ++i) {
-      const int64_t slot = i == wid ? slot0 : 2 * (int64_t)i;
-      const float mi = a.part_ml[slot * 32 + 2 * r], li = a.part_ml[slot * 32 + 2 * r + 1];
+      const int64_t slot = (i == wid ? slot0 : 2 * (int64_t)i) * a.rows + r;
+      const float mi = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1];
       if (li == 0.f) continue;
       const float f = exp2_approx(mi - m);
       l += li * f;
-      acc += a.part_o[(slot * 16 + r) * D + c] * f;
+      acc += a.part_o[slot * D + c] * f;
     }
     op[c] = rope::from_f32<T>(l == 0.f ? 0.f : acc / l);
     if (a.lse != nullptr && c == 0)

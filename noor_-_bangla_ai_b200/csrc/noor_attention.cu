@@ -8,6 +8,8 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <initializer_list>
+#include <type_traits>
 
 #include "noor_moe.h"
 
@@ -275,31 +277,52 @@ int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* 
 namespace {
 
 struct StreamPlan {
-  int grid = 0, warps = 0;
+  int grid = 0, pairs = 0, nb = 1;
   int64_t off_ml = 0, off_desc = 0, bytes = 0;
 };
 
-int warps_per_block(int D, int dtype) {
-  const bool f32 = dtype == NOOR_DTYPE_F32;
-  if (D <= 64) return f32 ? attn::Shape<64, 2>::kWarps : attn::Shape<64, 1>::kWarps;
-  if (D <= 128) return f32 ? attn::Shape<128, 2>::kWarps : attn::Shape<128, 1>::kWarps;
-  return f32 ? attn::Shape<256, 2>::kWarps : attn::Shape<256, 1>::kWarps;
+// Calls f(head dims' bound, parts, column groups) as integral constants.
+template <typename F>
+int by_shape(int D, int dtype, int nb, F&& f) {
+  using std::integral_constant;
+  auto parts = [&](auto dp, auto n) -> int {
+    return dtype == NOOR_DTYPE_F32 ? f(dp, integral_constant<int, 2>{}, n) : f(dp, integral_constant<int, 1>{}, n);
+  };
+  if (D <= 64) {
+    integral_constant<int, 64> dp;
+    return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 4>{});
+  }
+  if (D <= 128) {
+    integral_constant<int, 128> dp;
+    return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 4>{});
+  }
+  integral_constant<int, 256> dp;
+  return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 2>{});
 }
 
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
-// have that many tiles.
-int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int dtype, StreamPlan* p) {
+// have that many tiles.  Up to 8 query rows for a kv head use one column group
+// of the mma; more use as many as the registers hold, so that a tile's codes
+// are widened once for 32 rows (16 at more than 128 dims).
+int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int dtype, StreamPlan* p) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
-  const int64_t g = Hq / c->n_kv_heads, per = warps_per_block(c->head_dim, dtype);
-  const int64_t rtiles = std::min(b->n_rows * g, b->n_rows * g / 16 + b->batch);
+  const int64_t g = Hq / c->n_kv_heads;
+  p->nb = max_rows * g <= 8 ? 1 : c->head_dim <= 128 ? 4 : 2;
+  const int64_t R = 8 * p->nb;
+  int per = 0;
+  CKR(by_shape(c->head_dim, dtype, p->nb, [&](auto dp, auto parts, auto nb) -> int {
+    per = attn::Shape<dp(), parts(), nb()>::kPairs;
+    return NOOR_MOE_OK;
+  }));
+  const int64_t rtiles = std::min(b->n_rows * g, b->n_rows * g / R + b->batch);
   const int64_t tiles = ((int64_t)b->max_blocks * c->block + attn::kTile - 1) / attn::kTile;
   const double most = (double)rtiles * c->n_kv_heads * tiles;
   p->grid = (int)std::min<double>(sms, std::max(1.0, most));
-  p->warps = p->grid * (int)per;
-  p->off_ml = (int64_t)p->warps * 2 * 16 * c->head_dim * 4;
-  p->off_desc = p->off_ml + (int64_t)p->warps * 2 * 32 * 4;
-  p->bytes = p->off_desc + (int64_t)p->warps * 16;
+  p->pairs = p->grid * per;
+  p->off_ml = (int64_t)p->pairs * 2 * R * c->head_dim * 4;
+  p->off_desc = p->off_ml + (int64_t)p->pairs * 2 * R * 2 * 4;
+  p->bytes = p->off_desc + (int64_t)p->pairs * 16;
   return NOOR_MOE_OK;
 }
 
@@ -309,22 +332,15 @@ int check_heads(const noor_kv_cache* c, int Hq) {
   return NOOR_MOE_OK;
 }
 
-template <int DP, int FMT, int PARTS>
+template <int DP, int FMT, int PARTS, int NB>
 int launch_stream(const attn::Args& a, int grid, cudaStream_t s) {
-  using Sh = attn::Shape<DP, PARTS>;
-  auto kern = attn::stream_kernel<DP, FMT, PARTS>;
+  using Sh = attn::Shape<DP, PARTS, NB>;
+  auto kern = attn::stream_kernel<DP, FMT, PARTS, NB>;
   const int smem = Sh::smem_bytes(a.c.D);
   CKR(ensure_smem_limit(kern, smem));
-  kern<<<grid, Sh::kWarps * 32, smem, s>>>(a);
+  kern<<<grid, Sh::kPairs * 64, smem, s>>>(a);
   CK(cudaGetLastError());
   return NOOR_MOE_OK;
-}
-
-template <int FMT, int PARTS>
-int launch_stream_d(const attn::Args& a, int grid, cudaStream_t s) {
-  if (a.c.D <= 64) return launch_stream<64, FMT, PARTS>(a, grid, s);
-  if (a.c.D <= 128) return launch_stream<128, FMT, PARTS>(a, grid, s);
-  return launch_stream<256, FMT, PARTS>(a, grid, s);
 }
 
 }  // namespace
@@ -340,7 +356,7 @@ int noor_kv_attention_workspace(const noor_kv_cache* c, const noor_kv_batch* b, 
     CKR(check_heads(c, q_heads));
     if (!bytes || max_rows < 0) return fail(NOOR_MOE_ERR_INVALID, "null bytes or negative max_rows");
     StreamPlan p;
-    CKR(stream_plan(c, b, q_heads, dtype, &p));
+    CKR(stream_plan(c, b, q_heads, max_rows, dtype, &p));
     *bytes = p.bytes;
     return NOOR_MOE_OK;
   });
@@ -360,7 +376,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     CKR(check_view(q, dtype, "q"));
     CKR(check_view(out, dtype, "out"));
     StreamPlan p;
-    CKR(stream_plan(c, b, q_heads, dtype, &p));
+    CKR(stream_plan(c, b, q_heads, max_rows, dtype, &p));
     if (!workspace || workspace_bytes < p.bytes)
       return fail(NOOR_MOE_ERR_INVALID, "workspace of %lld bytes, needs %lld", (long long)workspace_bytes,
                   (long long)p.bytes);
@@ -378,18 +394,19 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     a.g = q_heads / c->n_kv_heads;
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window;
-    a.warps = p.warps;
+    a.pairs = p.pairs;
+    a.rows = 8 * p.nb;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.desc = reinterpret_cast<int4*>(ws + p.off_desc);
-    if (dtype == NOOR_DTYPE_BF16)
-      CKR((c->format == NOOR_KV_INT8 ? launch_stream_d<kv::INT8, 1>(a, p.grid, s) : launch_stream_d<kv::E4M3, 1>(a, p.grid, s)));
-    else
-      CKR((c->format == NOOR_KV_INT8 ? launch_stream_d<kv::INT8, 2>(a, p.grid, s) : launch_stream_d<kv::E4M3, 2>(a, p.grid, s)));
+    CKR(by_shape(c->head_dim, dtype, p.nb, [&](auto dp, auto parts, auto nb) -> int {
+      return c->format == NOOR_KV_INT8 ? launch_stream<dp(), kv::INT8, parts(), nb()>(a, p.grid, s)
+                                       : launch_stream<dp(), kv::E4M3, parts(), nb()>(a, p.grid, s);
+    }));
     return by_dtype(dtype, [&](auto t) -> int {
-      const int64_t rows = std::min<int64_t>(16, b->n_rows * a.g);
-      attn::combine_kernel<decltype(t)><<<dim3((unsigned)p.warps, (unsigned)rows), 128, 0, s>>>(a);
+      const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g);
+      attn::combine_kernel<decltype(t)><<<dim3((unsigned)p.pairs, (unsigned)rows), 128, 0, s>>>(a);
       CK(cudaGetLastError());
       return NOOR_MOE_OK;
     });
