@@ -1,7 +1,8 @@
 """Build recipe for libnoor_moe.so (sm_100a), in-tree.
 
-One nvcc invocation compiles the kernels and the C ABI into a shared library
-next to this file; the CUDA runtime is linked statically, NCCL dynamically.
+nvcc compiles the sources side by side and links the kernels and the C ABI
+into a shared library next to this file; the CUDA runtime is linked statically,
+NCCL dynamically.
 The debug build libnoor_moe_check.so is the same source compiled with
 -DNOOR_CHECK: every data-dependent row index a kernel uses (permute
 destinations, peer receive rows, row-map outputs, combine gathers, the
@@ -15,13 +16,16 @@ import glob
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnoor_moe.so")
 LIB_CHECK = os.path.join(HERE, "libnoor_moe_check.so")
-SOURCES = ["noor_moe.cu", "noor_attention.cu"]
+SOURCES = ["noor_moe.cu", "noor_attention.cu", "kv_stream_bf16_int8.cu", "kv_stream_bf16_e4m3.cu",
+           "kv_stream_f32_int8.cu", "kv_stream_f32_e4m3.cu", "kv_prompt.cu"]
 
 
 def headers() -> list:
@@ -33,7 +37,7 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "--expt-relaxed-constexpr",
     "-Xcompiler", "-fPIC,-O3,-fvisibility=hidden",
-    "-shared", "-cudart", "static",
+    "-cudart", "static",
 ]
 
 
@@ -59,11 +63,22 @@ def build(force: bool = False, verbose: bool = False, extra=(), check: bool = Fa
     if not force and not stale(lib):
         return lib
     defs = ["-DNOOR_CHECK"] if check else []
-    cmd = [nvcc(), *NVCC_FLAGS, *defs, *extra, "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-           "-o", lib + ".tmp", *[os.path.join(CSRC, f) for f in SOURCES], "-ldl"]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+    with tempfile.TemporaryDirectory() as tmp:
+        def compile_one(src):
+            obj = os.path.join(tmp, src + ".o")
+            cmd = [nvcc(), *NVCC_FLAGS, *defs, *extra, "-I", os.path.join(ROOT, "include"), "-I", CSRC,
+                   "-c", "-o", obj, os.path.join(CSRC, src)]
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            subprocess.run(cmd, check=True)
+            return obj
+
+        with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+            objs = list(ex.map(compile_one, SOURCES))
+        cmd = [nvcc(), *NVCC_FLAGS, "-shared", "-o", lib + ".tmp", *objs, "-ldl"]
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        subprocess.run(cmd, check=True)
     os.replace(lib + ".tmp", lib)
     return lib
 

@@ -65,6 +65,7 @@ struct Args {
                    // last pair << 1 | slot of its part)
   int32_t pairs;   // warp pairs of the grid that share the work
   int32_t rows;    // query rows of a row tile
+  int64_t min_e, max_e;  // sequences with min_e <= rows * g < max_e are this launch's
 };
 
 // ------------------------------------------------------------ mma pieces
@@ -131,6 +132,8 @@ __device__ __forceinline__ SeqWork seq_work(const Args& a, int i) {
   SeqWork w;
   w.s = kv::sequence(a.b, a.b.cu, a.b.lens, a.c.blk, i, a.c.status);
   if (w.s.n > 0 && w.s.len < w.s.n) kv::flag(a.c.status, NOOR_KV_BAD_LENGTH);
+  const int64_t e = (int64_t)w.s.n * a.g;
+  if (e < a.min_e || e >= a.max_e) w.s.n = 0;
   w.rtiles = (int)(((int64_t)w.s.n * a.g + a.rows - 1) / a.rows);
   // rows at negative positions see nothing; at least one tile, so that rows
   // which see nothing are written too

@@ -12,6 +12,7 @@
 
 #include <cuda_fp8.h>
 #include "common.cuh"
+#include "noor_moe.h"
 #include "rope.cuh"
 
 namespace noor {

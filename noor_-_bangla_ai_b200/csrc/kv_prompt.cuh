@@ -1,0 +1,563 @@
+// kv_prompt.cuh -- attention over the 8-bit cache for many query rows, on
+// tcgen05 tensor cores (BF16 activations, head_dim up to 128).
+//
+// A block takes one unit: 256 rows (query row, query head of the group) of one
+// kv head, as two row tiles of 128, and all their visible tokens in tiles of
+// 128.  The same sums as the streamed kernel (kv_attention.cuh):
+//   s = q.k (f16 codes and f16 queries, f32 sums), p = 2^(s f - m + shift) in
+//   f16, o += p v, with f = scale log2(e) 2^e(row) k scale(block).
+// Roles:
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, a thread for each row
+//   warps 8-11      widen: codes in shared memory -> f16 operand tiles
+//   warp 12         one thread issues the mma's; the warp owns TMEM
+//   warp 13         loader: page table, scales, bulk copies of raw pages
+// TMEM (512 columns): S of both row tiles (2 x 128; p overwrites its own s as
+// f16 and is read from there as the second product's first operand), o of both.
+// While one row tile's softmax runs, the tensor core does the other's p v and
+// next q k.  Both operand layouts are the cache's own (k rows and v columns
+// contiguous along the contraction), so widening copies straight across into
+// the 128-byte-swizzled tiles.
+//
+// m is a reference that follows the row's maximum lazily: o is rescaled only
+// when the maximum has grown by more than 2^8, so most tiles never touch o.
+// p <= 2^15 then fits f16; shift 7 keeps p down to 2^-31 of the largest.
+// A block's v scale is applied while widening, relative to the largest v scale
+// of the unit's pages (exact for powers of two).
+#pragma once
+
+#include "kv_attention.cuh"
+
+namespace noor {
+namespace prompt {
+
+using attn::Args;
+
+constexpr int kThreads = 448;
+constexpr int kTok = 128;    // tokens of a tile
+constexpr float kShift = 7.0f, kLazy = 8.0f;
+constexpr int kMeta = 4;     // tiles of block factors in flight
+
+template <int DP>
+struct Smem {
+  static constexpr int kQ = 128 * DP * 2;      // one row tile, f16
+  static constexpr int kK = kTok * DP * 2;     // one token tile, f16
+  static constexpr int kRaw = kTok * DP;       // one token tile of codes
+  static constexpr int kBytes = 2 * kQ + 4 * kK + 2 * kRaw + 1024;  // + alignment
+};
+
+struct Bars {
+  uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], s_full[2], p_full[2],
+      o_full[2], drain;
+};
+
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 16-byte piece `chunk` of row `row` in a 128-byte-swizzled block.
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
+  return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+template <int DP, int FMT>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
+  using S = Smem<DP>;
+  extern __shared__ uint8_t s_raw_base[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(s_raw_base) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;                    // [2][DP / 64][128 rows][128 B]
+  uint8_t* s_k = s_q + 2 * S::kQ;         // [2 slots][DP / 64][128 tokens][128 B]
+  uint8_t* s_v = s_k + 2 * S::kK;         // [2 slots][2][DP dims][128 B]
+  uint8_t* s_rk = s_v + 2 * S::kK;        // raw pages
+  uint8_t* s_rv = s_rk + S::kRaw;
+  __shared__ __align__(8) Bars bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ uint32_t s_vref;
+  __shared__ float s_kf[kMeta][8], s_vf[kMeta][8];  // factors of each 16 tokens
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int D = a.c.D, blk = a.c.blk;
+
+  // ---- the block's unit: last row tiles first, they see the most tokens
+  const int h = blockIdx.x % a.c.H;
+  int sb = -1, rt = 0;
+  {
+    int32_t before = 0;
+    const int32_t t = blockIdx.x / a.c.H;
+    for (int base = 0; base < a.b.B && sb < 0; base += 32) {
+      int32_t n = 0;
+      if (base + lane < a.b.B) n = attn::seq_work(a, base + lane).rtiles;
+      int32_t incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > t);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        sb = base + src;
+        rt = before + __shfl_sync(0xffffffffu, incl, src) - 1 - t;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  if (sb < 0) return;
+  const attn::SeqWork w = attn::seq_work(a, sb);
+  const int e0 = 256 * rt, nrows = min(256, w.s.n * a.g - e0), nw = nrows > 128 ? 2 : 1;
+  const int pos0 = w.s.len - w.s.n;
+  const int p_first = pos0 + e0 / a.g, p_last = pos0 + (e0 + nrows - 1) / a.g;
+  const int lo_tok = a.window > 0 ? max(p_first - a.window, 0) : 0, hi_tok = p_last + 1;
+  const int tb = lo_tok / kTok, te = (hi_tok + kTok - 1) / kTok, T = max(te - tb, 0);
+  const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bar.raw_full[i], 1);
+      tc::mbar_init(&bar.raw_empty[i], 4);
+      tc::mbar_init(&bar.k_full[i], 4);
+      tc::mbar_init(&bar.k_empty[i], 1);
+      tc::mbar_init(&bar.v_full[i], 4);
+      tc::mbar_init(&bar.v_empty[i], 1);
+      tc::mbar_init(&bar.q_full[i], 4);
+      tc::mbar_init(&bar.s_full[i], 1);
+      tc::mbar_init(&bar.p_full[i], 4);
+      tc::mbar_init(&bar.o_full[i], 1);
+    }
+    tc::mbar_init(&bar.drain, 1);
+    abort_flag = 0;
+    s_vref = 0x00800000u;  // the smallest normal number
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    async_fence();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(&tmem_slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // largest finite v scale of the unit's pages
+  {
+    uint32_t mx = 0;
+    for (int64_t p = lo_tok / blk + threadIdx.x; p * blk < hi_tok; p += kThreads) {
+      const int32_t page = __ldg(table + p);
+      if (page >= 0 && (int64_t)page < a.c.P) {
+        const uint32_t b = __float_as_uint(fabsf(__ldg(a.c.vs + (int64_t)page * a.c.H + h)));
+        if (b < 0x7F800000u) mx = max(mx, b);
+      }
+    }
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) atomicMax(&s_vref, mx);
+  }
+  __syncthreads();
+
+  // Bounded wait: false once a wait anywhere in the block gave up.
+  auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+    if (tc::mbar_try_wait(b, parity)) return true;
+    const long long start = clock64();
+    while (true) {
+      if (tc::mbar_try_wait(b, parity)) return true;
+      if (abort_flag) return false;
+      if (clock64() - start > kWaitLimitCycles) {
+        abort_flag = 1;
+        kv::flag(a.c.status, NOOR_KV_TIMEOUT);
+        return false;
+      }
+    }
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------- softmax
+    const int wg = warp >> 2, r = (warp & 3) * 32 + lane;  // row of this row tile
+    const int e = e0 + 128 * wg + r;
+    const bool live = 128 * wg + r < nrows;
+    const int row = w.s.row0 + e / a.g, head = h * a.g + e % a.g;
+    const int pos = live ? pos0 + e / a.g : -1;
+    const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128u * wg, t_o = t_s + 256u;
+    if (wg < nw) {
+      // the row's queries, scaled by a power of two (negative if the scale is)
+      // so that the largest is in 2^14 .. 2^15
+      const bf16* qp = static_cast<const bf16*>(a.q.p) + (int64_t)row * a.q.st + (int64_t)head * a.q.sh;
+      const bool vec = (reinterpret_cast<uintptr_t>(a.q.p) | (uintptr_t)(a.q.st * 2) | (uintptr_t)(a.q.sh * 2)) % 16 == 0;
+      auto load8 = [&](int d, float (&v)[8]) {
+        if (vec) {
+          rope::Vec<bf16>::load(qp + d, v);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = __bfloat162float(qp[d + x]);
+        }
+      };
+      float mx = 0.f;
+      if (live)
+        for (int d = 0; d < D; d += 8) {
+          float v[8];
+          load8(d, v);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(v[x]));
+        }
+      const int ex = max(min((int)(__float_as_uint(mx) >> 23) - 127, 127), -112);
+      float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+      const float fac = fabsf(a.scale2) * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
+      if (a.scale2 < 0.f) up = -up;
+      for (int d = 0; d < D; d += 8) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (live) load8(d, v);
+        uint4 u;
+        u.x = attn::pack_half(v[0] * up, v[1] * up);
+        u.y = attn::pack_half(v[2] * up, v[3] * up);
+        u.z = attn::pack_half(v[4] * up, v[5] * up);
+        u.w = attn::pack_half(v[6] * up, v[7] * up);
+        *reinterpret_cast<uint4*>(s_q + wg * S::kQ + (d >> 6) * (128 * 128) + swizzled(r, (d & 63) >> 3)) = u;
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.q_full[wg]);
+
+      // rows of this row tile, for the tiles that need no mask
+      const int wfirst = pos0 + (e0 + 128 * wg) / a.g;
+      const int wlast = pos0 + (e0 + min(128 * wg + 127, nrows - 1)) / a.g;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int i = 0; i < T && ok; ++i) {
+        const int tok0 = (tb + i) * kTok;
+        const bool whole = tok0 + kTok - 1 <= wfirst && (a.window <= 0 || wlast - tok0 <= a.window);
+        // visible columns of this row
+        const int chi = min(pos - tok0, kTok - 1), clo = a.window > 0 ? pos - a.window - tok0 : 0;
+        ok = __all_sync(0xffffffffu, wait(&bar.s_full[wg], i & 1));
+        if (!ok) break;
+        tc::tc_fence_after();
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = s_kf[i % kMeta][j] * fac;
+        float mx2 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32];
+          tc::tmem_ld32(t_s + 32 * c, s);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float g = -INFINITY;
+            if (whole) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) g = fmaxf(g, __uint_as_float(s[16 * y + x]));
+            } else {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const int col = 32 * c + 16 * y + x;
+                g = fmaxf(g, col >= clo && col <= chi ? __uint_as_float(s[16 * y + x]) : -INFINITY);
+              }
+            }
+            // (nothing visible: -inf, whatever the factor)
+            mx2 = fmaxf(mx2, g == -INFINITY ? -INFINITY : g * f[2 * c + y]);
+          }
+        }
+        const bool grow = mx2 > m + kLazy || (m == -INFINITY && mx2 > -INFINITY);
+        if (i == 0) {
+          m = mx2;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          // (o holds all earlier tiles: its last product ran before this s)
+          const float alpha = grow ? attn::exp2_approx(m - mx2) : 1.f;
+          if (grow) m = mx2;
+          l *= alpha;
+          for (int c = 0; c < D; c += 16) {
+            uint32_t v[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                  "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(t_o + c));
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * alpha);
+            tmem_st16(t_o + c, v);
+          }
+        }
+        const float mref = m == -INFINITY ? 0.f : m - kShift;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32], p[16];
+          tc::tmem_ld32(t_s + 32 * c, s);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            float p0 = attn::exp2_approx(fmaf(__uint_as_float(s[x]), f[2 * c + (x >> 4)], -mref));
+            float p1 = attn::exp2_approx(fmaf(__uint_as_float(s[x + 1]), f[2 * c + (x >> 4)], -mref));
+            if (!whole) {
+              const int col = 32 * c + x;
+              p0 = col >= clo && col <= chi ? p0 : 0.f;
+              p1 = col + 1 >= clo && col + 1 <= chi ? p1 : 0.f;
+            }
+            l += p0 + p1;
+            p[x >> 1] = attn::pack_half(p0, p1);
+          }
+          // columns 16 c .. of p lie over scores that were read already
+          tmem_st16(t_s + 16 * c, p);
+        }
+        tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bar.p_full[wg]);
+      }
+      if (ok && T > 0) {
+        ok = __all_sync(0xffffffffu, wait(&bar.o_full[wg], 0));
+        tc::tc_fence_after();
+      }
+      if (ok) {
+        const float inv = l == 0.f ? 0.f : 1.f / l * __uint_as_float(s_vref);
+        bf16* op = static_cast<bf16*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
+        const bool ovec = (reinterpret_cast<uintptr_t>(a.out.p) | (uintptr_t)(a.out.st * 2) | (uintptr_t)(a.out.sh * 2)) % 16 == 0;
+        for (int c = 0; c < D; c += 16) {
+          uint32_t v[16];
+          if (T > 0) {
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                  "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(t_o + c));
+            tc::tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) v[x] = 0;
+          }
+          float z[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) z[x] = __uint_as_float(v[x]) * inv;
+          if (live && ovec) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              *reinterpret_cast<uint4*>(op + c + 8 * y) =
+                  make_uint4(pack_bf16(z[8 * y], z[8 * y + 1]), pack_bf16(z[8 * y + 2], z[8 * y + 3]),
+                             pack_bf16(z[8 * y + 4], z[8 * y + 5]), pack_bf16(z[8 * y + 6], z[8 * y + 7]));
+          } else if (live) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) op[c + x] = __float2bfloat16_rn(z[x]);
+          }
+          __syncwarp();
+        }
+        if (live && a.lse != nullptr)
+          a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * 0.69314718055994531f;
+      }
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------- widen
+    const int th = threadIdx.x - 256;  // 0 .. 127
+    const int pieces = D >> 4;         // 16-byte pieces of a key row
+    bool ok = true;
+    for (int i = 0; i < T && ok; ++i) {
+      const int slot = i & 1;
+      const uint32_t ph = (i >> 1) & 1;
+      // keys: piece p of a row becomes chunks 2 p, 2 p + 1 of its 64-dim blocks
+      ok = __all_sync(0xffffffffu, wait(&bar.raw_full[0], i & 1) && wait(&bar.k_empty[slot], ph ^ 1));
+      if (!ok) break;
+      uint8_t* dk = s_k + slot * S::kK;
+      for (int x = th; x < kTok * pieces; x += 128) {
+        const int row = x / pieces, p = x - row * pieces;
+        const uint4 c = *reinterpret_cast<const uint4*>(s_rk + row * D + 16 * p);
+        uint4 u, v;
+        attn::widen<FMT>(c.x, u.x, u.y);
+        attn::widen<FMT>(c.y, u.z, u.w);
+        attn::widen<FMT>(c.z, v.x, v.y);
+        attn::widen<FMT>(c.w, v.z, v.w);
+        uint8_t* base = dk + (p >> 2) * (kTok * 128);
+        const int ch = 2 * (p & 3), first = (p >> 2) & 1;  // the order in which banks do not meet
+        *reinterpret_cast<uint4*>(base + swizzled(row, ch + first)) = first ? v : u;
+        *reinterpret_cast<uint4*>(base + swizzled(row, ch + (first ^ 1))) = first ? u : v;
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(&bar.k_full[slot]);
+        tc::mbar_arrive(&bar.raw_empty[0]);
+      }
+      // values: 16 tokens of a dim become chunks 2 q, 2 q + 1 of its 64-token block
+      ok = __all_sync(0xffffffffu, wait(&bar.raw_full[1], i & 1) && wait(&bar.v_empty[slot], ph ^ 1));
+      if (!ok) break;
+      uint8_t* dv = s_v + slot * S::kK;
+      const int tok0 = (tb + i) * kTok;
+      for (int x = th; x < D * 8; x += 128) {
+        const int d = x >> 3, q = x & 7;
+        const float vf = s_vf[i % kMeta][q];
+        uint4 u = make_uint4(0, 0, 0, 0), v = u;
+        if (vf != 0.f) {
+          uint4 c = *reinterpret_cast<const uint4*>(s_rv + (16 * q / blk) * (blk * D) + d * blk + 16 * q % blk);
+          const int nv = hi_tok - (tok0 + 16 * q);
+          if (nv < 16) {  // codes past the last visible token count as zero
+            uint32_t* cw = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int n = min(max(nv - 4 * y, 0), 4);
+              cw[y] &= n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+            }
+          }
+          attn::widen<FMT>(c.x, u.x, u.y);
+          attn::widen<FMT>(c.y, u.z, u.w);
+          attn::widen<FMT>(c.z, v.x, v.y);
+          attn::widen<FMT>(c.w, v.z, v.w);
+          if (vf != 1.f) {
+            const __half2 hf = __float2half2_rn(vf);
+            uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
+            uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const __half2 ua = __hmul2(*reinterpret_cast<__half2*>(uw + y), hf), va = __hmul2(*reinterpret_cast<__half2*>(vw + y), hf);
+              uw[y] = *reinterpret_cast<const uint32_t*>(&ua);
+              vw[y] = *reinterpret_cast<const uint32_t*>(&va);
+            }
+          }
+        }
+        uint8_t* base = dv + (q >> 2) * (DP * 128);
+        const int ch = 2 * (q & 3), first = (q >> 2) & 1;
+        *reinterpret_cast<uint4*>(base + swizzled(d, ch + first)) = first ? v : u;
+        *reinterpret_cast<uint4*>(base + swizzled(d, ch + (first ^ 1))) = first ? u : v;
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) {
+        tc::mbar_arrive(&bar.v_full[slot]);
+        tc::mbar_arrive(&bar.raw_empty[1]);
+      }
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------- mma
+    if (lane == 0 && T > 0) {
+      // f16 operands, f32 sums, both K-major, M 128, N 128 tokens or D dims
+      const uint32_t id_s = (1u << 4) | ((uint32_t)(kTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      bool issued = false;
+      auto scores = [&](int wg, int slot) {
+        const uint32_t q0 = tc::smem_addr(s_q + wg * S::kQ), k0 = tc::smem_addr(s_k + slot * S::kK);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+          tc::umma_bf16(tmem + 128u * wg, tc::sdesc_sw128(q0 + off), tc::sdesc_sw128(k0 + off), id_s, ks != 0);
+        }
+        issued = true;
+        tc::umma_commit(&bar.s_full[wg]);
+      };
+      bool ok = true;
+      for (int wg = 0; wg < nw && ok; ++wg) ok = wait(&bar.q_full[wg], 0);
+      if (ok) ok = wait(&bar.k_full[0], 0);
+      if (ok) {
+        tc::tc_fence_after();
+        for (int wg = 0; wg < nw; ++wg) scores(wg, 0);
+        tc::umma_commit(&bar.k_empty[0]);
+      }
+      for (int i = 0; i < T && ok; ++i) {
+        const int slot = i & 1, next = slot ^ 1;
+        for (int wg = 0; wg < nw && ok; ++wg) {
+          ok = wait(&bar.p_full[wg], i & 1) && (wg > 0 || wait(&bar.v_full[slot], (i >> 1) & 1));
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t v0 = tc::smem_addr(s_v + slot * S::kK);
+#pragma unroll
+          for (int ks = 0; ks < kTok / 16; ++ks)
+            umma_ts(tmem + 256u + 128u * wg, tmem + 128u * wg + 8u * ks,
+                    tc::sdesc_sw128(v0 + (ks >> 2) * (DP * 128) + (ks & 3) * 32), id_o, (i | ks) != 0);
+          if (wg == nw - 1) tc::umma_commit(&bar.v_empty[slot]);
+          if (i + 1 < T) {
+            if (wg == 0) {
+              ok = wait(&bar.k_full[next], ((i + 1) >> 1) & 1);
+              if (!ok) break;
+              tc::tc_fence_after();
+            }
+            scores(wg, next);
+            if (wg == nw - 1) tc::umma_commit(&bar.k_empty[next]);
+          } else {
+            tc::umma_commit(&bar.o_full[wg]);
+          }
+        }
+      }
+      if (issued) {  // every mma retires before TMEM is released
+        tc::umma_commit(&bar.drain);
+        const long long start = clock64();
+        while (!tc::mbar_try_wait(&bar.drain, 0) && clock64() - start < kWaitLimitCycles) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------- loader
+    const int pages = kTok / blk;
+    const uint32_t bytes = (uint32_t)blk * D;
+    const float vref = __uint_as_float(s_vref), nan = __uint_as_float(0x7FC00000u);
+    int issued = 0;  // tiles whose copies were issued (k, and v one step later)
+    bool ok = true, vpending = false;
+    for (int i = 0; i < T && ok; ++i) {
+      const int tok0 = (tb + i) * kTok;
+      int32_t page = -1;
+      if (lane < pages && tok0 + lane * blk < hi_tok) {
+        page = __ldg(table + tok0 / blk + lane);
+        if (page < 0 || (int64_t)page >= a.c.P) {
+          kv::flag(a.c.status, NOOR_KV_BAD_PAGE);
+          page = -1;
+        }
+      }
+      const int64_t ph = (int64_t)page * a.c.H + h;
+      // factors of each 16 tokens: NaN where the page or its values cannot be
+      // read (the rows that see them come out NaN), values then zero
+      float ks = page >= 0 ? __ldg(a.c.ks + ph) : nan, vs = page >= 0 ? __ldg(a.c.vs + ph) : nan;
+      const int src = (16 * (lane & 7)) / blk;
+      ks = __shfl_sync(0xffffffffu, ks, src);
+      vs = __shfl_sync(0xffffffffu, vs, src);
+      const bool fin = fabsf(vs) <= 3.4028235e38f;
+      ok = wait(&bar.raw_empty[0], (i & 1) ^ 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane < 8) {
+        s_kf[i % kMeta][lane] = fin ? ks : nan;
+        s_vf[i % kMeta][lane] = fin ? vs / vref : 0.f;
+      }
+      const unsigned who = __ballot_sync(0xffffffffu, page >= 0);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_expect_tx(&bar.raw_full[0], __popc(who) * bytes);
+      __syncwarp();
+      if (page >= 0) attn::bulk_load(s_rk + lane * bytes, a.c.k + ph * bytes, bytes, &bar.raw_full[0]);
+      issued = i + 1;
+      vpending = true;
+      ok = wait(&bar.raw_empty[1], (i & 1) ^ 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) tc::mbar_arrive_expect_tx(&bar.raw_full[1], __popc(who) * bytes);
+      __syncwarp();
+      if (page >= 0) attn::bulk_load(s_rv + lane * bytes, a.c.v + ph * bytes, bytes, &bar.raw_full[1]);
+      vpending = false;
+    }
+    if (!ok && lane == 0 && issued > 0) {  // gave up: the copies in flight land before the block ends
+      const long long start = clock64();
+      while (!tc::mbar_try_wait(&bar.raw_full[0], (issued - 1) & 1) && clock64() - start < kWaitLimitCycles) {
+      }
+      const int v = vpending ? issued - 1 : issued;
+      while (v > 0 && !tc::mbar_try_wait(&bar.raw_full[1], (v - 1) & 1) && clock64() - start < kWaitLimitCycles) {
+      }
+    }
+    __syncwarp();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace prompt
+}  // namespace noor

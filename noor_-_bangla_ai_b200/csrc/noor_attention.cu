@@ -17,6 +17,7 @@
 #include "host.h"
 #include "kv_attention.cuh"
 #include "kv_cache.cuh"
+#include "kv_stream.h"
 #include "rope.cuh"
 
 using namespace noor;
@@ -281,25 +282,6 @@ struct StreamPlan {
   int64_t off_ml = 0, off_desc = 0, bytes = 0;
 };
 
-// Calls f(head dims' bound, parts, column groups) as integral constants.
-template <typename F>
-int by_shape(int D, int dtype, int nb, F&& f) {
-  using std::integral_constant;
-  auto parts = [&](auto dp, auto n) -> int {
-    return dtype == NOOR_DTYPE_F32 ? f(dp, integral_constant<int, 2>{}, n) : f(dp, integral_constant<int, 1>{}, n);
-  };
-  if (D <= 64) {
-    integral_constant<int, 64> dp;
-    return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 4>{});
-  }
-  if (D <= 128) {
-    integral_constant<int, 128> dp;
-    return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 4>{});
-  }
-  integral_constant<int, 256> dp;
-  return nb == 1 ? parts(dp, integral_constant<int, 1>{}) : parts(dp, integral_constant<int, 2>{});
-}
-
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
 // have that many tiles.  Up to 8 query rows for a kv head use one column group
 // of the mma; more use as many as the registers hold, so that a tile's codes
@@ -311,8 +293,8 @@ int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_
   p->nb = max_rows * g <= 8 ? 1 : c->head_dim <= 128 ? 4 : 2;
   const int64_t R = 8 * p->nb;
   int per = 0;
-  CKR(by_shape(c->head_dim, dtype, p->nb, [&](auto dp, auto parts, auto nb) -> int {
-    per = attn::Shape<dp(), parts(), nb()>::kPairs;
+  CKR(attn::by_shape(c->head_dim, p->nb, [&](auto dp, auto nb) -> int {
+    per = dtype == NOOR_DTYPE_F32 ? attn::Shape<dp(), 2, nb()>::kPairs : attn::Shape<dp(), 1, nb()>::kPairs;
     return NOOR_MOE_OK;
   }));
   const int64_t rtiles = std::min(b->n_rows * g, b->n_rows * g / R + b->batch);
@@ -326,20 +308,18 @@ int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_
   return NOOR_MOE_OK;
 }
 
+// Rows (times query heads of a group) from which a sequence runs on the
+// tensor-core kernel.
+constexpr int64_t kPromptRows = 128;
+
+bool prompt_fits(const noor_kv_cache* c, const noor_kv_batch* b, int g, int max_rows, int dtype) {
+  return dtype == NOOR_DTYPE_BF16 && c->head_dim <= 128 && (int64_t)max_rows * g >= kPromptRows &&
+         b->n_rows * g >= kPromptRows;
+}
+
 int check_heads(const noor_kv_cache* c, int Hq) {
   if (Hq <= 0 || Hq > 65536 || Hq % c->n_kv_heads != 0)
     return fail(NOOR_MOE_ERR_INVALID, "%d query heads over %d kv heads", Hq, c->n_kv_heads);
-  return NOOR_MOE_OK;
-}
-
-template <int DP, int FMT, int PARTS, int NB>
-int launch_stream(const attn::Args& a, int grid, cudaStream_t s) {
-  using Sh = attn::Shape<DP, PARTS, NB>;
-  auto kern = attn::stream_kernel<DP, FMT, PARTS, NB>;
-  const int smem = Sh::smem_bytes(a.c.D);
-  CKR(ensure_smem_limit(kern, smem));
-  kern<<<grid, Sh::kPairs * 64, smem, s>>>(a);
-  CK(cudaGetLastError());
   return NOOR_MOE_OK;
 }
 
@@ -396,14 +376,27 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     a.window = window;
     a.pairs = p.pairs;
     a.rows = 8 * p.nb;
+    a.min_e = 0;
+    a.max_e = INT64_MAX;
+    // Sequences with many rows go to the tensor-core kernel, the others to the
+    // streamed one (only the device knows which a batch has).
+    if (prompt_fits(c, b, a.g, max_rows, dtype)) {
+      attn::Args t = a;
+      t.rows = 256;
+      t.min_e = kPromptRows;
+      const int64_t units = std::min(b->n_rows * a.g, b->n_rows * a.g / 256 + b->batch) * c->n_kv_heads;
+      if (units > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
+      CKR(c->format == NOOR_KV_INT8 ? attn::prompt_int8(t, (int)units, s) : attn::prompt_e4m3(t, (int)units, s));
+      a.max_e = kPromptRows;
+    }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.desc = reinterpret_cast<int4*>(ws + p.off_desc);
-    CKR(by_shape(c->head_dim, dtype, p.nb, [&](auto dp, auto parts, auto nb) -> int {
-      return c->format == NOOR_KV_INT8 ? launch_stream<dp(), kv::INT8, parts(), nb()>(a, p.grid, s)
-                                       : launch_stream<dp(), kv::E4M3, parts(), nb()>(a, p.grid, s);
-    }));
+    if (dtype == NOOR_DTYPE_BF16)
+      CKR(c->format == NOOR_KV_INT8 ? attn::stream_bf16_int8(a, p.nb, p.grid, s) : attn::stream_bf16_e4m3(a, p.nb, p.grid, s));
+    else
+      CKR(c->format == NOOR_KV_INT8 ? attn::stream_f32_int8(a, p.nb, p.grid, s) : attn::stream_f32_e4m3(a, p.nb, p.grid, s));
     return by_dtype(dtype, [&](auto t) -> int {
       const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g);
       attn::combine_kernel<decltype(t)><<<dim3((unsigned)p.pairs, (unsigned)rows), 128, 0, s>>>(a);
