@@ -70,6 +70,33 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // 16-byte piece `chunk` of row `row` in a 128-byte-swizzled block.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
@@ -175,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     if (tc::mbar_try_wait(b, parity)) return true;
     const long long start = clock64();
     while (true) {
-      if (tc::mbar_try_wait(b, parity)) return true;
+      if (tc::mbar_try_wait_sleep(b, parity)) return true;
       if (abort_flag) return false;
       if (clock64() - start > kWaitLimitCycles) {
         abort_flag = 1;
@@ -237,29 +264,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       const int wlast = pos0 + (e0 + min(128 * wg + 127, nrows - 1)) / a.g;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int i = 0; i < T && ok; ++i) {
-        const int tok0 = (tb + i) * kTok;
-        const bool whole = tok0 + kTok - 1 <= wfirst && (a.window <= 0 || wlast - tok0 <= a.window);
-        // visible columns of this row
-        const int chi = min(pos - tok0, kTok - 1), clo = a.window > 0 ? pos - a.window - tok0 : 0;
-        ok = __all_sync(0xffffffffu, wait(&bar.s_full[wg], i & 1));
-        if (!ok) break;
-        tc::tc_fence_after();
+      // One tile's scores to probabilities, compiled apart for tiles that every
+      // row sees whole: a test for each score costs more than its exponential.
+      auto tile = [&](auto all, int i, int clo, int chi) {
+        constexpr bool whole = decltype(all)::value;
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = s_kf[i % kMeta][j] * fac;
         float mx2 = -INFINITY;
+        uint32_t sb2[2][32];  // the next 32 columns load while these are worked on
+        tc::tmem_ld32(t_s, sb2[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          tc::tmem_ld32(t_s + 32 * c, s);
           tc::tmem_ld_wait();
+          tc::tmem_ld32(t_s + 32 * ((c + 1) & 3), sb2[(c + 1) & 1]);  // (the last: the second pass's first)
+          const uint32_t* s = sb2[c & 1];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             float g = -INFINITY;
-            if (whole) {
+            if constexpr (whole) {
 #pragma unroll
-              for (int x = 0; x < 16; ++x) g = fmaxf(g, __uint_as_float(s[16 * y + x]));
+              for (int x = 0; x < 16; x += 2)
+                g = max3(g, __uint_as_float(s[16 * y + x]), __uint_as_float(s[16 * y + x + 1]));
             } else {
 #pragma unroll
               for (int x = 0; x < 16; ++x) {
@@ -293,30 +319,50 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           }
         }
         const float mref = m == -INFINITY ? 0.f : m - kShift;
+        const uint64_t neg = pair2(-mref, -mref);
+        uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t s[32], p[16];
-          tc::tmem_ld32(t_s + 32 * c, s);
+          uint32_t p[16];
           tc::tmem_ld_wait();
+          if (c < 3) tc::tmem_ld32(t_s + 32 * (c + 1), sb2[(c + 1) & 1]);
+          const uint32_t* s = sb2[c & 1];
 #pragma unroll
           for (int x = 0; x < 32; x += 2) {
-            float p0 = attn::exp2_approx(fmaf(__uint_as_float(s[x]), f[2 * c + (x >> 4)], -mref));
-            float p1 = attn::exp2_approx(fmaf(__uint_as_float(s[x + 1]), f[2 * c + (x >> 4)], -mref));
-            if (!whole) {
+            const float fj = f[2 * c + (x >> 4)];
+            float2 z = split2(fma2(pair2(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), pair2(fj, fj), neg));
+            z.x = attn::exp2_approx(z.x);
+            z.y = attn::exp2_approx(z.y);
+            if constexpr (!whole) {
               const int col = 32 * c + x;
-              p0 = col >= clo && col <= chi ? p0 : 0.f;
-              p1 = col + 1 >= clo && col + 1 <= chi ? p1 : 0.f;
+              z.x = col >= clo && col <= chi ? z.x : 0.f;
+              z.y = col + 1 >= clo && col + 1 <= chi ? z.y : 0.f;
             }
-            l += p0 + p1;
-            p[x >> 1] = attn::pack_half(p0, p1);
+            sum[(x >> 1) & 3] = add2(sum[(x >> 1) & 3], pair2(z.x, z.y));
+            p[x >> 1] = attn::pack_half(z.x, z.y);
           }
           // columns 16 c .. of p lie over scores that were read already
           tmem_st16(t_s + 16 * c, p);
         }
+        const float2 t2 = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+        l += t2.x + t2.y;
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bar.p_full[wg]);
+      };
+      for (int i = 0; i < T && ok; ++i) {
+        const int tok0 = (tb + i) * kTok;
+        const bool whole = tok0 + kTok - 1 <= wfirst && (a.window <= 0 || wlast - tok0 <= a.window);
+        // visible columns of this row
+        const int chi = min(pos - tok0, kTok - 1), clo = a.window > 0 ? pos - a.window - tok0 : 0;
+        ok = __all_sync(0xffffffffu, wait(&bar.s_full[wg], i & 1));
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (whole)
+          tile(std::true_type{}, i, clo, chi);
+        else
+          tile(std::false_type{}, i, clo, chi);
       }
       if (ok && T > 0) {
         ok = __all_sync(0xffffffffu, wait(&bar.o_full[wg], 0));
@@ -360,8 +406,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     }
   } else if (warp < 12) {
     // ------------------------------------------------------- widen
+    // Each thread keeps its 16-byte piece and walks down the rows, so that
+    // addresses (and the swizzle, rows 16 or 32 apart) only advance; four
+    // pieces are in flight.
     const int th = threadIdx.x - 256;  // 0 .. 127
-    const int pieces = D >> 4;         // 16-byte pieces of a key row
+    constexpr int kPieces = DP / 16, kRowStep = 128 / kPieces;
+    const int kp = th % kPieces, kr = th / kPieces;
+    const bool kin = 16 * kp < D;
+    const int kch = 2 * (kp & 3), kfirst = (kp >> 2) & 1;  // the order in which banks do not meet
+    const uint32_t ksw0 = (kp >> 2) * (kTok * 128) + swizzled(kr, kch + kfirst);
+    const uint32_t ksw1 = (kp >> 2) * (kTok * 128) + swizzled(kr, kch + (kfirst ^ 1));
+    const int vq = th & 7, vd = th >> 3;
+    const int vch = 2 * (vq & 3), vfirst = (vq >> 2) & 1;
+    const uint32_t vsw0 = (vq >> 2) * (DP * 128) + swizzled(vd, vch + vfirst);
+    const uint32_t vsw1 = (vq >> 2) * (DP * 128) + swizzled(vd, vch + (vfirst ^ 1));
+    const uint8_t* vsrc = s_rv + (16 * vq / blk) * (blk * D) + vd * blk + 16 * vq % blk;
     bool ok = true;
     for (int i = 0; i < T && ok; ++i) {
       const int slot = i & 1;
@@ -370,18 +429,25 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       ok = __all_sync(0xffffffffu, wait(&bar.raw_full[0], i & 1) && wait(&bar.k_empty[slot], ph ^ 1));
       if (!ok) break;
       uint8_t* dk = s_k + slot * S::kK;
-      for (int x = th; x < kTok * pieces; x += 128) {
-        const int row = x / pieces, p = x - row * pieces;
-        const uint4 c = *reinterpret_cast<const uint4*>(s_rk + row * D + 16 * p);
-        uint4 u, v;
-        attn::widen<FMT>(c.x, u.x, u.y);
-        attn::widen<FMT>(c.y, u.z, u.w);
-        attn::widen<FMT>(c.z, v.x, v.y);
-        attn::widen<FMT>(c.w, v.z, v.w);
-        uint8_t* base = dk + (p >> 2) * (kTok * 128);
-        const int ch = 2 * (p & 3), first = (p >> 2) & 1;  // the order in which banks do not meet
-        *reinterpret_cast<uint4*>(base + swizzled(row, ch + first)) = first ? v : u;
-        *reinterpret_cast<uint4*>(base + swizzled(row, ch + (first ^ 1))) = first ? u : v;
+      if (kin) {
+#pragma unroll
+        for (int it = 0; it < kTok / kRowStep; it += 4) {
+          uint4 c[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            c[y] = *reinterpret_cast<const uint4*>(s_rk + (kr + (it + y) * kRowStep) * D + 16 * kp);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            uint4 u, v;
+            attn::widen<FMT>(c[y].x, u.x, u.y);
+            attn::widen<FMT>(c[y].y, u.z, u.w);
+            attn::widen<FMT>(c[y].z, v.x, v.y);
+            attn::widen<FMT>(c[y].w, v.z, v.w);
+            const uint32_t down = (it + y) * kRowStep * 128;
+            *reinterpret_cast<uint4*>(dk + ksw0 + down) = kfirst ? v : u;
+            *reinterpret_cast<uint4*>(dk + ksw1 + down) = kfirst ? u : v;
+          }
+        }
       }
       async_fence();
       __syncwarp();
@@ -393,42 +459,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       ok = __all_sync(0xffffffffu, wait(&bar.raw_full[1], i & 1) && wait(&bar.v_empty[slot], ph ^ 1));
       if (!ok) break;
       uint8_t* dv = s_v + slot * S::kK;
-      const int tok0 = (tb + i) * kTok;
-      for (int x = th; x < D * 8; x += 128) {
-        const int d = x >> 3, q = x & 7;
-        const float vf = s_vf[i % kMeta][q];
-        uint4 u = make_uint4(0, 0, 0, 0), v = u;
-        if (vf != 0.f) {
-          uint4 c = *reinterpret_cast<const uint4*>(s_rv + (16 * q / blk) * (blk * D) + d * blk + 16 * q % blk);
-          const int nv = hi_tok - (tok0 + 16 * q);
-          if (nv < 16) {  // codes past the last visible token count as zero
-            uint32_t* cw = reinterpret_cast<uint32_t*>(&c);
+      const float vf = s_vf[i % kMeta][vq];
+      const __half2 hf = __float2half2_rn(vf);
+      // codes past the last visible token, or of a page that cannot be read, count as zero
+      const int nv = vf != 0.f ? min(max(hi_tok - ((tb + i) * kTok + 16 * vq), 0), 16) : 0;
+      uint32_t keep[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int n = min(max(nv - 4 * y, 0), 4);
-              cw[y] &= n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+      for (int y = 0; y < 4; ++y) {
+        const int n = min(max(nv - 4 * y, 0), 4);
+        keep[y] = n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+      }
+#pragma unroll
+      for (int it = 0; it < DP / 16; it += 4) {
+        uint4 c[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (16 * (it + y) < D) c[y] = *reinterpret_cast<const uint4*>(vsrc + 16 * (it + y) * blk);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if (16 * (it + y) >= D) break;
+          uint4 u, v;
+          attn::widen<FMT>(c[y].x & keep[0], u.x, u.y);
+          attn::widen<FMT>(c[y].y & keep[1], u.z, u.w);
+          attn::widen<FMT>(c[y].z & keep[2], v.x, v.y);
+          attn::widen<FMT>(c[y].w & keep[3], v.z, v.w);
+          if (vf != 1.f && nv > 0) {
+            uint32_t* w8[8] = {&u.x, &u.y, &u.z, &u.w, &v.x, &v.y, &v.z, &v.w};
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+              const __half2 m2 = __hmul2(*reinterpret_cast<__half2*>(w8[z]), hf);
+              *w8[z] = *reinterpret_cast<const uint32_t*>(&m2);
             }
           }
-          attn::widen<FMT>(c.x, u.x, u.y);
-          attn::widen<FMT>(c.y, u.z, u.w);
-          attn::widen<FMT>(c.z, v.x, v.y);
-          attn::widen<FMT>(c.w, v.z, v.w);
-          if (vf != 1.f) {
-            const __half2 hf = __float2half2_rn(vf);
-            uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
-            uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const __half2 ua = __hmul2(*reinterpret_cast<__half2*>(uw + y), hf), va = __hmul2(*reinterpret_cast<__half2*>(vw + y), hf);
-              uw[y] = *reinterpret_cast<const uint32_t*>(&ua);
-              vw[y] = *reinterpret_cast<const uint32_t*>(&va);
-            }
-          }
+          const uint32_t down = 16 * (it + y) * 128;
+          *reinterpret_cast<uint4*>(dv + vsw0 + down) = vfirst ? v : u;
+          *reinterpret_cast<uint4*>(dv + vsw1 + down) = vfirst ? u : v;
         }
-        uint8_t* base = dv + (q >> 2) * (DP * 128);
-        const int ch = 2 * (q & 3), first = (q >> 2) & 1;
-        *reinterpret_cast<uint4*>(base + swizzled(d, ch + first)) = first ? v : u;
-        *reinterpret_cast<uint4*>(base + swizzled(d, ch + (first ^ 1))) = first ? u : v;
       }
       async_fence();
       __syncwarp();
@@ -444,11 +510,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       const uint32_t id_s = (1u << 4) | ((uint32_t)(kTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       bool issued = false;
+      // Descriptors are made once; a step along the contraction adds to the
+      // address field (16-byte units), so an mma costs a few instructions of this
+      // one thread.
+      const uint64_t dq = tc::sdesc_sw128(tc::smem_addr(s_q)), dk = tc::sdesc_sw128(tc::smem_addr(s_k)),
+                     dv = tc::sdesc_sw128(tc::smem_addr(s_v));
       auto scores = [&](int wg, int slot) {
-        const uint32_t q0 = tc::smem_addr(s_q + wg * S::kQ), k0 = tc::smem_addr(s_k + slot * S::kK);
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-          tc::umma_bf16(tmem + 128u * wg, tc::sdesc_sw128(q0 + off), tc::sdesc_sw128(k0 + off), id_s, ks != 0);
+        const uint64_t q0 = dq + (uint32_t)(wg * (S::kQ >> 4)), k0 = dk + (uint32_t)(slot * (S::kK >> 4));
+        const uint32_t d = tmem + 128u * wg;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          if (16 * ks >= D) break;
+          const uint32_t off = (ks >> 2) * (128 * 128 >> 4) + (ks & 3) * 2;
+          tc::umma_bf16(d, q0 + off, k0 + off, id_s, ks != 0);
         }
         issued = true;
         tc::umma_commit(&bar.s_full[wg]);
@@ -467,11 +541,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           ok = wait(&bar.p_full[wg], i & 1) && (wg > 0 || wait(&bar.v_full[slot], (i >> 1) & 1));
           if (!ok) break;
           tc::tc_fence_after();
-          const uint32_t v0 = tc::smem_addr(s_v + slot * S::kK);
+          const uint64_t v0 = dv + (uint32_t)(slot * (S::kK >> 4));
+          const uint32_t d = tmem + 256u + 128u * wg, p = tmem + 128u * wg;
 #pragma unroll
           for (int ks = 0; ks < kTok / 16; ++ks)
-            umma_ts(tmem + 256u + 128u * wg, tmem + 128u * wg + 8u * ks,
-                    tc::sdesc_sw128(v0 + (ks >> 2) * (DP * 128) + (ks & 3) * 32), id_o, (i | ks) != 0);
+            umma_ts(d, p + 8u * ks, v0 + (uint32_t)((ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2), id_o, ks != 0 || i != 0);
           if (wg == nw - 1) tc::umma_commit(&bar.v_empty[slot]);
           if (i + 1 < T) {
             if (wg == 0) {
