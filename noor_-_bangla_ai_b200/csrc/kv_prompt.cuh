@@ -32,7 +32,7 @@ namespace prompt {
 
 using attn::Args;
 
-constexpr int kThreads = 448;
+constexpr int kThreads = 512;  // warps 14 and 15 only fill their register group
 constexpr int kTok = 128;    // tokens of a tile
 constexpr float kShift = 7.0f, kLazy = 8.0f;
 constexpr int kMeta = 4;     // tiles of block factors in flight
@@ -212,7 +212,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     }
   };
 
+  // Registers: 128 a thread at launch (512 x 128, the whole file); the eight
+  // softmax warps take 176, the other eight keep 80: 256 x 176 + 256 x 80 = 65536.
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // ------------------------------------------------------- softmax
     const int wg = warp >> 2, r = (warp & 3) * 32 + lane;  // row of this row tile
     const int e = e0 + 128 * wg + r;
@@ -405,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       }
     }
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------- widen
     // Each thread keeps its 16-byte piece and walks down the rows, so that
     // addresses (and the swizzle, rows 16 or 32 apart) only advance; four
@@ -504,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       }
     }
   } else if (warp == 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------- mma
     if (lane == 0 && T > 0) {
       // f16 operands, f32 sums, both K-major, M 128, N 128 tokens or D dims
@@ -568,7 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       }
     }
     __syncwarp();
+  } else if (warp > 13) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------- loader
     const int pages = kTok / blk;
     const uint32_t bytes = (uint32_t)blk * D;
