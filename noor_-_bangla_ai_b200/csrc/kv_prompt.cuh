@@ -97,6 +97,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// One thread of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // 16-byte piece `chunk` of row `row` in a 128-byte-swizzled block.
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
@@ -510,63 +517,69 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   } else if (warp == 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------- mma
-    if (lane == 0 && T > 0) {
+    // The whole warp runs the loop, so that descriptors and TMEM addresses stay
+    // in uniform registers; one elected thread issues.
+    if (T > 0) {
       // f16 operands, f32 sums, both K-major, M 128, N 128 tokens or D dims
       const uint32_t id_s = (1u << 4) | ((uint32_t)(kTok >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-      bool issued = false;
       // Descriptors are made once; a step along the contraction adds to the
-      // address field (16-byte units), so an mma costs a few instructions of this
-      // one thread.
+      // address field (16-byte units).
       const uint64_t dq = tc::sdesc_sw128(tc::smem_addr(s_q)), dk = tc::sdesc_sw128(tc::smem_addr(s_k)),
                      dv = tc::sdesc_sw128(tc::smem_addr(s_v));
-      auto scores = [&](int wg, int slot) {
+      bool issued = false;
+      auto scores = [&](int wg, int slot, bool free_k) {
         const uint64_t q0 = dq + (uint32_t)(wg * (S::kQ >> 4)), k0 = dk + (uint32_t)(slot * (S::kK >> 4));
         const uint32_t d = tmem + 128u * wg;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          if (16 * ks >= D) break;
-          const uint32_t off = (ks >> 2) * (128 * 128 >> 4) + (ks & 3) * 2;
-          tc::umma_bf16(d, q0 + off, k0 + off, id_s, ks != 0);
-        }
         issued = true;
-        tc::umma_commit(&bar.s_full[wg]);
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) {
+            if (16 * ks >= D) break;
+            const uint32_t off = (ks >> 2) * (128 * 128 >> 4) + (ks & 3) * 2;
+            tc::umma_bf16(d, q0 + off, k0 + off, id_s, ks != 0);
+          }
+          tc::umma_commit(&bar.s_full[wg]);
+          if (free_k) tc::umma_commit(&bar.k_empty[slot]);
+        }
+        __syncwarp();
       };
       bool ok = true;
-      for (int wg = 0; wg < nw && ok; ++wg) ok = wait(&bar.q_full[wg], 0);
-      if (ok) ok = wait(&bar.k_full[0], 0);
+      for (int wg = 0; wg < nw && ok; ++wg) ok = __all_sync(0xffffffffu, wait(&bar.q_full[wg], 0));
+      if (ok) ok = __all_sync(0xffffffffu, wait(&bar.k_full[0], 0));
       if (ok) {
         tc::tc_fence_after();
-        for (int wg = 0; wg < nw; ++wg) scores(wg, 0);
-        tc::umma_commit(&bar.k_empty[0]);
+        for (int wg = 0; wg < nw; ++wg) scores(wg, 0, wg == nw - 1);
       }
       for (int i = 0; i < T && ok; ++i) {
         const int slot = i & 1, next = slot ^ 1;
+        const uint64_t v0 = dv + (uint32_t)(slot * (S::kK >> 4));
         for (int wg = 0; wg < nw && ok; ++wg) {
-          ok = wait(&bar.p_full[wg], i & 1) && (wg > 0 || wait(&bar.v_full[slot], (i >> 1) & 1));
+          ok = __all_sync(0xffffffffu, wait(&bar.p_full[wg], i & 1) && (wg > 0 || wait(&bar.v_full[slot], (i >> 1) & 1)));
           if (!ok) break;
           tc::tc_fence_after();
-          const uint64_t v0 = dv + (uint32_t)(slot * (S::kK >> 4));
           const uint32_t d = tmem + 256u + 128u * wg, p = tmem + 128u * wg;
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kTok / 16; ++ks)
-            umma_ts(d, p + 8u * ks, v0 + (uint32_t)((ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2), id_o, ks != 0 || i != 0);
-          if (wg == nw - 1) tc::umma_commit(&bar.v_empty[slot]);
+            for (int ks = 0; ks < kTok / 16; ++ks)
+              umma_ts(d, p + 8u * ks, v0 + (uint32_t)((ks >> 2) * (DP * 128 >> 4) + (ks & 3) * 2), id_o, ks != 0 || i != 0);
+            if (wg == nw - 1) tc::umma_commit(&bar.v_empty[slot]);
+            if (i + 1 == T) tc::umma_commit(&bar.o_full[wg]);
+          }
+          __syncwarp();
           if (i + 1 < T) {
             if (wg == 0) {
-              ok = wait(&bar.k_full[next], ((i + 1) >> 1) & 1);
+              ok = __all_sync(0xffffffffu, wait(&bar.k_full[next], ((i + 1) >> 1) & 1));
               if (!ok) break;
               tc::tc_fence_after();
             }
-            scores(wg, next);
-            if (wg == nw - 1) tc::umma_commit(&bar.k_empty[next]);
-          } else {
-            tc::umma_commit(&bar.o_full[wg]);
+            scores(wg, next, wg == nw - 1);
           }
         }
       }
       if (issued) {  // every mma retires before TMEM is released
-        tc::umma_commit(&bar.drain);
+        if (elect_one()) tc::umma_commit(&bar.drain);
+        __syncwarp();
         const long long start = clock64();
         while (!tc::mbar_try_wait(&bar.drain, 0) && clock64() - start < kWaitLimitCycles) {
         }
