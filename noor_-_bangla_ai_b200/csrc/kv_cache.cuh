@@ -366,9 +366,26 @@ struct ReadArgs {
   void* v_out;
 };
 
-// One block per (touched block, head).
+// Four codes of one 32-bit word times a scale.
+template <int FMT>
+__device__ __forceinline__ float4 values4(uint32_t w, float s) {
+  return make_float4(Code<FMT>::value(w & 0xFF) * s, Code<FMT>::value((w >> 8) & 0xFF) * s,
+                     Code<FMT>::value((w >> 16) & 0xFF) * s, Code<FMT>::value(w >> 24) * s);
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(bf16* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+constexpr int kReadThreads = 256;
+
+// One block per (touched block, head).  Keys go straight across, 4 codes a
+// thread.  Values lie token minor: a thread takes 16 tokens of 4 dims (four
+// 16-byte loads), turns each 4 x 4 bytes over in registers and writes 4 dims
+// of each token, so a warp's stores are whole rows.  Bound by memory: codes in,
+// 2 or 4 bytes a code out.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
   const Cache& c = a.c;
   const int D = c.D, blk = c.blk, tid = threadIdx.x;
   const int t = blockIdx.x / c.H, h = blockIdx.x - t * c.H;
@@ -379,14 +396,44 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
   const float nan = __uint_as_float(0x7FC00000u);
   const float ks = bad ? nan : c.ks[ph], vs = bad ? nan : c.vs[ph];
   const uint8_t* kc = c.k + ph * blk * D + (int64_t)k.first * D;
-  const uint8_t* vc = c.v + ph * blk * D + k.first;
-  T* ko = static_cast<T*>(a.k_out) + ((int64_t)k.row0 * c.H + h) * D;
-  T* vo = static_cast<T*>(a.v_out) + ((int64_t)k.row0 * c.H + h) * D;
-  for (int i = tid; i < k.n * D; i += blockDim.x) {
-    const int s = i / D, d = i - s * D;
-    const int64_t o = (int64_t)s * c.H * D + d;
-    ko[o] = rope::from_f32<T>(bad ? nan : Code<FMT>::value(kc[i]) * ks);
-    vo[o] = rope::from_f32<T>(bad ? nan : Code<FMT>::value(vc[(int64_t)d * blk + s]) * vs);
+  const uint8_t* vc = c.v + ph * blk * D;
+  const int64_t row = (int64_t)c.H * D;
+  T* ko = static_cast<T*>(a.k_out) + (int64_t)k.row0 * row + h * D;
+  T* vo = static_cast<T*>(a.v_out) + (int64_t)k.row0 * row + h * D;
+  const int quads = D >> 2;
+#pragma unroll 4
+  for (int i = tid; i < k.n * quads; i += kReadThreads) {
+    const int s = i / quads, d = (i - s * quads) * 4;
+    const uint32_t w = bad ? 0 : __ldg(reinterpret_cast<const uint32_t*>(kc + s * D + d));
+    float4 v = values4<FMT>(w, ks);
+    if (bad) v = make_float4(nan, nan, nan, nan);
+    store4(ko + s * row + d, v);
+  }
+  for (int i = tid; i < (blk >> 4) * quads; i += kReadThreads) {
+    const int g = i / quads, d = (i - g * quads) * 4;
+    if (16 * g + 16 <= k.first || 16 * g >= k.first + k.n) continue;
+    uint4 r[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      r[x] = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(vc + (int64_t)(d + x) * blk + 16 * g));
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const uint32_t w0 = y == 0 ? r[0].x : y == 1 ? r[0].y : y == 2 ? r[0].z : r[0].w;
+      const uint32_t w1 = y == 0 ? r[1].x : y == 1 ? r[1].y : y == 2 ? r[1].z : r[1].w;
+      const uint32_t w2 = y == 0 ? r[2].x : y == 1 ? r[2].y : y == 2 ? r[2].z : r[2].w;
+      const uint32_t w3 = y == 0 ? r[3].x : y == 1 ? r[3].y : y == 2 ? r[3].z : r[3].w;
+      // 4 x 4 bytes turned over
+      const uint32_t a0 = __byte_perm(w0, w1, 0x5140), a1 = __byte_perm(w0, w1, 0x7362);
+      const uint32_t b0 = __byte_perm(w2, w3, 0x5140), b1 = __byte_perm(w2, w3, 0x7362);
+      const uint32_t o[4] = {__byte_perm(a0, b0, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x5410),
+                             __byte_perm(a1, b1, 0x7632)};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int s = 16 * g + 4 * y + x - k.first;
+        if (s < 0 || s >= k.n) continue;
+        store4(vo + s * row + d, bad ? make_float4(nan, nan, nan, nan) : values4<FMT>(o[x], vs));
+      }
+    }
   }
 }
 

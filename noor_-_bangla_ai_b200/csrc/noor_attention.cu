@@ -262,9 +262,9 @@ int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* 
     return by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
       if (c->format == NOOR_KV_INT8)
-        kv::read_kernel<T, kv::INT8><<<(unsigned)grid, 256, 0, s>>>(a);
+        kv::read_kernel<T, kv::INT8><<<(unsigned)grid, kv::kReadThreads, 0, s>>>(a);
       else
-        kv::read_kernel<T, kv::E4M3><<<(unsigned)grid, 256, 0, s>>>(a);
+        kv::read_kernel<T, kv::E4M3><<<(unsigned)grid, kv::kReadThreads, 0, s>>>(a);
       CK(cudaGetLastError());
       return NOOR_MOE_OK;
     });
