@@ -15,6 +15,8 @@
 #include "noor_moe.h"
 #include "rope.cuh"
 
+#include <type_traits>
+
 namespace noor {
 namespace kv {
 
@@ -144,25 +146,12 @@ struct Code<INT8> {
   // exponent of the smallest power of two that holds amax (a finite f32, as bits)
   static constexpr int kExp = 6;                  // 127 = 1.984375 * 2^6
   static constexpr uint32_t kMant = 0x7E0000u;    // mantissa bits of 1.984375
-  __device__ static uint8_t make(double x) {
-    const int v = __double2int_rn(fmin(fmax(x, -127.0), 127.0));
-    return (uint8_t)(int8_t)v;
-  }
-  __device__ static uint8_t make(float x) {
-    const int v = __float2int_rn(fminf(fmaxf(x, -127.0f), 127.0f));
-    return (uint8_t)(int8_t)v;
-  }
   __device__ static float value(uint8_t c) { return (float)(int8_t)c; }
 };
 template <>
 struct Code<E4M3> {
   static constexpr int kExp = 8;                  // 448 = 1.75 * 2^8
   static constexpr uint32_t kMant = 0x600000u;
-  // A NaN code is never stored (the block's scale says NaN): a reader's zero
-  // weight times any stored code is zero.
-  __device__ static uint8_t finite(uint8_t c) { return (c & 0x7F) == 0x7F ? 0 : c; }
-  __device__ static uint8_t make(double x) { return finite(__nv_cvt_double_to_fp8(x, __NV_SATFINITE, __NV_E4M3)); }
-  __device__ static uint8_t make(float x) { return finite(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3)); }
   __device__ static float value(uint8_t c) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
   }
@@ -180,7 +169,8 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
 }
 
 // The scale of a block that held tokens at s_old and now needs s_new: the
-// larger, as a power of two; NaN stays.
+// larger, as a power of two; NaN stays.  (A poisoned block's codes are stored
+// as zeros: a reader's zero weight times any stored code is zero.)
 __device__ __forceinline__ float grown_scale(float s_old, float s_new) {
   if (!(s_old > 0.f)) return s_old == 0.f ? s_new : __uint_as_float(0x7FC00000u);
   uint32_t b = __float_as_uint(s_old);
@@ -197,117 +187,361 @@ struct AppendArgs {
   Batch b;
   rope::View k, v;
   rope::Args r;       // k's rotation; q and q_out for the q part
-  int32_t kv_blocks;  // blocks of the grid that write the cache (the rest rotate q)
+  int32_t heads;      // kv heads of one grid block
+  int32_t kv_blocks;  // grid blocks that write the cache: task major, then k or v, then head group (the rest rotate q)
   int32_t q_tok;      // rows of q per block
+  bool kvec, vvec;    // k / v can be read four elements at a time
+  bool qvec;          // q can be rotated 16 bytes at a time
 };
 
-// Magnitude bits of the largest |x| over the block's threads.
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* s_red) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) s_red[warp] = v;
+constexpr int kHeadsAtOnce = 64;  // 256 threads over the 4 that a head of 16 dims takes
+
+// Largest magnitudes (as bits) of the heads that a grid block works on at
+// once, in three alternating rows: while one is read, the next is cleared.
+struct Maxima {
+  uint32_t m[3][kHeadsAtOnce];
+};
+
+// Every thread's v joins its head's maximum; returns the head's.  `pass`
+// counts the calls.  All threads of the block call it.
+__device__ __forceinline__ uint32_t head_max(uint32_t v, int hl, Maxima& s, int pass) {
+  uint32_t* m = s.m[pass % 3];
+  const int first = __shfl_sync(0xffffffffu, hl, 0);
+  if (__all_sync(0xffffffffu, hl == first)) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0 && hl < kHeadsAtOnce) atomicMax(m + hl, v);
+  } else if (hl < kHeadsAtOnce) {
+    atomicMax(m + hl, v);
+  }
+  if (threadIdx.x < kHeadsAtOnce) s.m[(pass + 1) % 3][threadIdx.x] = 0;
   __syncthreads();
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kAppendThreads / 32; ++i) m = max(m, s_red[i]);
-  __syncthreads();
-  return m;
+  return hl < kHeadsAtOnce ? m[hl] : 0;
 }
 
-// Write the new tokens of one (touched block, head): grid.x counts them head
-// minor.
-template <typename T, int FMT>
-__device__ void append_block(const AppendArgs& a, uint8_t* smem) {
+// Four elements as floats.
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const bf16* p) {
+  const uint2 r = *reinterpret_cast<const uint2*>(p);
+  return make_float4(bf16_lo(r.x), bf16_hi(r.x), bf16_lo(r.y), bf16_hi(r.y));
+}
+__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 load2(const bf16* p) {
+  const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
+  return make_float2(bf16_lo(r), bf16_hi(r));
+}
+
+// Codes of two values in steps, x in the low byte.
+template <int FMT>
+__device__ __forceinline__ uint32_t codes2(float x, float y) {
+  if constexpr (FMT == INT8) {
+    // 1.5 2^23 + x rounds x to an integer, ties to even; |x| <= 127 by the scale's choice
+    return (__float_as_uint(x + 12582912.f) & 0xFFu) | ((__float_as_uint(y + 12582912.f) & 0xFFu) << 8);
+  } else {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y), "f"(x));
+    return r;
+  }
+}
+// The same in f64, rounded once.
+template <int FMT>
+__device__ __forceinline__ uint32_t codes2(double x, double y) {
+  if constexpr (FMT == INT8) {
+    // a rotated value may pass the scale's bound by its rounding: 127.0..01 is 127
+    return ((uint32_t)__double2loint(x + 6755399441055744.0) & 0xFFu) |
+           (((uint32_t)__double2loint(y + 6755399441055744.0) & 0xFFu) << 8);
+  } else {
+    // onto e4m3's grid (3 bits below the leading one, steps of 2^-9 at least)
+    // in f64, then exactly to f32 and the code
+    auto grid = [](double v) -> float {
+      const int e = max((__double2hiint(v) >> 20 & 0x7FF) - 1023, -6);
+      const double big = __hiloint2double(((e - 3 + 52 + 1023) << 20) | 0x80000, 0);
+      return (float)((v + big) - big);
+    };
+    return codes2<E4M3>(grid(x), grid(y));
+  }
+}
+
+// A block's old codes, four of a word, rounded again under a grown scale.
+template <int FMT>
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
+  const float a = Code<FMT>::value(w & 0xFF), b = Code<FMT>::value((w >> 8) & 0xFF), c = Code<FMT>::value((w >> 16) & 0xFF),
+              d = Code<FMT>::value(w >> 24);
+  return codes2<FMT>(a * ratio, b * ratio) | (codes2<FMT>(c * ratio, d * ratio) << 16);
+}
+
+// Keys of one touched block, kv heads h0 .. h1 - 1.  A thread owns two pairs of
+// a head and every G-th token; a decode step's single token leaves room for
+// several heads at once.  Its angle is made once in f64 and advanced from
+// token to token by the angle of G positions (a complex product; 16 of them
+// lose a few units of 2^-53), so a sine and cosine pair is paid for once per
+// thread and not per element.  The largest magnitude is found in f32; only
+// where that falls within 1e-5 of a power of two's bound is it found again in
+// f64.  The codes are rounded from the f64 rotation.
+// Bound by memory once enough blocks run: the elements are read once into
+// registers.
+template <typename T, int FMT, int TPT>
+__device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, Maxima& s_max) {
   const Cache& c = a.c;
-  const int D = c.D, blk = c.blk;
-  __shared__ Task s_task;
-  __shared__ uint32_t s_red[kAppendThreads / 32];
-  const int tid = threadIdx.x;
-  const int t = blockIdx.x / c.H, h = blockIdx.x - t * c.H;
-  if (tid < 32) {
-    const Task k = find_task(c, a.b, nullptr, true, t, tid);
-    if (tid == 0) s_task = k;
-  }
-  __syncthreads();
-  const Task k = s_task;
-  if (k.b < 0 || k.page < 0) return;
-  const int64_t ph = k.page * c.H + h;
-  T* s_x = reinterpret_cast<T*>(smem);               // [n][D] keys, then values
-  uint8_t* s_c = smem + (size_t)blk * D * sizeof(T);  // codes, [n][D]
-  const float s_old_k = k.first > 0 ? c.ks[ph] : 0.f, s_old_v = k.first > 0 ? c.vs[ph] : 0.f;
-
-  // ---- keys: rotate in f64 (twice, once for the largest, once for the codes)
-  const T* kp = static_cast<const T*>(a.k.p) + (int64_t)k.row0 * a.k.st + h * a.k.sh;
-  for (int i = tid; i < k.n * D; i += kAppendThreads) {
-    const int s = i / D, d = i - s * D;
-    s_x[i] = kp[s * a.k.st + d];
-  }
-  __syncthreads();
-  const int pairs = D >> 1, rot = a.r.rot;
+  const int D = c.D, blk = c.blk, tid = threadIdx.x, rot = a.r.rot;
+  const int quads = D >> 2, G = min(kAppendThreads / quads, k.n), slots = quads * G, at_once = kAppendThreads / slots;
+  const int hl = tid / slots, qd = tid % quads, g = tid / quads - hl * G;
+  const bool thread_live = hl < at_once;
+  // the thread's pairs (x0, x1), (x2, x3) as dims
+  const bool half = a.r.layout == rope::HALF;
+  auto dim0 = [&](int p) { return half && 2 * p < rot ? p : 2 * p; };
+  auto dim1 = [&](int p) { return half && 2 * p < rot ? p + (rot >> 1) : 2 * p + 1; };
+  const int d0 = dim0(2 * qd), d1 = dim1(2 * qd), d2 = dim0(2 * qd + 1), d3 = dim1(2 * qd + 1);
+  const bool split = d2 == d0 + 1 && d3 == d1 + 1;                  // two runs of two
+  const bool run = d1 == d0 + 1 && d2 == d0 + 2 && d3 == d0 + 3;    // one run of four
+  // first angle and step of both pairs
+  double c0[2] = {1.0, 1.0}, s0[2] = {0.0, 0.0}, cg[2] = {1.0, 1.0}, sg[2] = {0.0, 0.0};
   const int32_t pos0 = k.j * blk + k.first;
-  uint32_t amax = 0;
-  float scale = 1.f;
-  double inv = 1.0;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int i = tid; i < k.n * pairs; i += kAppendThreads) {
-      const int s = i / pairs, p = i - s * pairs;
-      const bool r = 2 * p < rot;
-      const int d0 = r && a.r.layout == rope::HALF ? p : 2 * p;
-      const int d1 = r && a.r.layout == rope::HALF ? p + (rot >> 1) : d0 + 1;
-      double x0 = (double)rope::to_f32(s_x[s * D + d0]), x1 = (double)rope::to_f32(s_x[s * D + d1]);
-      if (r) {
-        double sn, cs;
-        sincospi(2.0 * rope::turn_fraction(pos0 + s, __ldg(a.r.inv_freq + p)), &sn, &cs);
-        const double y0 = (x0 * cs - x1 * sn) * a.r.factor, y1 = (x0 * sn + x1 * cs) * a.r.factor;
-        x0 = y0;
-        x1 = y1;
+  bool turned[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int p = 2 * qd + x;
+    turned[x] = thread_live && 2 * p < rot;
+    if (turned[x]) {
+      const float f = __ldg(a.r.inv_freq + p);
+      sincospi(2.0 * rope::turn_fraction(pos0 + g, f), &s0[x], &c0[x]);
+      c0[x] *= a.r.factor;
+      s0[x] *= a.r.factor;
+      if (g + G < k.n) sincospi(2.0 * rope::turn_fraction(G, f), &sg[x], &cg[x]);
+    }
+  }
+  for (int hb = h0, pass = 0; hb < h1; hb += at_once, ++pass) {
+    const int h = hb + hl;
+    const bool live = thread_live && h < h1;
+    const int64_t ph = k.page * c.H + (live ? h : hb);
+    const T* kp = static_cast<const T*>(a.k.p) + (int64_t)k.row0 * a.k.st + h * a.k.sh;
+    const float s_old = k.first > 0 ? __ldg(c.ks + ph) : 0.f;
+    float4 x[TPT];
+#pragma unroll
+    for (int j = 0; j < TPT; ++j) {
+      if (G * j >= k.n) break;
+      const int s = g + G * j;
+      x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (live && s < k.n) {
+        const T* p = kp + s * a.k.st;
+        if (a.kvec && run) {
+          x[j] = load4(p + d0);
+        } else if (a.kvec && split) {
+          const float2 u = load2(p + d0), v = load2(p + d1);
+          x[j] = make_float4(u.x, v.x, u.y, v.y);
+        } else {
+          x[j] = make_float4(rope::to_f32(p[d0]), rope::to_f32(p[d1]), rope::to_f32(p[d2]), rope::to_f32(p[d3]));
+        }
       }
-      if (pass == 0) {
-        amax = max(amax, max(__float_as_uint((float)fabs(x0)), __float_as_uint((float)fabs(x1))));
+    }
+    // ---- scale
+    uint32_t amax = 0;
+    {
+      float c1[2] = {(float)c0[0], (float)c0[1]}, s1[2] = {(float)s0[0], (float)s0[1]};
+      const float cf[2] = {(float)cg[0], (float)cg[1]}, sf[2] = {(float)sg[0], (float)sg[1]};
+#pragma unroll
+      for (int j = 0; j < TPT; ++j) {
+        if (G * j >= k.n) break;
+        const float v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float y0 = v[2 * y] * c1[y] - v[2 * y + 1] * s1[y], y1 = v[2 * y] * s1[y] + v[2 * y + 1] * c1[y];
+          amax = max(amax, max(__float_as_uint(fabsf(y0)), __float_as_uint(fabsf(y1))));
+          const float cn = c1[y] * cf[y] - s1[y] * sf[y];
+          s1[y] = s1[y] * cf[y] + c1[y] * sf[y];
+          c1[y] = cn;
+        }
+      }
+    }
+    amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
+    // (84 steps of 2^-23 are 1e-5; a block's heads decide together)
+    const bool border = live && rot > 0 && amax < 0x7F800000u - 84 &&
+                        scale_for<FMT>(amax - min(amax, 84u)) != scale_for<FMT>(amax + 84u);
+    if (__syncthreads_or(border)) {
+      __shared__ unsigned long long s_exact[kHeadsAtOnce];
+      if (tid < kHeadsAtOnce) s_exact[tid] = 0;
+      __syncthreads();
+      double m = 0.0, c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
+#pragma unroll 1
+      for (int s = g; live && s < k.n; s += G) {
+        const T* p = kp + s * a.k.st;
+        const double v[4] = {(double)rope::to_f32(p[d0]), (double)rope::to_f32(p[d1]), (double)rope::to_f32(p[d2]),
+                             (double)rope::to_f32(p[d3])};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          m = fmax(m, fmax(fabs(v[2 * y] * c1[y] - v[2 * y + 1] * s1[y]), fabs(v[2 * y] * s1[y] + v[2 * y + 1] * c1[y])));
+          const double cn = c1[y] * cg[y] - s1[y] * sg[y];
+          s1[y] = s1[y] * cg[y] + c1[y] * sg[y];
+          c1[y] = cn;
+        }
+      }
+      if (live) atomicMax(&s_exact[hl], (unsigned long long)__double_as_longlong(m));
+      __syncthreads();
+      if (border) amax = __float_as_uint(__double2float_ru(__longlong_as_double((long long)s_exact[hl])));
+      __syncthreads();
+    }
+    if (!live) continue;
+    const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
+    const bool poisoned = scale != scale;
+    const double inv = 1.0 / (double)scale;
+    uint8_t* kc = c.k + ph * blk * D;
+    // ---- the old codes under a grown scale
+    if (k.first > 0 && scale != s_old) {
+      const float ratio = poisoned ? 0.f : s_old / scale;
+      for (int i = tid - hl * slots; i < k.first * quads; i += slots) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(kc) + i;
+        *w = poisoned ? 0 : recode4<FMT>(*w, ratio);
+      }
+    }
+    // ---- codes of the new tokens
+    double c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
+#pragma unroll
+    for (int j = 0; j < TPT; ++j) {
+      const int s = g + G * j;
+      if (s >= k.n) break;
+      double v[4] = {(double)x[j].x, (double)x[j].y, (double)x[j].z, (double)x[j].w};
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        if (turned[y]) {
+          const double y0 = v[2 * y] * c1[y] - v[2 * y + 1] * s1[y], y1 = v[2 * y] * s1[y] + v[2 * y + 1] * c1[y];
+          v[2 * y] = y0;
+          v[2 * y + 1] = y1;
+          const double cn = c1[y] * cg[y] - s1[y] * sg[y];
+          s1[y] = s1[y] * cg[y] + c1[y] * sg[y];
+          c1[y] = cn;
+        }
+      }
+      const uint32_t e = poisoned ? 0 : codes2<FMT>(v[0] * inv, v[1] * inv), f = poisoned ? 0 : codes2<FMT>(v[2] * inv, v[3] * inv);
+      uint8_t* o = kc + (int64_t)(k.first + s) * D;
+      if (run) {
+        *reinterpret_cast<uint32_t*>(o + d0) = e | (f << 16);
+      } else if (split && d1 % 2 == 0) {
+        *reinterpret_cast<uint16_t*>(o + d0) = (uint16_t)((e & 0xFF) | ((f & 0xFF) << 8));
+        *reinterpret_cast<uint16_t*>(o + d1) = (uint16_t)((e >> 8) | (f & 0xFF00));
       } else {
-        s_c[s * D + d0] = Code<FMT>::make(x0 * inv);
-        s_c[s * D + d1] = Code<FMT>::make(x1 * inv);
+        o[d0] = (uint8_t)e;
+        o[d1] = (uint8_t)(e >> 8);
+        o[d2] = (uint8_t)f;
+        o[d3] = (uint8_t)(f >> 8);
       }
     }
-    if (pass == 0) {
-      amax = block_max(amax, s_red);
-      scale = k.first > 0 ? grown_scale(s_old_k, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
-      inv = 1.0 / (double)scale;
-    }
+    if (tid == hl * slots) c.ks[ph] = scale;
   }
-  uint8_t* kc = c.k + ph * blk * D;
-  if (k.first > 0 && scale != s_old_k) {  // (NaN too: harmless)
-    const float ratio = s_old_k / scale;
-    for (int i = tid; i < k.first * D; i += kAppendThreads) kc[i] = Code<FMT>::make(Code<FMT>::value(kc[i]) * ratio);
-  }
-  __syncthreads();
-  for (int i = tid; i < k.n * D; i += kAppendThreads) kc[(int64_t)k.first * D + i] = s_c[i];
-  if (tid == 0) c.ks[ph] = scale;
-  __syncthreads();
+}
 
-  // ---- values
-  const T* vp = static_cast<const T*>(a.v.p) + (int64_t)k.row0 * a.v.st + h * a.v.sh;
-  amax = 0;
-  for (int i = tid; i < k.n * D; i += kAppendThreads) {
-    const int s = i / D, d = i - s * D;
-    const T x = vp[s * a.v.st + d];
-    s_x[i] = x;
-    amax = max(amax, __float_as_uint(fabsf(rope::to_f32(x))));
+// Values of one touched block: a thread takes 4 dims of 16 tokens in
+// registers, turns the codes over and writes 16 tokens of each dim, the
+// cache's order.  Where a 16-token run is not all new it is read, merged and
+// written back (this block alone owns the page).  Only runs with new tokens
+// take threads; where they leave room, several heads are done at once.
+template <typename T, int FMT>
+__device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1, Maxima& s_max) {
+  const Cache& c = a.c;
+  const int D = c.D, blk = c.blk, tid = threadIdx.x, quads = D >> 2;
+  const int r0 = k.first >> 4, runs = ((k.first + k.n - 1) >> 4) - r0 + 1;
+  const int slots = quads * runs, at_once = kAppendThreads / slots;   // at most 4 x 64
+  const int hl = tid / slots, run = (tid - hl * slots) / quads, d = (tid % quads) * 4, lo = 16 * (r0 + run);
+  const bool all_new = lo >= k.first && lo + 16 <= k.first + k.n;
+  for (int hb = h0, pass = 0; hb < h1; hb += at_once, ++pass) {
+    const int h = hb + hl;
+    const bool live = hl < at_once && h < h1;
+    const int64_t ph = k.page * c.H + (live ? h : hb);
+    const T* vp = static_cast<const T*>(a.v.p) + (int64_t)k.row0 * a.v.st + h * a.v.sh + d;
+    const float s_old = k.first > 0 ? __ldg(c.vs + ph) : 0.f;
+    uint8_t* vc = c.v + ph * blk * D + (int64_t)d * blk + lo;
+    typename std::conditional<sizeof(T) == 2, uint2, float4>::type x[16];
+    uint32_t amax = 0;
+    if (live) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int s = lo + i - k.first;
+      const bool in = s >= 0 && s < k.n;
+      const T* p = vp + s * a.v.st;
+      if constexpr (sizeof(T) == 2) {
+        x[i] = make_uint2(0, 0);
+        if (in) {
+          if (a.vvec) {
+            x[i] = *reinterpret_cast<const uint2*>(p);
+          } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+            x[i] = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
+          }
+        }
+        // magnitudes of both halves, in f32's bits
+        amax = max(amax, max(max((x[i].x << 16) & 0x7FFFFFFFu, x[i].x & 0x7FFF0000u),
+                             max((x[i].y << 16) & 0x7FFFFFFFu, x[i].y & 0x7FFF0000u)));
+      } else {
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) x[i] = a.vvec ? load4(p) : make_float4(p[0], p[1], p[2], p[3]);
+        amax = max(amax, max(max(__float_as_uint(fabsf(x[i].x)), __float_as_uint(fabsf(x[i].y))),
+                             max(__float_as_uint(fabsf(x[i].z)), __float_as_uint(fabsf(x[i].w)))));
+      }
+    }
+    }
+    amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
+    if (!live) continue;
+    const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
+    const bool poisoned = scale != scale, grow = k.first > 0 && scale != s_old;
+    const float inv = 1.f / scale, ratio = s_old / scale;
+    if (tid == hl * slots) c.vs[ph] = scale;
+    if (grow && r0 > 0) {  // whole runs of old codes under a grown scale
+      for (int i = tid - hl * slots; i < D * r0; i += slots) {
+        uint4* p = reinterpret_cast<uint4*>(c.v + ph * blk * D + (int64_t)(i / r0) * blk) + i % r0;
+        uint4 o = make_uint4(0, 0, 0, 0);
+        if (!poisoned) {
+          o = *p;
+          o = make_uint4(recode4<FMT>(o.x, ratio), recode4<FMT>(o.y, ratio), recode4<FMT>(o.z, ratio), recode4<FMT>(o.w, ratio));
+        }
+        *p = o;
+      }
+    }
+    uint4 old[4];
+    if (!all_new) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) old[y] = *reinterpret_cast<const uint4*>(vc + (int64_t)y * blk);
+    }
+    uint32_t w[4][4];  // [dim][word of 4 tokens]
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      uint32_t t[4];  // a token's 4 codes
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 v;
+        if constexpr (sizeof(T) == 2)
+          v = make_float4(bf16_lo(x[4 * z + i].x), bf16_hi(x[4 * z + i].x), bf16_lo(x[4 * z + i].y), bf16_hi(x[4 * z + i].y));
+        else
+          v = x[4 * z + i];
+        t[i] = poisoned ? 0 : codes2<FMT>(v.x * inv, v.y * inv) | (codes2<FMT>(v.z * inv, v.w * inv) << 16);
+      }
+      const uint32_t a0 = __byte_perm(t[0], t[1], 0x5140), a1 = __byte_perm(t[0], t[1], 0x7362);
+      const uint32_t b0 = __byte_perm(t[2], t[3], 0x5140), b1 = __byte_perm(t[2], t[3], 0x7362);
+      w[0][z] = __byte_perm(a0, b0, 0x5410);
+      w[1][z] = __byte_perm(a0, b0, 0x7632);
+      w[2][z] = __byte_perm(a1, b1, 0x5410);
+      w[3][z] = __byte_perm(a1, b1, 0x7632);
+    }
+    if (!all_new) {
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        // bytes of new tokens and of old ones in this word
+        uint32_t mn = 0, mo = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int s = lo + 4 * z + i;
+          if (s < k.first) mo |= 0xFFu << (8 * i);
+          else if (s < k.first + k.n) mn |= 0xFFu << (8 * i);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t o = z == 0 ? old[y].x : z == 1 ? old[y].y : z == 2 ? old[y].z : old[y].w;
+          uint32_t kept = o;
+          if (grow && mo) kept = (o & ~mo) | ((poisoned ? 0 : recode4<FMT>(o, ratio)) & mo);
+          w[y][z] = (w[y][z] & mn) | (kept & ~mn);
+        }
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) *reinterpret_cast<uint4*>(vc + (int64_t)y * blk) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
   }
-  amax = block_max(amax, s_red);
-  scale = k.first > 0 ? grown_scale(s_old_v, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
-  const float finv = 1.0f / scale;
-  uint8_t* vc = c.v + ph * blk * D;
-  const bool grow = k.first > 0 && scale != s_old_v;
-  const float ratio = grow ? s_old_v / scale : 1.f;
-  for (int i = tid; i < D * blk; i += kAppendThreads) {
-    const int d = i / blk, s = i - d * blk;
-    if (s >= k.first && s < k.first + k.n)
-      vc[i] = Code<FMT>::make(rope::to_f32(s_x[(s - k.first) * D + d]) * finv);
-    else if (grow && s < k.first)
-      vc[i] = Code<FMT>::make(Code<FMT>::value(vc[i]) * ratio);
-  }
-  if (tid == 0) c.vs[ph] = scale;
 }
 
 // Rotate q_tok rows of q to their sequences' positions.
@@ -347,13 +581,28 @@ __device__ void append_rotate_q(const AppendArgs& a, uint8_t* smem) {
   }
 }
 
-template <typename T, int FMT, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+template <typename T, int FMT, int TPT>
+__global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kernel(const AppendArgs a) {
   extern __shared__ __align__(16) uint8_t s_append[];
-  if ((int)blockIdx.x < a.kv_blocks)
-    append_block<T, FMT>(a, s_append);
+  __shared__ Maxima s_max;
+  if ((int)blockIdx.x >= a.kv_blocks) {
+    if (a.qvec)
+      append_rotate_q<T, true>(a, s_append);
+    else
+      append_rotate_q<T, false>(a, s_append);
+    return;
+  }
+  if (threadIdx.x < kHeadsAtOnce) s_max.m[0][threadIdx.x] = 0;
+  __syncthreads();
+  const int groups = (a.c.H + a.heads - 1) / a.heads;
+  const int t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
+  const Task k = find_task(a.c, a.b, nullptr, true, t, threadIdx.x & 31);
+  if (k.b < 0 || k.page < 0) return;
+  const int h0 = (r >> 1) * a.heads, h1 = min(h0 + a.heads, a.c.H);
+  if (r & 1)
+    append_values<T, FMT>(a, k, h0, h1, s_max);
   else
-    append_rotate_q<T, VEC>(a, s_append);
+    append_keys<T, FMT, TPT>(a, k, h0, h1, s_max);
 }
 
 // ------------------------------------------------------------- read back
@@ -364,13 +613,36 @@ struct ReadArgs {
   const int32_t* starts;
   void* k_out;
   void* v_out;
+  int32_t heads;  // kv heads of one grid block
 };
 
 // Four codes of one 32-bit word times a scale.
 template <int FMT>
 __device__ __forceinline__ float4 values4(uint32_t w, float s) {
-  return make_float4(Code<FMT>::value(w & 0xFF) * s, Code<FMT>::value((w >> 8) & 0xFF) * s,
-                     Code<FMT>::value((w >> 16) & 0xFF) * s, Code<FMT>::value(w >> 24) * s);
+  if constexpr (FMT == INT8) {
+    // code + 128 in the low byte of 2^23 is the float 2^23 + 128 + code
+    w ^= 0x80808080u;
+    const float bias = 8388736.f;
+    return make_float4((__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540)) - bias) * s,
+                       (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541)) - bias) * s,
+                       (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7542)) - bias) * s,
+                       (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7543)) - bias) * s);
+  } else {
+    const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)w, __NV_E4M3)));
+    const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)(w >> 16), __NV_E4M3)));
+    return make_float4(a.x * s, a.y * s, b.x * s, b.y * s);
+  }
+}
+__device__ __forceinline__ void store16(float* p, const float4 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[i] = v[i];
+}
+__device__ __forceinline__ void store16(bf16* p, const float4 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    reinterpret_cast<uint4*>(p)[i] =
+        make_uint4(pack_bf16(v[2 * i].x, v[2 * i].y), pack_bf16(v[2 * i].z, v[2 * i].w),
+                   pack_bf16(v[2 * i + 1].x, v[2 * i + 1].y), pack_bf16(v[2 * i + 1].z, v[2 * i + 1].w));
 }
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store4(bf16* p, float4 v) {
@@ -379,59 +651,63 @@ __device__ __forceinline__ void store4(bf16* p, float4 v) {
 
 constexpr int kReadThreads = 256;
 
-// One block per (touched block, head).  Keys go straight across, 4 codes a
-// thread.  Values lie token minor: a thread takes 16 tokens of 4 dims (four
-// 16-byte loads), turns each 4 x 4 bytes over in registers and writes 4 dims
-// of each token, so a warp's stores are whole rows.  Bound by memory: codes in,
-// 2 or 4 bytes a code out.
+// One grid block per touched block, group of heads, and k or v.  Keys go
+// straight across, 16 codes a thread.  Values lie token minor: a thread takes
+// 16 tokens of 4 dims (four 16-byte loads), turns each 4 x 4 bytes over in
+// registers and writes 4 dims of each token, so a warp's stores are whole
+// rows.  Bound by memory: codes in, 2 or 4 bytes a code out.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
   const Cache& c = a.c;
   const int D = c.D, blk = c.blk, tid = threadIdx.x;
-  const int t = blockIdx.x / c.H, h = blockIdx.x - t * c.H;
+  const int groups = (c.H + a.heads - 1) / a.heads, t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
+  const int h0 = (r >> 1) * a.heads, nh = min(a.heads, c.H - h0);
   const Task k = find_task(c, a.b, a.starts, false, t, tid & 31);
   if (k.b < 0) return;
   const bool bad = k.page < 0;
-  const int64_t ph = bad ? 0 : k.page * c.H + h;
   const float nan = __uint_as_float(0x7FC00000u);
-  const float ks = bad ? nan : c.ks[ph], vs = bad ? nan : c.vs[ph];
-  const uint8_t* kc = c.k + ph * blk * D + (int64_t)k.first * D;
-  const uint8_t* vc = c.v + ph * blk * D;
-  const int64_t row = (int64_t)c.H * D;
-  T* ko = static_cast<T*>(a.k_out) + (int64_t)k.row0 * row + h * D;
-  T* vo = static_cast<T*>(a.v_out) + (int64_t)k.row0 * row + h * D;
-  const int quads = D >> 2;
+  const int64_t ph0 = bad ? 0 : k.page * c.H + h0, row = (int64_t)c.H * D, head = (int64_t)blk * D;
+  if ((r & 1) == 0) {
+    const int pieces = D >> 4, per = k.n * pieces;
+    const uint8_t* kc = c.k + ph0 * head + (int64_t)k.first * D;
+    T* ko = static_cast<T*>(a.k_out) + (int64_t)k.row0 * row + h0 * D;
 #pragma unroll 4
-  for (int i = tid; i < k.n * quads; i += kReadThreads) {
-    const int s = i / quads, d = (i - s * quads) * 4;
-    const uint32_t w = bad ? 0 : __ldg(reinterpret_cast<const uint32_t*>(kc + s * D + d));
-    float4 v = values4<FMT>(w, ks);
-    if (bad) v = make_float4(nan, nan, nan, nan);
-    store4(ko + s * row + d, v);
-  }
-  for (int i = tid; i < (blk >> 4) * quads; i += kReadThreads) {
-    const int g = i / quads, d = (i - g * quads) * 4;
-    if (16 * g + 16 <= k.first || 16 * g >= k.first + k.n) continue;
-    uint4 r[4];
+    for (int i = tid; i < nh * per; i += kReadThreads) {
+      const int hl = i / per, j = i - hl * per, s = j / pieces, d = (j - s * pieces) * 16;
+      const uint4 w = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(kc + hl * head + s * D + d));
+      const float ks = bad ? nan : __ldg(c.ks + ph0 + hl);
+      const float4 v[4] = {values4<FMT>(w.x, ks), values4<FMT>(w.y, ks), values4<FMT>(w.z, ks), values4<FMT>(w.w, ks)};
+      store16(ko + s * row + hl * D + d, v);
+    }
+  } else {
+    // 16-token runs that the call's tokens touch
+    const int quads = D >> 2, r0 = k.first >> 4, runs = ((k.first + k.n - 1) >> 4) - r0 + 1, per = runs * quads;
+    const uint8_t* vc = c.v + ph0 * head;
+    T* vo = static_cast<T*>(a.v_out) + (int64_t)k.row0 * row + h0 * D;
+    for (int i = tid; i < nh * per; i += kReadThreads) {
+      const int hl = i / per, j = i - hl * per, g = j / quads, d = (j - g * quads) * 4, lo = 16 * (r0 + g);
+      uint4 w[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      r[x] = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(vc + (int64_t)(d + x) * blk + 16 * g));
+      for (int x = 0; x < 4; ++x)
+        w[x] = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(vc + hl * head + (int64_t)(d + x) * blk + lo));
+      const float vs = bad ? nan : __ldg(c.vs + ph0 + hl);
+      T* o = vo + hl * D + d;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const uint32_t w0 = y == 0 ? r[0].x : y == 1 ? r[0].y : y == 2 ? r[0].z : r[0].w;
-      const uint32_t w1 = y == 0 ? r[1].x : y == 1 ? r[1].y : y == 2 ? r[1].z : r[1].w;
-      const uint32_t w2 = y == 0 ? r[2].x : y == 1 ? r[2].y : y == 2 ? r[2].z : r[2].w;
-      const uint32_t w3 = y == 0 ? r[3].x : y == 1 ? r[3].y : y == 2 ? r[3].z : r[3].w;
-      // 4 x 4 bytes turned over
-      const uint32_t a0 = __byte_perm(w0, w1, 0x5140), a1 = __byte_perm(w0, w1, 0x7362);
-      const uint32_t b0 = __byte_perm(w2, w3, 0x5140), b1 = __byte_perm(w2, w3, 0x7362);
-      const uint32_t o[4] = {__byte_perm(a0, b0, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x5410),
-                             __byte_perm(a1, b1, 0x7632)};
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t w0 = y == 0 ? w[0].x : y == 1 ? w[0].y : y == 2 ? w[0].z : w[0].w;
+        const uint32_t w1 = y == 0 ? w[1].x : y == 1 ? w[1].y : y == 2 ? w[1].z : w[1].w;
+        const uint32_t w2 = y == 0 ? w[2].x : y == 1 ? w[2].y : y == 2 ? w[2].z : w[2].w;
+        const uint32_t w3 = y == 0 ? w[3].x : y == 1 ? w[3].y : y == 2 ? w[3].z : w[3].w;
+        // 4 x 4 bytes turned over
+        const uint32_t a0 = __byte_perm(w0, w1, 0x5140), a1 = __byte_perm(w0, w1, 0x7362);
+        const uint32_t b0 = __byte_perm(w2, w3, 0x5140), b1 = __byte_perm(w2, w3, 0x7362);
+        const uint32_t q[4] = {__byte_perm(a0, b0, 0x5410), __byte_perm(a0, b0, 0x7632), __byte_perm(a1, b1, 0x5410),
+                               __byte_perm(a1, b1, 0x7632)};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int s = 16 * g + 4 * y + x - k.first;
-        if (s < 0 || s >= k.n) continue;
-        store4(vo + s * row + d, bad ? make_float4(nan, nan, nan, nan) : values4<FMT>(o[x], vs));
+        for (int x = 0; x < 4; ++x) {
+          const int s = lo + 4 * y + x - k.first;
+          if (s >= 0 && s < k.n) store4(o + s * row, values4<FMT>(q[x], vs));
+        }
       }
     }
   }

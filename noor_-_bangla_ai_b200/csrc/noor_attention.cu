@@ -144,6 +144,23 @@ int64_t most_tasks(const noor_kv_cache* c, const noor_kv_batch* b) {
   return std::min<int64_t>(b->n_rows, b->n_rows / c->block + 2 * std::min<int64_t>(b->batch, b->n_rows));
 }
 
+// kv heads that one grid block takes in turn, so that finding its place and
+// (for keys) the angles is paid for once: as many as leave eight blocks for
+// every SM, at most 8.
+int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
+  int sms = 0;
+  CKR(sm_count(c->device, &sms));
+  *heads = 1;
+  while (*heads < 8 && *heads < c->n_kv_heads && tasks * c->n_kv_heads / (2 * *heads) >= 8 * (int64_t)sms) *heads *= 2;
+  return NOOR_MOE_OK;
+}
+
+// Four elements of a head can be loaded at once from any multiple of four.
+bool four_elements(const rope::View& v, int dtype) {
+  const size_t e = esize(dtype);
+  return reinterpret_cast<uintptr_t>(v.p) % (4 * e) == 0 && v.st % 4 == 0 && v.sh % 4 == 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -221,25 +238,33 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     a.r.q_out = view(q ? q_out : nullptr);
     a.r.hq = q ? q_heads : 0;
     a.q_tok = 4;
-    const int64_t kvb = most_tasks(c, b) * c->n_kv_heads, qb = q ? (b->n_rows + a.q_tok - 1) / a.q_tok : 0;
+    const int64_t tasks = most_tasks(c, b), qb = q ? (b->n_rows + a.q_tok - 1) / a.q_tok : 0;
+    CKR(heads_per_block(c, 2 * tasks, &a.heads));
+    const int64_t kvb = tasks * 2 * ((c->n_kv_heads + a.heads - 1) / a.heads);
     if (kvb + qb > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
     a.kv_blocks = (int32_t)kvb;
-    const bool vec = !q || vector_heads(a.r, dtype, {a.r.q, a.r.q_out});
-    const int smem = (int)std::max<size_t>((size_t)c->block * c->head_dim * (esize(dtype) + 1),
-                                           (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2));
+    a.kvec = four_elements(a.k, dtype);
+    a.vvec = four_elements(a.v, dtype);
+    a.qvec = q && vector_heads(a.r, dtype, {a.r.q, a.r.q_out});
+    const size_t smem = q ? (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
       auto go = [&](auto kern) -> int {
-        // the kernel's static arrays count against the 48 KB too
-        CKR(ensure_smem_limit(kern, smem > 47 * 1024 ? std::max(smem, 48 * 1024 + 1) : smem));
         kern<<<(unsigned)(kvb + qb), kv::kAppendThreads, smem, s>>>(a);
         CK(cudaGetLastError());
         return NOOR_MOE_OK;
       };
-      if (c->format == NOOR_KV_INT8)
-        return vec ? go(kv::append_kernel<T, kv::INT8, true>) : go(kv::append_kernel<T, kv::INT8, false>);
-      return vec ? go(kv::append_kernel<T, kv::E4M3, true>) : go(kv::append_kernel<T, kv::E4M3, false>);
+      // tokens a thread can own: a block's over the 256 / (head_dim / 4) that share a pair
+      const int share = kv::kAppendThreads / (c->head_dim / 4), own = (c->block + share - 1) / share;
+      auto by_own = [&](auto fmt) -> int {
+        if (own <= 2) return go(kv::append_kernel<T, fmt(), 2>);
+        if (own <= 4) return go(kv::append_kernel<T, fmt(), 4>);
+        if (own <= 8) return go(kv::append_kernel<T, fmt(), 8>);
+        return go(kv::append_kernel<T, fmt(), 16>);
+      };
+      return c->format == NOOR_KV_INT8 ? by_own(std::integral_constant<int, kv::INT8>{})
+                                       : by_own(std::integral_constant<int, kv::E4M3>{});
     });
   });
 }
@@ -255,8 +280,10 @@ int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* 
     if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
       return fail(NOOR_MOE_ERR_INVALID, "outputs must be 16-byte aligned");
     DeviceGuard g(c->device);
-    const kv::ReadArgs a{cache_of(c), batch_of(b), starts, k_out, v_out};
-    const int64_t grid = most_tasks(c, b) * c->n_kv_heads;
+    kv::ReadArgs a{cache_of(c), batch_of(b), starts, k_out, v_out, 1};
+    const int64_t tasks = most_tasks(c, b);
+    CKR(heads_per_block(c, 2 * tasks, &a.heads));
+    const int64_t grid = tasks * 2 * ((c->n_kv_heads + a.heads - 1) / a.heads);
     if (grid > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return by_dtype(dtype, [&](auto t) -> int {
