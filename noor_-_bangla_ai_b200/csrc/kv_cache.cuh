@@ -234,7 +234,8 @@ __device__ __forceinline__ float2 load2(const bf16* p) {
 template <int FMT>
 __device__ __forceinline__ uint32_t codes2(float x, float y) {
   if constexpr (FMT == INT8) {
-    // 1.5 2^23 + x rounds x to an integer, ties to even; |x| <= 127 by the scale's choice
+    // 1.5 2^23 + x rounds x to an integer, ties to even; |x| <= 127 by the
+    // scale's choice
     return (__float_as_uint(x + 12582912.f) & 0xFFu) | ((__float_as_uint(y + 12582912.f) & 0xFFu) << 8);
   } else {
     uint16_t r;
@@ -242,25 +243,6 @@ __device__ __forceinline__ uint32_t codes2(float x, float y) {
     return r;
   }
 }
-// The same in f64, rounded once.
-template <int FMT>
-__device__ __forceinline__ uint32_t codes2(double x, double y) {
-  if constexpr (FMT == INT8) {
-    // a rotated value may pass the scale's bound by its rounding: 127.0..01 is 127
-    return ((uint32_t)__double2loint(x + 6755399441055744.0) & 0xFFu) |
-           (((uint32_t)__double2loint(y + 6755399441055744.0) & 0xFFu) << 8);
-  } else {
-    // onto e4m3's grid (3 bits below the leading one, steps of 2^-9 at least)
-    // in f64, then exactly to f32 and the code
-    auto grid = [](double v) -> float {
-      const int e = max((__double2hiint(v) >> 20 & 0x7FF) - 1023, -6);
-      const double big = __hiloint2double(((e - 3 + 52 + 1023) << 20) | 0x80000, 0);
-      return (float)((v + big) - big);
-    };
-    return codes2<E4M3>(grid(x), grid(y));
-  }
-}
-
 // A block's old codes, four of a word, rounded again under a grown scale.
 template <int FMT>
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
@@ -269,14 +251,30 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
   return codes2<FMT>(a * ratio, b * ratio) | (codes2<FMT>(c * ratio, d * ratio) << 16);
 }
 
+// x rounded to f32 such that rounding that to a code gives what rounding x
+// would: where the nearest f32 could be a border of a code or of a scale (they
+// have at most 9 significant bits) and x is not it, the neighbour on x's side.
+// Powers of two scale both alike, so this can come before the scale is known.
+__device__ __forceinline__ float toward(double x) {
+  float h = (float)x;
+  if ((__float_as_uint(h) & 0x7FFFu) == 0) {
+    const double r = x - (double)h;
+    if (r != 0.0 && h == h) {
+      const bool up = (r > 0.0) == (h > 0.0);  // away from zero
+      if (h == 0.f) h = r > 0.0 ? 1e-45f : -1e-45f;
+      else h = __uint_as_float(__float_as_uint(h) + (up ? 1 : -1));
+    }
+  }
+  return h;
+}
+
 // Keys of one touched block, kv heads h0 .. h1 - 1.  A thread owns two pairs of
 // a head and every G-th token; a decode step's single token leaves room for
 // several heads at once.  Its angle is made once in f64 and advanced from
 // token to token by the angle of G positions (a complex product; 16 of them
 // lose a few units of 2^-53), so a sine and cosine pair is paid for once per
-// thread and not per element.  The largest magnitude is found in f32; only
-// where that falls within 1e-5 of a power of two's bound is it found again in
-// f64.  The codes are rounded from the f64 rotation.
+// thread and not per element.  The rotation is done in f64 and kept as the f32
+// that rounds alike, so the codes are those of the exact rotation.
 // Bound by memory once enough blocks run: the elements are read once into
 // registers.
 template <typename T, int FMT, int TPT>
@@ -333,56 +331,31 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
         }
       }
     }
-    // ---- scale
+    // ---- rotate; the largest magnitude chooses the scale
     uint32_t amax = 0;
-    {
-      float c1[2] = {(float)c0[0], (float)c0[1]}, s1[2] = {(float)s0[0], (float)s0[1]};
-      const float cf[2] = {(float)cg[0], (float)cg[1]}, sf[2] = {(float)sg[0], (float)sg[1]};
+    double c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
 #pragma unroll
-      for (int j = 0; j < TPT; ++j) {
-        if (G * j >= k.n) break;
-        const float v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float y0 = v[2 * y] * c1[y] - v[2 * y + 1] * s1[y], y1 = v[2 * y] * s1[y] + v[2 * y + 1] * c1[y];
-          amax = max(amax, max(__float_as_uint(fabsf(y0)), __float_as_uint(fabsf(y1))));
-          const float cn = c1[y] * cf[y] - s1[y] * sf[y];
-          s1[y] = s1[y] * cf[y] + c1[y] * sf[y];
-          c1[y] = cn;
-        }
-      }
-    }
-    amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
-    // (84 steps of 2^-23 are 1e-5; a block's heads decide together)
-    const bool border = live && rot > 0 && amax < 0x7F800000u - 84 &&
-                        scale_for<FMT>(amax - min(amax, 84u)) != scale_for<FMT>(amax + 84u);
-    if (__syncthreads_or(border)) {
-      __shared__ unsigned long long s_exact[kHeadsAtOnce];
-      if (tid < kHeadsAtOnce) s_exact[tid] = 0;
-      __syncthreads();
-      double m = 0.0, c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
-#pragma unroll 1
-      for (int s = g; live && s < k.n; s += G) {
-        const T* p = kp + s * a.k.st;
-        const double v[4] = {(double)rope::to_f32(p[d0]), (double)rope::to_f32(p[d1]), (double)rope::to_f32(p[d2]),
-                             (double)rope::to_f32(p[d3])};
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          m = fmax(m, fmax(fabs(v[2 * y] * c1[y] - v[2 * y + 1] * s1[y]), fabs(v[2 * y] * s1[y] + v[2 * y + 1] * c1[y])));
+    for (int j = 0; j < TPT; ++j) {
+      if (G * j >= k.n) break;
+      auto turn = [&](float& u, float& v, int y) {
+        if (turned[y]) {
+          const double a0 = u, a1 = v;
+          u = toward(a0 * c1[y] - a1 * s1[y]);
+          v = toward(a0 * s1[y] + a1 * c1[y]);
           const double cn = c1[y] * cg[y] - s1[y] * sg[y];
           s1[y] = s1[y] * cg[y] + c1[y] * sg[y];
           c1[y] = cn;
         }
-      }
-      if (live) atomicMax(&s_exact[hl], (unsigned long long)__double_as_longlong(m));
-      __syncthreads();
-      if (border) amax = __float_as_uint(__double2float_ru(__longlong_as_double((long long)s_exact[hl])));
-      __syncthreads();
+        amax = max(amax, max(__float_as_uint(fabsf(u)), __float_as_uint(fabsf(v))));
+      };
+      turn(x[j].x, x[j].y, 0);
+      turn(x[j].z, x[j].w, 1);
     }
+    amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
     if (!live) continue;
     const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
     const bool poisoned = scale != scale;
-    const double inv = 1.0 / (double)scale;
+    const float inv = 1.f / scale;
     uint8_t* kc = c.k + ph * blk * D;
     // ---- the old codes under a grown scale
     if (k.first > 0 && scale != s_old) {
@@ -393,24 +366,12 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
       }
     }
     // ---- codes of the new tokens
-    double c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
 #pragma unroll
     for (int j = 0; j < TPT; ++j) {
       const int s = g + G * j;
       if (s >= k.n) break;
-      double v[4] = {(double)x[j].x, (double)x[j].y, (double)x[j].z, (double)x[j].w};
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        if (turned[y]) {
-          const double y0 = v[2 * y] * c1[y] - v[2 * y + 1] * s1[y], y1 = v[2 * y] * s1[y] + v[2 * y + 1] * c1[y];
-          v[2 * y] = y0;
-          v[2 * y + 1] = y1;
-          const double cn = c1[y] * cg[y] - s1[y] * sg[y];
-          s1[y] = s1[y] * cg[y] + c1[y] * sg[y];
-          c1[y] = cn;
-        }
-      }
-      const uint32_t e = poisoned ? 0 : codes2<FMT>(v[0] * inv, v[1] * inv), f = poisoned ? 0 : codes2<FMT>(v[2] * inv, v[3] * inv);
+      const uint32_t e = poisoned ? 0 : codes2<FMT>(x[j].x * inv, x[j].y * inv),
+                     f = poisoned ? 0 : codes2<FMT>(x[j].z * inv, x[j].w * inv);
       uint8_t* o = kc + (int64_t)(k.first + s) * D;
       if (run) {
         *reinterpret_cast<uint32_t*>(o + d0) = e | (f << 16);
@@ -449,7 +410,7 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
     const float s_old = k.first > 0 ? __ldg(c.vs + ph) : 0.f;
     uint8_t* vc = c.v + ph * blk * D + (int64_t)d * blk + lo;
     typename std::conditional<sizeof(T) == 2, uint2, float4>::type x[16];
-    uint32_t amax = 0;
+    uint32_t amax = 0, amax2 = 0;
     if (live) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -466,9 +427,7 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
             x[i] = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
           }
         }
-        // magnitudes of both halves, in f32's bits
-        amax = max(amax, max(max((x[i].x << 16) & 0x7FFFFFFFu, x[i].x & 0x7FFF0000u),
-                             max((x[i].y << 16) & 0x7FFFFFFFu, x[i].y & 0x7FFF0000u)));
+        amax2 = __vmaxu2(amax2, __vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu));  // magnitudes, two at a time
       } else {
         x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (in) x[i] = a.vvec ? load4(p) : make_float4(p[0], p[1], p[2], p[3]);
@@ -477,6 +436,7 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
       }
     }
     }
+    if constexpr (sizeof(T) == 2) amax = max(amax2 & 0x7FFF0000u, amax2 << 16);
     amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
     if (!live) continue;
     const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
@@ -585,6 +545,7 @@ template <typename T, int FMT, int TPT>
 __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kernel(const AppendArgs a) {
   extern __shared__ __align__(16) uint8_t s_append[];
   __shared__ Maxima s_max;
+  __shared__ Task s_task;
   if ((int)blockIdx.x >= a.kv_blocks) {
     if (a.qvec)
       append_rotate_q<T, true>(a, s_append);
@@ -593,16 +554,28 @@ __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kern
     return;
   }
   if (threadIdx.x < kHeadsAtOnce) s_max.m[0][threadIdx.x] = 0;
-  __syncthreads();
   const int groups = (a.c.H + a.heads - 1) / a.heads;
   const int t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
-  const Task k = find_task(a.c, a.b, nullptr, true, t, threadIdx.x & 31);
+  if (threadIdx.x < 32) {
+    const Task f = find_task(a.c, a.b, nullptr, true, t, threadIdx.x);
+    if (threadIdx.x == 0) s_task = f;
+  }
+  __syncthreads();
+  const Task k = s_task;
   if (k.b < 0 || k.page < 0) return;
   const int h0 = (r >> 1) * a.heads, h1 = min(h0 + a.heads, a.c.H);
   if (r & 1)
     append_values<T, FMT>(a, k, h0, h1, s_max);
   else
     append_keys<T, FMT, TPT>(a, k, h0, h1, s_max);
+}
+
+// The rotation of q by itself, for batches whose q would wait for the few
+// blocks that the registers of append_kernel let run at once.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kAppendThreads) rotate_q_kernel(const AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t s_rotate[];
+  append_rotate_q<T, VEC>(a, s_rotate);
 }
 
 // ------------------------------------------------------------- read back
@@ -662,7 +635,13 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
   const int D = c.D, blk = c.blk, tid = threadIdx.x;
   const int groups = (c.H + a.heads - 1) / a.heads, t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
   const int h0 = (r >> 1) * a.heads, nh = min(a.heads, c.H - h0);
-  const Task k = find_task(c, a.b, a.starts, false, t, tid & 31);
+  __shared__ Task s_task;
+  if (tid < 32) {
+    const Task f = find_task(c, a.b, a.starts, false, t, tid);
+    if (tid == 0) s_task = f;
+  }
+  __syncthreads();
+  const Task k = s_task;
   if (k.b < 0) return;
   const bool bad = k.page < 0;
   const float nan = __uint_as_float(0x7FC00000u);

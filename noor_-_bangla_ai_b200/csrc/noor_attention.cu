@@ -155,6 +155,9 @@ int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
   return NOOR_MOE_OK;
 }
 
+// Blocks of q rotation (4 rows each) from which they get their own launch.
+constexpr int64_t kApartBlocks = 256;
+
 // Four elements of a head can be loaded at once from any multiple of four.
 bool four_elements(const rope::View& v, int dtype) {
   const size_t e = esize(dtype);
@@ -240,6 +243,9 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     a.q_tok = 4;
     const int64_t tasks = most_tasks(c, b), qb = q ? (b->n_rows + a.q_tok - 1) / a.q_tok : 0;
     CKR(heads_per_block(c, 2 * tasks, &a.heads));
+    // few tokens a block leave its threads room for more heads
+    const int64_t per_head = std::min<int64_t>(b->n_rows / tasks, 64) * (c->head_dim / 4);
+    a.heads = (int32_t)std::max<int64_t>(a.heads, std::min<int64_t>(c->n_kv_heads, kv::kAppendThreads / std::max<int64_t>(per_head, 1)));
     const int64_t kvb = tasks * 2 * ((c->n_kv_heads + a.heads - 1) / a.heads);
     if (kvb + qb > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
     a.kv_blocks = (int32_t)kvb;
@@ -248,10 +254,21 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     a.qvec = q && vector_heads(a.r, dtype, {a.r.q, a.r.q_out});
     const size_t smem = q ? (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // q in blocks of the same launch, or where there is much of it in its own
+    const bool apart = qb >= kApartBlocks;
     return by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
+      if (apart) {
+        kv::AppendArgs alone = a;
+        alone.kv_blocks = 0;
+        if (a.qvec)
+          kv::rotate_q_kernel<T, true><<<(unsigned)qb, kv::kAppendThreads, smem, s>>>(alone);
+        else
+          kv::rotate_q_kernel<T, false><<<(unsigned)qb, kv::kAppendThreads, smem, s>>>(alone);
+        CK(cudaGetLastError());
+      }
       auto go = [&](auto kern) -> int {
-        kern<<<(unsigned)(kvb + qb), kv::kAppendThreads, smem, s>>>(a);
+        kern<<<(unsigned)(kvb + (apart ? 0 : qb)), kv::kAppendThreads, smem, s>>>(a);
         CK(cudaGetLastError());
         return NOOR_MOE_OK;
       };
