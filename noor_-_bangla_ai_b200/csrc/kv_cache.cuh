@@ -218,16 +218,25 @@ __device__ __forceinline__ uint32_t head_max(uint32_t v, int hl, Maxima& s, int 
   return hl < kHeadsAtOnce ? m[hl] : 0;
 }
 
-// Four elements as floats.
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const bf16* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  return make_float4(bf16_lo(r.x), bf16_hi(r.x), bf16_lo(r.y), bf16_hi(r.y));
+// Four elements as they are stored.
+template <typename T>
+using Raw4 = typename std::conditional<sizeof(T) == 2, uint2, float4>::type;
+__device__ __forceinline__ float4 two_runs(const float* p, const float* q) {
+  const float2 u = *reinterpret_cast<const float2*>(p), v = *reinterpret_cast<const float2*>(q);
+  return make_float4(u.x, u.y, v.x, v.y);
 }
-__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ __forceinline__ float2 load2(const bf16* p) {
-  const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
-  return make_float2(bf16_lo(r), bf16_hi(r));
+__device__ __forceinline__ uint2 two_runs(const bf16* p, const bf16* q) {
+  return make_uint2(*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(q));
+}
+__device__ __forceinline__ float4 four(float a, float b, float c, float d) { return make_float4(a, b, c, d); }
+__device__ __forceinline__ uint2 four(bf16 a, bf16 b, bf16 c, bf16 d) {
+  return make_uint2(__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16,
+                    __bfloat16_as_ushort(c) | (uint32_t)__bfloat16_as_ushort(d) << 16);
+}
+// As floats; `turned`: runs (0, 2) and (1, 3) were loaded and the pairs are (0, 1), (2, 3).
+__device__ __forceinline__ float4 widen4(float4 r, bool turned) { return turned ? make_float4(r.x, r.z, r.y, r.w) : r; }
+__device__ __forceinline__ float4 widen4(uint2 r, bool turned) {
+  return widen4(make_float4(bf16_lo(r.x), bf16_hi(r.x), bf16_lo(r.y), bf16_hi(r.y)), turned);
 }
 
 // Codes of two values in steps, x in the low byte.
@@ -307,30 +316,39 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
       if (g + G < k.n) sincospi(2.0 * rope::turn_fraction(G, f), &sg[x], &cg[x]);
     }
   }
+  Raw4<T> raw[TPT];
+  auto load = [&](int hb) {
+    const bool live = thread_live && hb + hl < h1;
+    const T* kp = static_cast<const T*>(a.k.p) + (int64_t)k.row0 * a.k.st + (hb + hl) * a.k.sh;
+#pragma unroll
+    for (int j = 0; j < TPT; ++j) {
+      if (G * j >= k.n) break;
+      const int s = g + G * j;
+      raw[j] = Raw4<T>{};
+      if (live && s < k.n) {
+        const T* p = kp + s * a.k.st;
+        if (a.kvec && run)
+          raw[j] = *reinterpret_cast<const Raw4<T>*>(p + d0);
+        else if (a.kvec && split)
+          raw[j] = two_runs(p + d0, p + d1);
+        else
+          raw[j] = four(p[d0], p[d1], p[d2], p[d3]);
+      }
+    }
+  };
+  load(h0);
   for (int hb = h0, pass = 0; hb < h1; hb += at_once, ++pass) {
     const int h = hb + hl;
     const bool live = thread_live && h < h1;
     const int64_t ph = k.page * c.H + (live ? h : hb);
-    const T* kp = static_cast<const T*>(a.k.p) + (int64_t)k.row0 * a.k.st + h * a.k.sh;
     const float s_old = k.first > 0 ? __ldg(c.ks + ph) : 0.f;
     float4 x[TPT];
 #pragma unroll
     for (int j = 0; j < TPT; ++j) {
       if (G * j >= k.n) break;
-      const int s = g + G * j;
-      x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (live && s < k.n) {
-        const T* p = kp + s * a.k.st;
-        if (a.kvec && run) {
-          x[j] = load4(p + d0);
-        } else if (a.kvec && split) {
-          const float2 u = load2(p + d0), v = load2(p + d1);
-          x[j] = make_float4(u.x, v.x, u.y, v.y);
-        } else {
-          x[j] = make_float4(rope::to_f32(p[d0]), rope::to_f32(p[d1]), rope::to_f32(p[d2]), rope::to_f32(p[d3]));
-        }
-      }
+      x[j] = widen4(raw[j], a.kvec && !run && split);
     }
+    if (hb + at_once < h1) load(hb + at_once);  // the next heads', while these are worked on
     // ---- rotate; the largest magnitude chooses the scale
     uint32_t amax = 0;
     double c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
@@ -389,54 +407,79 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
   }
 }
 
-// Values of one touched block: a thread takes 4 dims of 16 tokens in
+// Values of one touched block: a thread takes DPT dims of 16 tokens in
 // registers, turns the codes over and writes 16 tokens of each dim, the
 // cache's order.  Where a 16-token run is not all new it is read, merged and
 // written back (this block alone owns the page).  Only runs with new tokens
 // take threads; where they leave room, several heads are done at once.
-template <typename T, int FMT>
+template <typename T, int FMT, int DPT>
 __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1, Maxima& s_max) {
   const Cache& c = a.c;
-  const int D = c.D, blk = c.blk, tid = threadIdx.x, quads = D >> 2;
+  const int D = c.D, blk = c.blk, tid = threadIdx.x, parts = D / DPT;
   const int r0 = k.first >> 4, runs = ((k.first + k.n - 1) >> 4) - r0 + 1;
-  const int slots = quads * runs, at_once = kAppendThreads / slots;   // at most 4 x 64
-  const int hl = tid / slots, run = (tid - hl * slots) / quads, d = (tid % quads) * 4, lo = 16 * (r0 + run);
+  const int slots = parts * runs, at_once = kAppendThreads / slots;   // at most 4 x 64
+  const int hl = tid / slots, run = (tid - hl * slots) / parts, d = (tid % parts) * DPT, lo = 16 * (r0 + run);
   const bool all_new = lo >= k.first && lo + 16 <= k.first + k.n;
+  // 16 tokens of DPT dims as they are stored, in 32-bit words
+  constexpr int W = DPT * (int)sizeof(T) / 4;
+  uint32_t next[16][W];
+  auto load = [&](int hb) {
+    const bool live = hl < at_once && hb + hl < h1;
+    const T* vp = static_cast<const T*>(a.v.p) + (int64_t)k.row0 * a.v.st + (hb + hl) * a.v.sh + d;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int s = lo + i - k.first;
+#pragma unroll
+      for (int x = 0; x < W; ++x) next[i][x] = 0;
+      if (live && s >= 0 && s < k.n) {
+        const T* p = vp + s * a.v.st;
+        if constexpr (W == 4) {
+          if (a.vvec) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            next[i][0] = u.x; next[i][1] = u.y; next[i][2] = u.z; next[i][3] = u.w;
+            continue;
+          }
+        } else if constexpr (W == 2) {
+          if (a.vvec) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            next[i][0] = u.x; next[i][1] = u.y;
+            continue;
+          }
+        } else {
+          if (a.vvec) {
+            next[i][0] = *reinterpret_cast<const uint32_t*>(p);
+            continue;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+          if constexpr (sizeof(T) == 2) {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(p) + 2 * x;
+            next[i][x] = e[0] | (uint32_t)e[1] << 16;
+          } else {
+            next[i][x] = __float_as_uint(p[x]);
+          }
+        }
+      }
+    }
+  };
+  load(h0);
   for (int hb = h0, pass = 0; hb < h1; hb += at_once, ++pass) {
     const int h = hb + hl;
     const bool live = hl < at_once && h < h1;
     const int64_t ph = k.page * c.H + (live ? h : hb);
-    const T* vp = static_cast<const T*>(a.v.p) + (int64_t)k.row0 * a.v.st + h * a.v.sh + d;
     const float s_old = k.first > 0 ? __ldg(c.vs + ph) : 0.f;
     uint8_t* vc = c.v + ph * blk * D + (int64_t)d * blk + lo;
-    typename std::conditional<sizeof(T) == 2, uint2, float4>::type x[16];
-    uint32_t amax = 0, amax2 = 0;
-    if (live) {
+    uint32_t x[16][W], amax = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int s = lo + i - k.first;
-      const bool in = s >= 0 && s < k.n;
-      const T* p = vp + s * a.v.st;
-      if constexpr (sizeof(T) == 2) {
-        x[i] = make_uint2(0, 0);
-        if (in) {
-          if (a.vvec) {
-            x[i] = *reinterpret_cast<const uint2*>(p);
-          } else {
-            const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
-            x[i] = make_uint2(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16);
-          }
-        }
-        amax2 = __vmaxu2(amax2, __vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu));  // magnitudes, two at a time
-      } else {
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in) x[i] = a.vvec ? load4(p) : make_float4(p[0], p[1], p[2], p[3]);
-        amax = max(amax, max(max(__float_as_uint(fabsf(x[i].x)), __float_as_uint(fabsf(x[i].y))),
-                             max(__float_as_uint(fabsf(x[i].z)), __float_as_uint(fabsf(x[i].w)))));
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int y = 0; y < W; ++y) {
+        x[i][y] = next[i][y];
+        amax = sizeof(T) == 2 ? __vmaxu2(amax, x[i][y] & 0x7FFF7FFFu) : max(amax, x[i][y] & 0x7FFFFFFFu);
       }
-    }
-    }
-    if constexpr (sizeof(T) == 2) amax = max(amax2 & 0x7FFF0000u, amax2 << 16);
+    if constexpr (sizeof(T) == 2) amax = max(amax & 0x7FFF0000u, amax << 16);
+    if (hb + at_once < h1) load(hb + at_once);  // the next heads', while these are worked on
     amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
     if (!live) continue;
     const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
@@ -454,53 +497,45 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
         *p = o;
       }
     }
-    uint4 old[4];
-    if (!all_new) {
+    auto value = [&](int i, int y) -> float {  // dim y of token i
+      if constexpr (sizeof(T) == 2)
+        return (y & 1) ? bf16_hi(x[i][y >> 1]) : bf16_lo(x[i][y >> 1]);
+      else
+        return __uint_as_float(x[i][y]);
+    };
 #pragma unroll
-      for (int y = 0; y < 4; ++y) old[y] = *reinterpret_cast<const uint4*>(vc + (int64_t)y * blk);
-    }
-    uint32_t w[4][4];  // [dim][word of 4 tokens]
-#pragma unroll
-    for (int z = 0; z < 4; ++z) {
-      uint32_t t[4];  // a token's 4 codes
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float4 v;
-        if constexpr (sizeof(T) == 2)
-          v = make_float4(bf16_lo(x[4 * z + i].x), bf16_hi(x[4 * z + i].x), bf16_lo(x[4 * z + i].y), bf16_hi(x[4 * z + i].y));
-        else
-          v = x[4 * z + i];
-        t[i] = poisoned ? 0 : codes2<FMT>(v.x * inv, v.y * inv) | (codes2<FMT>(v.z * inv, v.w * inv) << 16);
-      }
-      const uint32_t a0 = __byte_perm(t[0], t[1], 0x5140), a1 = __byte_perm(t[0], t[1], 0x7362);
-      const uint32_t b0 = __byte_perm(t[2], t[3], 0x5140), b1 = __byte_perm(t[2], t[3], 0x7362);
-      w[0][z] = __byte_perm(a0, b0, 0x5410);
-      w[1][z] = __byte_perm(a0, b0, 0x7632);
-      w[2][z] = __byte_perm(a1, b1, 0x5410);
-      w[3][z] = __byte_perm(a1, b1, 0x7632);
-    }
-    if (!all_new) {
+    for (int y = 0; y < DPT; y += 2) {
+      uint32_t w[2][4];  // [dim y, y + 1][word of 4 tokens]
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
-        // bytes of new tokens and of old ones in this word
-        uint32_t mn = 0, mo = 0;
+        uint32_t t[4];  // a token's 2 codes
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int s = lo + 4 * z + i;
-          if (s < k.first) mo |= 0xFFu << (8 * i);
-          else if (s < k.first + k.n) mn |= 0xFFu << (8 * i);
-        }
+        for (int i = 0; i < 4; ++i)
+          t[i] = poisoned ? 0 : codes2<FMT>(value(4 * z + i, y) * inv, value(4 * z + i, y + 1) * inv);
+        const uint32_t lo2 = __byte_perm(t[0], t[1], 0x5410), hi2 = __byte_perm(t[2], t[3], 0x5410);
+        w[0][z] = __byte_perm(lo2, hi2, 0x6420);
+        w[1][z] = __byte_perm(lo2, hi2, 0x7531);
+      }
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint32_t o = z == 0 ? old[y].x : z == 1 ? old[y].y : z == 2 ? old[y].z : old[y].w;
-          uint32_t kept = o;
-          if (grow && mo) kept = (o & ~mo) | ((poisoned ? 0 : recode4<FMT>(o, ratio)) & mo);
-          w[y][z] = (w[y][z] & mn) | (kept & ~mn);
+      for (int e = 0; e < 2; ++e) {
+        uint4* dst = reinterpret_cast<uint4*>(vc + (int64_t)(y + e) * blk);
+        if (!all_new) {
+          const uint4 was = *dst;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            // bytes of new tokens and of old ones in this word
+            const int s = lo + 4 * z, n_old = min(max(k.first - s, 0), 4), n_end = min(max(k.first + k.n - s, 0), 4);
+            const uint32_t mo = n_old == 4 ? 0xFFFFFFFFu : (1u << (8 * n_old)) - 1u;
+            const uint32_t mn = (n_end == 4 ? 0xFFFFFFFFu : (1u << (8 * n_end)) - 1u) & ~mo;
+            const uint32_t o = z == 0 ? was.x : z == 1 ? was.y : z == 2 ? was.z : was.w;
+            uint32_t kept = o;
+            if (grow && mo) kept = (o & ~mo) | ((poisoned ? 0 : recode4<FMT>(o, ratio)) & mo);
+            w[e][z] = (w[e][z] & mn) | (kept & ~mn);
+          }
         }
+        *dst = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
       }
     }
-#pragma unroll
-    for (int y = 0; y < 4; ++y) *reinterpret_cast<uint4*>(vc + (int64_t)y * blk) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
   }
 }
 
@@ -565,7 +600,7 @@ __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kern
   if (k.b < 0 || k.page < 0) return;
   const int h0 = (r >> 1) * a.heads, h1 = min(h0 + a.heads, a.c.H);
   if (r & 1)
-    append_values<T, FMT>(a, k, h0, h1, s_max);
+    append_values<T, FMT, TPT == 16 ? 4 : 2>(a, k, h0, h1, s_max);
   else
     append_keys<T, FMT, TPT>(a, k, h0, h1, s_max);
 }

@@ -275,9 +275,8 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
       // tokens a thread can own: a block's over the 256 / (head_dim / 4) that share a pair
       const int share = kv::kAppendThreads / (c->head_dim / 4), own = (c->block + share - 1) / share;
       auto by_own = [&](auto fmt) -> int {
-        if (own <= 2) return go(kv::append_kernel<T, fmt(), 2>);
-        if (own <= 4) return go(kv::append_kernel<T, fmt(), 4>);
-        if (own <= 8) return go(kv::append_kernel<T, fmt(), 8>);
+        if (own <= 4 && c->head_dim <= 128) return go(kv::append_kernel<T, fmt(), 4>);
+        if (c->head_dim <= 128) return go(kv::append_kernel<T, fmt(), 8>);
         return go(kv::append_kernel<T, fmt(), 16>);
       };
       return c->format == NOOR_KV_INT8 ? by_own(std::integral_constant<int, kv::INT8>{})
