@@ -56,6 +56,7 @@ struct Args {
   rope::View q, out;
   float* lse;
   int32_t Hq, g;   // query heads, query heads per kv head
+  bool qvec;       // q can be read four elements at a time
   float scale2;    // scale * log2(e)
   int32_t window;
   // partial results: [2 * pairs] slots of `rows` rows of D o's, and of `rows` (m, l)
@@ -199,19 +200,22 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   pair_sync(pair);
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be launched; it waits for this grid's end
   // ---- this pair's share of the list
   const int wid = pair * gridDim.x + blockIdx.x;
-  int64_t total = 0;
+  int64_t total = 0, n0 = 0;  // n0: tiles of this lane's sequence among the first 32
   for (int base = 0; base < a.b.B; base += 32) {
     int64_t n = 0;
     if (base + lane < a.b.B) {
       const SeqWork w = seq_work(a, base + lane);
       n = (int64_t)w.rtiles * w.tiles * a.c.H;
     }
+    if (base == 0) n0 = n;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     total += n;
   }
+  if (wid >= a.pairs) return;
   if (half == 0 && lane == 0) a.desc[wid] = make_int4(-1, 0, 0, 0);
   // no more shares than tiles: every share has one, so a cut unit's parts lie
   // in consecutive pairs
@@ -224,10 +228,13 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   {
     bool found = false;
     for (int base = 0; base < a.b.B && !found; base += 32) {
-      int64_t n = 0;
-      if (base + lane < a.b.B) {
-        const SeqWork w = seq_work(a, base + lane);
-        n = (int64_t)w.rtiles * w.tiles * a.c.H;
+      int64_t n = n0;
+      if (base > 0) {
+        n = 0;
+        if (base + lane < a.b.B) {
+          const SeqWork w = seq_work(a, base + lane);
+          n = (int64_t)w.rtiles * w.tiles * a.c.H;
+        }
       }
       int64_t incl = n;
 #pragma unroll
@@ -353,9 +360,23 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       const T* qp = nullptr;
       if (r < nrows)
         qp = static_cast<const T*>(a.q.p) + (int64_t)(w.s.row0 + e / a.g) * a.q.st + (int64_t)(h * a.g + e % a.g) * a.q.sh;
+      // the quad's four lanes hold the whole row between them; all its loads are
+      // in flight together
+      kv::Raw4<T> raw[DP / 16];
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
+        raw[ks] = kv::Raw4<T>{};
+        if (qp != nullptr && d0 < D)
+          raw[ks] = a.qvec ? *reinterpret_cast<const kv::Raw4<T>*>(qp + d0)
+                           : kv::four(qp[d0], qp[d0 + 1], qp[d0 + 2], qp[d0 + 3]);
+      }
       float mx = 0.f;
-      if (qp != nullptr)
-        for (int d = qc; d < D; d += 4) mx = fmaxf(mx, fabsf(rope::to_f32(qp[d])));
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const float4 v = kv::widen4(raw[ks], false);
+        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+      }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       // 2^e <= mx < 2^(e + 1) becomes 2^14: up = 2^(14 - e), within f32's exponents
@@ -366,12 +387,9 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       qfac[nb][1] = __shfl_sync(0xffffffffu, down, 8 * qc + 4);
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
-        float v[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = qp != nullptr && d0 < D ? rope::to_f32(qp[d0 + x]) * up : 0.f;
-        const uint2 hi = make_uint2(pack_half(v[0], v[1]), pack_half(v[2], v[3]));
-        const uint2 lo = make_uint2(pack_rest(v[0], v[1], hi.x), pack_rest(v[2], v[3], hi.y));
+        const float4 v = kv::widen4(raw[ks], false);
+        const uint2 hi = make_uint2(pack_half(v.x * up, v.y * up), pack_half(v.z * up, v.w * up));
+        const uint2 lo = make_uint2(pack_rest(v.x * up, v.y * up, hi.x), pack_rest(v.z * up, v.w * up, hi.y));
         if constexpr (Sh::kQShared) {
           if (half == 0) {  // both warps use it
             s_q[(ks * NB + nb) * 32 + lane] = hi;
@@ -663,6 +681,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 // later pair's is its first (slot 0).
 template <typename T>
 __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched while the streamed kernel still runs)
   const int wid = blockIdx.x, r = blockIdx.y;
   const int4 d = a.desc[wid];
   if (d.x < 0) return;
@@ -684,6 +703,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Args a) {
   T* op = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
   for (int c = threadIdx.x; c < D; c += blockDim.x) {
     float acc = 0.f, l = 0.f;
+#pragma unroll 4
     for (int i = wid; i <= last; ++i) {
       const int64_t slot = (i == wid ? slot0 : 2 * (int64_t)i) * a.rows + r;
       const float mi = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1];

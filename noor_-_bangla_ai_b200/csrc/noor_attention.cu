@@ -155,8 +155,8 @@ int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
   return NOOR_MOE_OK;
 }
 
-// Blocks of q rotation (4 rows each) from which they get their own launch.
-constexpr int64_t kApartBlocks = 256;
+// Rows of q from which its rotation gets its own launch.
+constexpr int64_t kApartRows = 1024;
 
 // Four elements of a head can be loaded at once from any multiple of four.
 bool four_elements(const rope::View& v, int dtype) {
@@ -189,7 +189,12 @@ int noor_rope_apply(const noor_rotary* r, const noor_heads* q, const noor_heads*
     DeviceGuard g(device);
     rope::Args a{r->inv_freq, r->rotate_dim, r->layout, r->factor, inverse ? -1.f : 1.f, view(q), view(q_out),
                  view(k), view(k ? k_out : nullptr), q_heads, k ? k_heads : 0, head_dim, positions, tokens};
-    const int tok = 4;
+    // tokens of a block: one for a decode step, whose time is latency, up to 4
+    // while eight blocks for every SM remain
+    int sms = 0;
+    CKR(sm_count(device, &sms));
+    int tok = 4;
+    while (tok > 1 && tokens / tok < 8 * sms) tok /= 2;
     const unsigned grid = (unsigned)((tokens + tok - 1) / tok);
     const size_t smem = (size_t)tok * (r->rotate_dim / 2) * sizeof(float2);
     const bool vec = vector_heads(a, dtype, {a.q, a.q_out, a.k, a.k_out});
@@ -240,7 +245,10 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     a.r.q = view(q);
     a.r.q_out = view(q ? q_out : nullptr);
     a.r.hq = q ? q_heads : 0;
+    int sms = 0;
+    CKR(sm_count(c->device, &sms));
     a.q_tok = 4;
+    while (a.q_tok > 1 && b->n_rows / a.q_tok < 8 * sms) a.q_tok /= 2;
     const int64_t tasks = most_tasks(c, b), qb = q ? (b->n_rows + a.q_tok - 1) / a.q_tok : 0;
     CKR(heads_per_block(c, 2 * tasks, &a.heads));
     // few tokens a block leave its threads room for more heads
@@ -255,7 +263,7 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     const size_t smem = q ? (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // q in blocks of the same launch, or where there is much of it in its own
-    const bool apart = qb >= kApartBlocks;
+    const bool apart = q && b->n_rows >= kApartRows;
     return by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
       if (apart) {
@@ -344,7 +352,7 @@ int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_
   const int64_t tiles = ((int64_t)b->max_blocks * c->block + attn::kTile - 1) / attn::kTile;
   const double most = (double)rtiles * c->n_kv_heads * tiles;
   p->grid = (int)std::min<double>(sms, std::max(1.0, most));
-  p->pairs = p->grid * per;
+  p->pairs = (int)std::min<double>((double)p->grid * per, std::max(1.0, most));  // no share without a tile
   p->off_ml = (int64_t)p->pairs * 2 * R * c->head_dim * 4;
   p->off_desc = p->off_ml + (int64_t)p->pairs * 2 * R * 2 * 4;
   p->bytes = p->off_desc + (int64_t)p->pairs * 16;
@@ -415,6 +423,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     a.lse = lse;
     a.Hq = q_heads;
     a.g = q_heads / c->n_kv_heads;
+    a.qvec = four_elements(a.q, dtype);
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window;
     a.pairs = p.pairs;
@@ -442,8 +451,17 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
       CKR(c->format == NOOR_KV_INT8 ? attn::stream_f32_int8(a, p.nb, p.grid, s) : attn::stream_f32_e4m3(a, p.nb, p.grid, s));
     return by_dtype(dtype, [&](auto t) -> int {
       const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g);
-      attn::combine_kernel<decltype(t)><<<dim3((unsigned)p.pairs, (unsigned)rows), 128, 0, s>>>(a);
-      CK(cudaGetLastError());
+      // launched behind the streamed kernel without waiting for its end
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3((unsigned)p.pairs, (unsigned)rows);
+      cfg.blockDim = dim3(128);
+      cfg.stream = s;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      CK(cudaLaunchKernelEx(&cfg, attn::combine_kernel<decltype(t)>, a));
       return NOOR_MOE_OK;
     });
   });

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const Args a, int tok) {
   __syncthreads();
   const int units = head_units<T, VEC>(a.D, a.rot, a.layout);
   const int heads = a.hq + a.hk, per_tok = heads * units;
+#pragma unroll 2
   for (int i = threadIdx.x; i < nt * per_tok; i += blockDim.x) {
     const int t = i / per_tok, r = i - t * per_tok;
     int h = r / units;
