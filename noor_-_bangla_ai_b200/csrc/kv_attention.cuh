@@ -163,7 +163,7 @@ struct Shape {
   static constexpr int kRows = 8 * NB;
   static constexpr bool kQShared = DP / 8 * NB * PARTS > 32;
   static constexpr int kPairs = DP == 64 ? (NB == 1 ? 8 : 4)
-                                : DP == 128 ? (NB == 1 ? (PARTS == 1 ? 7 : 6) : 4)
+                                : DP == 128 ? (NB == 1 ? 6 : 4)
                                             : (NB == 1 ? 3 : 2);
   static constexpr int kStages = 2;
   static constexpr int kQBytes = kQShared ? DP / 16 * NB * PARTS * 32 * 8 : 0;
@@ -286,45 +286,50 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
     const int tb = max(w.t0 + (int)(at - u0), lo_tok / kTile);
     const int te = min(w.t0 + (int)(stop - u0), (hi_tok + kTile - 1) / kTile);
 
-    // The first warp issues tile t into a stage: lane p one copy for page p of
-    // the tile.
+    // Page numbers and scales of 32 pages at a time, a page for each lane: the
+    // list in use and the one after it, loaded a list ahead, so that no tile
+    // waits for the page table.  -1: past the visible tokens; -2: unreadable
+    // (its scales are NaN).
     const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
-    const int tile_pages = kTile / blk;
-    auto issue = [&](int t, int stage) {
-      int32_t page = -1;
-      if (lane < tile_pages && t * kTile + lane * blk < hi_tok) {
-        page = __ldg(table + t * tile_pages + lane);
-        if (page < 0 || (int64_t)page >= a.c.P) {
+    const int tile_pages = kTile / blk, page0 = tb * tile_pages, page_end = (hi_tok + blk - 1) / blk;
+    auto list_pages = [&](int first) -> int32_t {
+      const int i = first + lane;
+      return i < page_end ? __ldg(table + i) : -1;
+    };
+    auto list_scales = [&](int first, int32_t& pg, float& ks, float& vs) {
+      ks = vs = 0.f;
+      if (first + lane < page_end) {
+        if (pg < 0 || (int64_t)pg >= a.c.P) {
           kv::flag(a.c.status, NOOR_KV_BAD_PAGE);
-          page = -1;
+          pg = -2;
+          ks = vs = nan;
+        } else {
+          const int64_t ph = (int64_t)pg * a.c.H + h;
+          ks = __ldg(a.c.ks + ph);
+          vs = __ldg(a.c.vs + ph);
         }
       }
+    };
+    int32_t pg = list_pages(page0), pg_next = list_pages(page0 + 32);
+    float pks, pvs, pks_next = 0.f, pvs_next = 0.f;
+    list_scales(page0, pg, pks, pvs);
+    // The first warp issues tile t into a stage: lane p one copy for page p of
+    // the tile, at place `at` of the list.
+    auto issue = [&](int32_t list, int at, int stage) {
+      const int32_t page = __shfl_sync(0xffffffffu, list, (at + lane) & 31);
+      const bool mine = lane < tile_pages && page >= 0;
       if (dead) return;
-      const unsigned who = __ballot_sync(0xffffffffu, page >= 0);
+      const unsigned who = __ballot_sync(0xffffffffu, mine);
       const uint32_t bytes = (uint32_t)blk * D;
       if (lane == 0) {
         tc::mbar_arrive_expect_tx(bars + stage, __popc(who) * bytes);
         tc::mbar_arrive_expect_tx(bars + NST + stage, __popc(who) * bytes);
       }
       __syncwarp();
-      if (page >= 0) {
+      if (mine) {
         const int64_t ph = ((int64_t)page * a.c.H + h) * bytes;
         bulk_load(s_k + stage * kbytes + lane * bytes, a.c.k + ph, bytes, bars + stage);
         bulk_load(s_v + stage * vbytes + lane * (bytes + 2 * blk), a.c.v + ph, bytes, bars + NST + stage);
-      }
-    };
-    // Scales of the page that holds this lane's score tokens of tile t: NaN
-    // for a page that cannot be read, 0 past the visible tokens.
-    auto scales = [&](int t, float& ks, float& vs, bool& have) {
-      const int tok = t * kTile + 32 * half + 8 * (gr >> 1);
-      ks = vs = 0.f;
-      have = false;
-      if (tok / blk * blk < hi_tok) {
-        const int32_t page = __ldg(table + tok / blk);
-        have = page >= 0 && (int64_t)page < a.c.P;
-        const int64_t ph = (int64_t)page * a.c.H + h;
-        ks = have ? __ldg(a.c.ks + ph) : nan;
-        vs = have ? __ldg(a.c.vs + ph) : nan;
       }
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -339,16 +344,11 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       dead = __any_sync(0xffffffffu, dead);
     };
 
-    float ks_s[NST], vs_s[NST];
-    bool have_s[NST];
     if (half == 0) {
 #pragma unroll
       for (int i = 0; i < NST; ++i)
-        if (tb + i < te) issue(tb + i, i);
+        if (tb + i < te) issue(pg, i * tile_pages, i);
     }
-#pragma unroll
-    for (int i = 0; i < NST; ++i)
-      if (tb + i < te) scales(tb + i, ks_s[i], vs_s[i], have_s[i]);
 
     // ---- query fragments: this lane holds row gr of each group of 8, dims
     // d0 .. d0 + 3 of step ks = 4 j + s, d0 = 16 (4 j + c) + 4 s
@@ -427,8 +427,9 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 
     for (int t = tb; t < te; ++t) {
       const int stage = (t - tb) % NST;
-      const float ks = ks_s[0], vs = vs_s[0];
-      const bool have = have_s[0];
+      const int place = (t - tb) * tile_pages & 31;  // of the tile's first page in the list
+      const int my_page = place + (32 * half + 8 * (gr >> 1)) / blk;  // of this lane's score tokens
+      const float ks = __shfl_sync(0xffffffffu, pks, my_page), vs = __shfl_sync(0xffffffffu, pvs, my_page);
       const int tok0 = t * kTile + 32 * half;
       // ---- scores of this warp's 32 tokens
       wait(bars + stage, (kphase >> stage) & 1);
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       // could not be read) are whatever the memory holds, and count as zero
       wait(bars + NST + stage, (vphase >> stage) & 1);
       vphase ^= 1u << stage;
-      const bool vhave = __shfl_sync(0xffffffffu, (int)have, 8 * qc) != 0;  // of tokens 8c .. 8c + 7
+      const bool vhave = __shfl_sync(0xffffffffu, pg, place + (32 * half + 8 * qc) / blk) >= 0;  // of tokens 8c .. 8c + 7
       const int nv = vhave ? min(max(hi_tok - (tok0 + 8 * qc), 0), 8) : 0;
       const bool clip = __any_sync(0xffffffffu, nv < 8);
       const uint32_t vm0 = nv >= 4 ? 0xFFFFFFFFu : (1u << (8 * nv)) - 1u;
@@ -577,16 +578,21 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             for (int nb = 0; nb < NB; ++nb) mma_f16(o[i][nb], a0, a1, a2, a3, pf[pt][nb][2 * y], pf[pt][nb][2 * y + 1]);
         }
       }
-#pragma unroll
-      for (int i = 0; i + 1 < NST; ++i) {
-        ks_s[i] = ks_s[i + 1];
-        vs_s[i] = vs_s[i + 1];
-        have_s[i] = have_s[i + 1];
-      }
       pair_sync(pair);  // both warps have read the stage
-      if (t + NST < te) {
-        if (half == 0) issue(t + NST, stage);
-        scales(t + NST, ks_s[NST - 1], vs_s[NST - 1], have_s[NST - 1]);
+      if (t + NST < te && half == 0) {
+        const int at = place + NST * tile_pages;
+        if (at < 32)
+          issue(pg, at, stage);
+        else
+          issue(pg_next, at - 32, stage);
+      }
+      // halfway through a list the next one's pages are there: load its scales
+      if (place == 16) list_scales(page0 + ((t - tb) * tile_pages & ~31) + 32, pg_next, pks_next, pvs_next);
+      if (place + tile_pages == 32) {  // to the next list
+        pg = pg_next;
+        pks = pks_next;
+        pvs = pvs_next;
+        pg_next = list_pages(page0 + (t + 1 - tb) * tile_pages + 32);
       }
     }
 
