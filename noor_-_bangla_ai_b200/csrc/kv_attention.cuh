@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   using T = typename std::conditional<PARTS == 1, bf16, float>::type;
   constexpr int NST = Sh::kStages, R = Sh::kRows;
   extern __shared__ __align__(128) uint8_t s_attn[];
-  const int D = a.c.D, blk = a.c.blk;
+  const int D = a.c.D, blk = a.c.blk, lblk = 31 - __clz(blk);  // (16, 32 or 64)
   const int pair = threadIdx.x >> 6, half = (threadIdx.x >> 5) & 1, lane = threadIdx.x & 31, gr = lane >> 2, qc = lane & 3;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_attn) + pair * 2 * NST;  // k barriers, then v
   uint8_t* mine = s_attn + Sh::kBarBytes + pair * Sh::pair_bytes(D);
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
     // waits for the page table.  -1: past the visible tokens; -2: unreadable
     // (its scales are NaN).
     const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
-    const int tile_pages = kTile / blk, page0 = tb * tile_pages, page_end = (hi_tok + blk - 1) / blk;
+    const int tile_pages = kTile >> lblk, page0 = tb * tile_pages, page_end = (hi_tok + blk - 1) >> lblk;
     auto list_pages = [&](int first) -> int32_t {
       const int i = first + lane;
       return i < page_end ? __ldg(table + i) : -1;
@@ -425,11 +425,17 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       }
     float vref = 1.17549435e-38f;
 
-    for (int t = tb; t < te; ++t) {
-      const int stage = (t - tb) % NST;
-      const int place = (t - tb) * tile_pages & 31;  // of the tile's first page in the list
-      const int my_page = place + (32 * half + 8 * (gr >> 1)) / blk;  // of this lane's score tokens
-      const float ks = __shfl_sync(0xffffffffu, pks, my_page), vs = __shfl_sync(0xffffffffu, pvs, my_page);
+    // Fixed parts of this lane's addresses: its score tokens' page and rows, its
+    // value tokens' page and bytes.
+    const int k_page = (32 * half + 8 * (gr >> 1)) >> lblk, v_page = (32 * half + 8 * qc) >> lblk;
+    const uint8_t* k_lane = s_k + (32 * half + my_tok) * D + 16 * qc;
+    const uint8_t* v_lane = s_v + v_page * (blk * D + 2 * blk) + gr * blk + ((32 * half + 8 * qc) & (blk - 1));
+    bool list_bad = __any_sync(0xffffffffu, pg == -2);
+    // One tile, compiled apart for tiles that every row sees whole and whose
+    // pages can be read: those need no mask.
+    auto tile = [&](auto all, int t, int stage, int place) {
+      constexpr bool whole = decltype(all)::value;
+      const float ks = __shfl_sync(0xffffffffu, pks, place + k_page), vs = __shfl_sync(0xffffffffu, pvs, place + k_page);
       const int tok0 = t * kTile + 32 * half;
       // ---- scores of this warp's 32 tokens
       wait(bars + stage, (kphase >> stage) & 1);
@@ -441,7 +447,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int x = 0; x < 4; ++x) sc[i][nb][x] = 0.f;
-      const uint8_t* kt = s_k + stage * kbytes + (32 * half + my_tok) * D + 16 * qc;
+      const uint8_t* kt = k_lane + stage * kbytes;
 #pragma unroll
       for (int j = 0; j < DP / 64; ++j) {
         if (64 * j >= D) break;
@@ -478,7 +484,6 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         }
       }
       // ---- scale, mask, running maximum
-      const bool whole = tok0 + 31 <= p_first && (a.window <= 0 || p_last - tok0 <= a.window);
       float alpha[NB][2], mref[NB][2];
       const float vmax = fmaxf(fabsf(vs), __shfl_xor_sync(0xffffffffu, fabsf(vs), 16));
       const float vnew = fmaxf(vref, vmax);
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float v = sc[i][nb][x] * ((x & 1) ? f1 : f0);
-            if (!whole) {
+            if constexpr (!whole) {
               const int tok = tok0 + my_tok + 2 * (2 * i + (x >> 1)), p = qpos[nb][x & 1];
               if (tok > p || (a.window > 0 && p - tok > a.window)) v = -INFINITY;
             }
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             const float p = exp2_approx(sc[i][nb][x] - mref[nb][x & 1]);
             sum[x & 1] += p;
             // a masked token's p is zero whatever its block's scale
-            sc[i][nb][x] = sc[i][nb][x] == -INFINITY ? 0.f : p * vrel;
+            sc[i][nb][x] = !whole && sc[i][nb][x] == -INFINITY ? 0.f : p * vrel;
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -552,19 +557,20 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       // could not be read) are whatever the memory holds, and count as zero
       wait(bars + NST + stage, (vphase >> stage) & 1);
       vphase ^= 1u << stage;
-      const bool vhave = __shfl_sync(0xffffffffu, pg, place + (32 * half + 8 * qc) / blk) >= 0;  // of tokens 8c .. 8c + 7
-      const int nv = vhave ? min(max(hi_tok - (tok0 + 8 * qc), 0), 8) : 0;
-      const bool clip = __any_sync(0xffffffffu, nv < 8);
-      const uint32_t vm0 = nv >= 4 ? 0xFFFFFFFFu : (1u << (8 * nv)) - 1u;
-      const uint32_t vm1 = nv >= 8 ? 0xFFFFFFFFu : nv <= 4 ? 0u : (1u << (8 * (nv - 4))) - 1u;
-      const int vtok = 32 * half + 8 * qc;
-      const uint8_t* vt = s_v + stage * vbytes + (vtok / blk) * (blk * D + 2 * blk) + gr * blk + vtok % blk;
+      uint32_t vm0 = 0xFFFFFFFFu, vm1 = 0xFFFFFFFFu;
+      if constexpr (!whole) {
+        const bool vhave = __shfl_sync(0xffffffffu, pg, place + v_page) >= 0;  // of tokens 8c .. 8c + 7
+        const int nv = vhave ? min(max(hi_tok - (tok0 + 8 * qc), 0), 8) : 0;
+        vm0 = nv >= 4 ? 0xFFFFFFFFu : (1u << (8 * nv)) - 1u;
+        vm1 = nv >= 8 ? 0xFFFFFFFFu : nv <= 4 ? 0u : (1u << (8 * (nv - 4))) - 1u;
+      }
+      const uint8_t* vt = v_lane + stage * vbytes;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         if (16 * i >= D) break;
         uint2 v0 = *reinterpret_cast<const uint2*>(vt + 16 * i * blk);
         uint2 v1 = *reinterpret_cast<const uint2*>(vt + (16 * i + 8) * blk);
-        if (clip) {
+        if constexpr (!whole) {
           v0.x &= vm0; v0.y &= vm1; v1.x &= vm0; v1.y &= vm1;
         }
 #pragma unroll
@@ -578,6 +584,14 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             for (int nb = 0; nb < NB; ++nb) mma_f16(o[i][nb], a0, a1, a2, a3, pf[pt][nb][2 * y], pf[pt][nb][2 * y + 1]);
         }
       }
+    };
+    for (int t = tb; t < te; ++t) {
+      const int stage = (t - tb) % NST, place = (t - tb) * tile_pages & 31;  // of the tile's first page in the list
+      const int tok0 = t * kTile + 32 * half;
+      if (tok0 + 31 <= p_first && (a.window <= 0 || p_last - tok0 <= a.window) && !list_bad)
+        tile(std::true_type{}, t, stage, place);
+      else
+        tile(std::false_type{}, t, stage, place);
       pair_sync(pair);  // both warps have read the stage
       if (t + NST < te && half == 0) {
         const int at = place + NST * tile_pages;
@@ -592,6 +606,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         pg = pg_next;
         pks = pks_next;
         pvs = pvs_next;
+        list_bad = __any_sync(0xffffffffu, pg == -2);
         pg_next = list_pages(page0 + (t + 1 - tb) * tile_pages + 32);
       }
     }
