@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -29,6 +30,13 @@ STATUS = {1: "row offsets are not ascending within the rows given",
           4: "a bounded wait on the device gave up"}
 
 
+# A decode step's calls cost more on the host than on the GPU, so arguments are
+# packed as the C structures' bytes (noor_heads, noor_kv_batch) and each tensor
+# is asked for its shape and strides once.
+_HEADS = struct.Struct("Pqq")
+_BATCH = struct.Struct("PqPPqii")
+
+
 def _torch():
     import torch
     return torch
@@ -41,38 +49,39 @@ def _code_dtype(fmt: str):
 
 def _dtype_code(t) -> int:
     torch = _torch()
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return api.DTYPE_BF16
-    if t.dtype == torch.float32:
+    if t.dtype is torch.float32:
         return api.DTYPE_F32
     raise ValueError(f"expected bfloat16 or float32, got {t.dtype}")
 
 
-def _heads(t, what: str, dim: Optional[int] = None) -> api.Heads:
-    """noor_heads of a CUDA tensor [tokens, heads, head_dim]."""
-    if t.dim() != 3 or not t.is_cuda:
-        raise ValueError(f"{what} must be a CUDA tensor [tokens, heads, head_dim], got {tuple(t.shape)} on {t.device}")
-    if dim is not None and t.shape[2] != dim:
-        raise ValueError(f"{what} has head_dim {t.shape[2]}, expected {dim}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+def _heads(t, what: str, device: int, dim: int) -> bytes:
+    """noor_heads of a tensor [tokens, heads, dim] on CUDA device `device`."""
+    st = t.stride()
+    if len(st) != 3 or t.get_device() != device:
+        raise ValueError(f"{what} must be a tensor [tokens, heads, head_dim] on cuda:{device}, got {tuple(t.shape)} on "
+                         f"{t.device}")
+    if t.size(2) != dim:
+        raise ValueError(f"{what} has head_dim {t.size(2)}, expected {dim}")
+    if st[2] != 1 and dim > 1:
         raise ValueError(f"{what}: a head's elements must be contiguous")
-    return api.Heads(t.data_ptr(), t.stride(0), t.stride(1))
+    return _HEADS.pack(t.data_ptr(), st[0], st[1])
 
 
-def _int32(t, what: str, shape: Sequence[Optional[int]], device) -> int:
-    """Data pointer of an int32 tensor on `device`, its shape checked."""
-    torch = _torch()
-    if t.dtype != torch.int32 or t.device != device:
-        raise ValueError(f"{what} must be an int32 tensor on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.numel() > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what} must be contiguous along its last dimension")
+def _ints(t, what: str, n: int, device: int) -> int:
+    """Data pointer of a contiguous int32 tensor [n] on `device`."""
+    if t.dtype is not _torch().int32 or t.get_device() != device:
+        raise ValueError(f"{what} must be an int32 tensor on cuda:{device}, got {t.dtype} on {t.device}")
+    if t.dim() != 1 or t.size(0) != n:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({n},)")
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{what} must be contiguous")
     return t.data_ptr()
 
 
-def _stream(device) -> int:
-    return _torch()._C._cuda_getCurrentRawStream(device.index)
+def _stream(device: int) -> int:
+    return _torch()._C._cuda_getCurrentRawStream(device)
 
 
 # ------------------------------------------------------------ rotary
@@ -134,7 +143,9 @@ class Rotary:
         self.inv_freq = inv_freq.contiguous()
         self.rotate_dim = 2 * inv_freq.numel()
         self.layout, self.factor = layout, float(factor)
+        self.device = self.inv_freq.get_device()
         self.desc = api.RotaryDesc(self.inv_freq.data_ptr(), self.rotate_dim, LAYOUTS[layout], self.factor)
+        self.ref = ctypes.byref(self.desc)
 
     @classmethod
     def create(cls, head_dim: int, theta: float = 10000.0, fraction: Optional[float] = None,
@@ -146,23 +157,28 @@ class Rotary:
 def _rope_call(q, k, positions, rotary: Rotary, inverse: bool):
     torch = _torch()
     dt = _dtype_code(q)
-    D = q.shape[-1]
-    hq = _heads(q, "q")
-    if rotary.inv_freq.device != q.device:
-        raise ValueError(f"the rotary table is on {rotary.inv_freq.device}, q on {q.device}")
-    pos = _int32(positions, "positions", (q.shape[0],), q.device)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.dim() != 3 or not q.is_cuda:
+        raise ValueError(f"q must be a CUDA tensor [tokens, heads, head_dim], got {tuple(q.shape)} on {q.device}")
+    T, nq, D = q.shape
+    dev = q.get_device()
+    hq = _heads(q, "q", dev, D)
+    if rotary.device != dev:
+        raise ValueError(f"the rotary table is on cuda:{rotary.device}, q on cuda:{dev}")
+    pos = _ints(positions, "positions", T, dev)
+    q_out = torch.empty((T, nq, D), dtype=q.dtype, device=q.device)
     k_out = hk = hk_out = None
+    nk = 0
     if k is not None:
-        if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0]:
-            raise ValueError("k must have q's tokens, type and device")
-        hk = _heads(k, "k", D)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        hk_out = ctypes.byref(_heads(k_out, "k"))
-    api.check(api.lib().noor_rope_apply(
-        ctypes.byref(rotary.desc), ctypes.byref(hq), ctypes.byref(_heads(q_out, "q")), q.shape[1],
-        ctypes.byref(hk) if hk is not None else None, hk_out, k.shape[1] if k is not None else 0, pos, q.shape[0], D,
-        dt, int(inverse), q.device.index, _stream(q.device)))
+        hk = _heads(k, "k", dev, D)
+        nk = k.size(1)
+        if k.dtype is not q.dtype or k.size(0) != T:
+            raise ValueError("k must have q's tokens and type")
+        k_out = torch.empty((T, nk, D), dtype=q.dtype, device=q.device)
+        hk_out = _HEADS.pack(k_out.data_ptr(), nk * D, D)
+    rc = api.lib().noor_rope_apply(rotary.ref, hq, _HEADS.pack(q_out.data_ptr(), nq * D, D), nq, hk, hk_out, nk, pos, T, D,
+                                   dt, inverse, dev, _stream(dev))
+    if rc:
+        api.check(rc)
     return q_out, k_out
 
 
@@ -177,28 +193,35 @@ def _rope_autograd():
 
         class RopeFunction(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, q, k, positions, rotary):
-                ctx.rotary = rotary
+            def forward(ctx, q, k, positions, rotary, inverse):
+                ctx.args = (rotary, inverse)
                 ctx.set_materialize_grads(False)
                 ctx.save_for_backward(positions)
-                q_out, k_out = _rope_call(q, k, positions, rotary, False)
+                q_out, k_out = _rope_call(q, k, positions, rotary, inverse)
                 return q_out if k is None else (q_out, k_out)
 
             @staticmethod
-            @torch.autograd.function.once_differentiable
             def backward(ctx, gq, gk=None):
-                # the rotation's transpose; gradients may come broadcast
+                # The transpose: the rotation the other way, itself differentiable.
+                # Gradients may come broadcast, or not at all.
+                rotary, inverse = ctx.args
                 (positions,) = ctx.saved_tensors
-                gs = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (gq, gk)]
-                need = [g is not None and n for g, n in zip(gs, ctx.needs_input_grad)]
-                dq = dk = None
-                if need[0] and need[1]:
-                    dq, dk = _rope_call(gs[0], gs[1], positions, ctx.rotary, True)
-                elif need[0]:
-                    dq, _ = _rope_call(gs[0], None, positions, ctx.rotary, True)
-                elif need[1]:
-                    dk, _ = _rope_call(gs[1], None, positions, ctx.rotary, True)
-                return dq, dk, None, None
+                need = ctx.needs_input_grad
+                gq = gq if need[0] else None
+                gk = gk if need[1] else None
+                if gq is not None and gq.stride(-1) != 1:
+                    gq = gq.contiguous()
+                if gk is not None and gk.stride(-1) != 1:
+                    gk = gk.contiguous()
+                if gq is None and gk is None:
+                    return None, None, None, None, None
+                first, second = (gq, gk) if gq is not None else (gk, None)
+                if torch.is_grad_enabled():
+                    out = RopeFunction.apply(first, second, positions, rotary, not inverse)
+                    d0, d1 = out if second is not None else (out, None)
+                else:
+                    d0, d1 = _rope_call(first, second, positions, rotary, not inverse)
+                return (d0, d1, None, None, None) if gq is not None else (None, d0, None, None, None)
 
         _rope_function = RopeFunction
     return _rope_function
@@ -210,7 +233,7 @@ def rope_apply(q, positions, rotary: Rotary, k=None):
     q', or (q', k')."""
     torch = _torch()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _rope_autograd().apply(q, k, positions, rotary)
+        return _rope_autograd().apply(q, k, positions, rotary, False)
     q_out, k_out = _rope_call(q, k, positions, rotary, False)
     return q_out if k is None else (q_out, k_out)
 
@@ -269,8 +292,11 @@ class KVCache:
         self.num_blocks, self.n_kv_heads, self.block, self.head_dim = P, H, blk, D
         self.format, self.device = fmt, k_codes.device
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._dev = k_codes.get_device()
         self.desc = api.KVCacheDesc(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                    self.status.data_ptr(), P, H, D, blk, FORMATS[fmt], self.device.index)
+                                    self.status.data_ptr(), P, H, D, blk, FORMATS[fmt], self._dev)
+        self._ref = ctypes.byref(self.desc)
+        self._workspace = {}  # bytes of attention's workspace by its sizes
 
     def check(self) -> None:
         """Wait for the device and raise NoorMoEError if a kernel found a
@@ -280,19 +306,18 @@ class KVCache:
             self.status.zero_()
             raise api.NoorMoEError(6 if code == 4 else 1, f"cache: {STATUS.get(code, code)}")
 
-    def _batch(self, block_table, kv_lens, cu_rows, rows: int) -> api.KVBatch:
-        table = _int32(block_table, "block_table", (None, None), self.device)
-        B = block_table.shape[0]
-        lens = _int32(kv_lens, "kv_lens", (B,), self.device) if kv_lens is not None else None
-        cu = _int32(cu_rows, "cu_rows", (B + 1,), self.device)
-        return api.KVBatch(table, block_table.stride(0), lens, cu, rows, B, block_table.shape[1])
-
-    def _rows(self, t, what: str, like=None) -> api.Heads:
-        if t.device != self.device:
-            raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
-        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
-            raise ValueError(f"{what} must have the other rows' number and type")
-        return _heads(t, what, self.head_dim)
+    def _batch(self, block_table, kv_lens, cu_rows, rows: int) -> bytes:
+        """noor_kv_batch."""
+        if block_table.dim() != 2 or block_table.dtype is not _torch().int32 or block_table.get_device() != self._dev:
+            raise ValueError(f"block_table must be an int32 tensor [batch, max_blocks] on cuda:{self._dev}, got "
+                             f"{block_table.dtype} {tuple(block_table.shape)} on {block_table.device}")
+        B, maxb = block_table.shape
+        ts = block_table.stride()
+        if ts[1] != 1 and maxb > 1:
+            raise ValueError("block_table's rows must be contiguous")
+        return _BATCH.pack(block_table.data_ptr(), ts[0],
+                           0 if kv_lens is None else _ints(kv_lens, "kv_lens", B, self._dev),
+                           _ints(cu_rows, "cu_rows", B + 1, self._dev), rows, B, maxb)
 
     def append(self, k, v, block_table, kv_lens, cu_rows, rotary: Optional[Rotary] = None, q=None):
         """Write the new tokens' k and v [rows, kv heads, head_dim]; row i of
@@ -302,23 +327,32 @@ class KVCache:
         undefined), else None."""
         torch = _torch()
         dt = _dtype_code(k)
-        hk, hv = self._rows(k, "k"), self._rows(v, "v", k)
-        if k.shape[1] != self.n_kv_heads or v.shape[1] != self.n_kv_heads:
+        dev, D = self._dev, self.head_dim
+        hk, hv = _heads(k, "k", dev, D), _heads(v, "v", dev, D)
+        rows = k.size(0)
+        if k.size(1) != self.n_kv_heads or v.size(1) != self.n_kv_heads:
             raise ValueError(f"k and v must have {self.n_kv_heads} heads")
-        if q is not None and rotary is None:
-            raise ValueError("q is rotated beside the write: it needs `rotary`")
-        if rotary is not None and rotary.inv_freq.device != self.device:
-            raise ValueError(f"the rotary table is on {rotary.inv_freq.device}, the cache on {self.device}")
-        batch = self._batch(block_table, kv_lens, cu_rows, k.shape[0])
-        q_out = hq = hq_out = None
+        if v.size(0) != rows or v.dtype is not k.dtype:
+            raise ValueError("v must have k's rows and type")
+        batch = self._batch(block_table, kv_lens, cu_rows, rows)
+        rot = q_out = hq = hq_out = None
+        nq = 0
+        if rotary is not None:
+            if rotary.device != dev:
+                raise ValueError(f"the rotary table is on cuda:{rotary.device}, the cache on cuda:{dev}")
+            rot = rotary.ref
         if q is not None:
-            hq = ctypes.byref(self._rows(q, "q", k))
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            hq_out = ctypes.byref(_heads(q_out, "q"))
-        api.check(api.lib().noor_kv_append(
-            ctypes.byref(self.desc), ctypes.byref(batch), ctypes.byref(hk), ctypes.byref(hv),
-            ctypes.byref(rotary.desc) if rotary is not None else None, hq, hq_out, q.shape[1] if q is not None else 0,
-            dt, _stream(self.device)))
+            if rotary is None:
+                raise ValueError("q is rotated beside the write: it needs `rotary`")
+            hq = _heads(q, "q", dev, D)
+            nq = q.size(1)
+            if q.size(0) != rows or q.dtype is not k.dtype:
+                raise ValueError("q must have k's rows and type")
+            q_out = torch.empty((rows, nq, D), dtype=q.dtype, device=q.device)
+            hq_out = _HEADS.pack(q_out.data_ptr(), nq * D, D)
+        rc = api.lib().noor_kv_append(self._ref, batch, hk, hv, rot, hq, hq_out, nq, dt, _stream(dev))
+        if rc:
+            api.check(rc)
         return q_out
 
     def read(self, block_table, starts, cu_rows, rows: int, dtype=None, kv_lens=None):
@@ -327,14 +361,16 @@ class KVCache:
         kv_lens bounds the tokens (None: the tables' whole width).  Returns k, v
         [rows, kv heads, head_dim] in `dtype` (bfloat16 by default)."""
         torch = _torch()
-        dtype = torch.bfloat16 if dtype is None else dtype
-        out = [torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
-        dt = _dtype_code(out[0])
         batch = self._batch(block_table, kv_lens, cu_rows, rows)
-        st = _int32(starts, "starts", (batch.batch,), self.device) if starts is not None else None
-        api.check(api.lib().noor_kv_read(ctypes.byref(self.desc), ctypes.byref(batch), st, out[0].data_ptr(),
-                                         out[1].data_ptr(), dt, _stream(self.device)))
-        return out[0], out[1]
+        st = None if starts is None else _ints(starts, "starts", block_table.size(0), self._dev)
+        shape = (rows, self.n_kv_heads, self.head_dim)
+        dtype = torch.bfloat16 if dtype is None else dtype
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty(shape, dtype=dtype, device=self.device)
+        rc = api.lib().noor_kv_read(self._ref, batch, st, k.data_ptr(), v.data_ptr(), _dtype_code(k), _stream(self._dev))
+        if rc:
+            api.check(rc)
+        return k, v
 
     def attention(self, q, block_table, kv_lens, cu_rows, max_rows: int, scale: Optional[float] = None,
                   window: int = 0, out=None, return_lse: bool = False):
@@ -345,22 +381,30 @@ class KVCache:
         (out, lse) with lse [rows, heads] f32.  `out` may be q."""
         torch = _torch()
         dt = _dtype_code(q)
-        hq = self._rows(q, "q")
-        if q.shape[1] % self.n_kv_heads != 0:
-            raise ValueError(f"{q.shape[1]} query heads over {self.n_kv_heads} kv heads")
-        batch = self._batch(block_table, kv_lens, cu_rows, q.shape[0])
+        dev, D = self._dev, self.head_dim
+        hq = _heads(q, "q", dev, D)
+        rows, nq = q.size(0), q.size(1)
+        if nq % self.n_kv_heads != 0:
+            raise ValueError(f"{nq} query heads over {self.n_kv_heads} kv heads")
+        batch = self._batch(block_table, kv_lens, cu_rows, rows)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-        ho = self._rows(out, "out", q)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-        need = ctypes.c_int64()
-        args = (ctypes.byref(self.desc), ctypes.byref(batch))
-        api.check(api.lib().noor_kv_attention_workspace(*args, q.shape[1], max_rows, dt, ctypes.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        api.check(api.lib().noor_kv_attention(
-            *args, ctypes.byref(hq), ctypes.byref(ho), lse.data_ptr() if lse is not None else None, q.shape[1], max_rows,
-            float(self.head_dim) ** -0.5 if scale is None else float(scale), window, dt, ws.data_ptr(), need.value,
-            _stream(self.device)))
+            out = torch.empty((rows, nq, D), dtype=q.dtype, device=q.device)
+            ho = _HEADS.pack(out.data_ptr(), nq * D, D)
+        else:
+            if out.shape != q.shape or out.dtype is not q.dtype:
+                raise ValueError("out must have q's shape and type")
+            ho = _heads(out, "out", dev, D)
+        lse = torch.empty((rows, nq), dtype=torch.float32, device=q.device) if return_lse else None
+        lib = api.lib()
+        key = (rows, nq, max_rows, dt, *block_table.shape)
+        need = self._workspace.get(key)
+        if need is None:
+            n = ctypes.c_int64()
+            api.check(lib.noor_kv_attention_workspace(self._ref, batch, nq, max_rows, dt, ctypes.byref(n)))
+            need = self._workspace[key] = n.value
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        rc = lib.noor_kv_attention(self._ref, batch, hq, ho, lse.data_ptr() if return_lse else None, nq, max_rows,
+                                   D ** -0.5 if scale is None else scale, window, dt, ws.data_ptr(), need, _stream(dev))
+        if rc:
+            api.check(rc)
         return (out, lse) if return_lse else out
