@@ -105,7 +105,6 @@ int by_dtype(int dtype, F&& f) {
 
 int check_cache(const noor_kv_cache* c) {
   if (!c) return fail(NOOR_MOE_ERR_INVALID, "null cache");
-  CKR(check_device(c->device));
   if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale) return fail(NOOR_MOE_ERR_INVALID, "null cache array");
   for (const void* p : {(const void*)c->k_codes, (const void*)c->v_codes, (const void*)c->k_scale, (const void*)c->v_scale})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return fail(NOOR_MOE_ERR_INVALID, "cache arrays must be 16-byte aligned");
@@ -117,6 +116,7 @@ int check_cache(const noor_kv_cache* c) {
     return fail(NOOR_MOE_ERR_INVALID, "unknown cache format %d", c->format);
   if (c->num_blocks <= 0 || c->num_blocks > INT32_MAX || c->n_kv_heads <= 0 || c->n_kv_heads > 4096)
     return fail(NOOR_MOE_ERR_INVALID, "num_blocks or n_kv_heads out of range");
+  if (c->device < 0) return fail(NOOR_MOE_ERR_INVALID, "device %d", c->device);
   return NOOR_MOE_OK;
 }
 
@@ -228,6 +228,7 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
       CKR(check_view(q_out, dtype, "q_out"));
       if (q_heads <= 0 || q_heads > 4096) return fail(NOOR_MOE_ERR_INVALID, "q_heads %d out of range", q_heads);
     }
+    CKR(check_device(c->device));
     DeviceGuard g(c->device);
     kv::AppendArgs a{};
     a.c = cache_of(c);
@@ -303,6 +304,7 @@ int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* 
     if (!k_out || !v_out) return fail(NOOR_MOE_ERR_INVALID, "null output");
     if (reinterpret_cast<uintptr_t>(k_out) % 16 != 0 || reinterpret_cast<uintptr_t>(v_out) % 16 != 0)
       return fail(NOOR_MOE_ERR_INVALID, "outputs must be 16-byte aligned");
+    CKR(check_device(c->device));
     DeviceGuard g(c->device);
     kv::ReadArgs a{cache_of(c), batch_of(b), starts, k_out, v_out, 1};
     const int64_t tasks = most_tasks(c, b);
@@ -406,13 +408,14 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     if (b->n_rows == 0) return NOOR_MOE_OK;
     CKR(check_view(q, dtype, "q"));
     CKR(check_view(out, dtype, "out"));
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+      return fail(NOOR_MOE_ERR_INVALID, "workspace is null or not 16-byte aligned");
     StreamPlan p;
     CKR(stream_plan(c, b, q_heads, max_rows, dtype, &p));
-    if (!workspace || workspace_bytes < p.bytes)
+    if (workspace_bytes < p.bytes)
       return fail(NOOR_MOE_ERR_INVALID, "workspace of %lld bytes, needs %lld", (long long)workspace_bytes,
                   (long long)p.bytes);
-    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
-      return fail(NOOR_MOE_ERR_INVALID, "workspace must be 16-byte aligned");
+    CKR(check_device(c->device));
     DeviceGuard g(c->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     attn::Args a{};

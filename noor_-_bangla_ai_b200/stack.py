@@ -10,6 +10,11 @@ and RoPE::apply (rope.rs:49-90) but is not a B200 kernel of this library.  The
 FFN sublayer of every block -- sandwich norm, router, experts, dense branch,
 combine, residual -- is one call of the library's noor_moe_ffn_sublayer_forward.
 
+Serving is on the library's kernels on both sides: forward_cached (prompts,
+then a few tokens at a time) rotates and writes keys and values into a paged
+8-bit cache and attends over it (attention.py); only the projections are torch
+matmuls.
+
 Tensors live on one CUDA device; BF16 layers keep the residual stream in
 bfloat16 between sublayers, F32 layers in float32.
 """
@@ -21,6 +26,7 @@ from typing import List, Optional, Sequence, Tuple
 import numpy as np
 
 from . import api
+from . import attention as _attn
 
 
 def rope_inv_freq(head_dim: int, theta: float, fraction: Optional[float] = None) -> Tuple[np.ndarray, int]:
@@ -42,6 +48,13 @@ class RoPE:
     def __init__(self, head_dim: int, theta: float, fraction: Optional[float] = None):
         self.inv_freq, self.rotate_dim = rope_inv_freq(head_dim, theta, fraction)
         self.head_dim = head_dim
+        self._rotary = {}
+
+    def rotary(self, device: int = 0) -> "_attn.Rotary":
+        """The same rotation as a device table for attention.py's calls."""
+        if device not in self._rotary:
+            self._rotary[device] = _attn.Rotary(self.inv_freq, "interleaved", device=device)
+        return self._rotary[device]
 
     def apply(self, x, seq_offset: int = 0):
         """x: torch tensor (..., seq, head_dim); the rotation is computed in f32."""
@@ -119,8 +132,74 @@ class GQAAttention:
         out = o.transpose(0, 1).reshape(S, nh * hd) @ self._w("wo", dev, dt)
         return out.to(out_dtype), max_logit
 
+    def forward_cached(self, x, rope: RoPE, cache: "_attn.KVCache", rows: "CacheRows"):
+        """x: (rows, d_model) new tokens of the batch's sequences.  Rotates q and
+        k to their positions, writes k and v into the cache and attends over it
+        (attention.rs:67-191 with its KV cache).  Queries, keys and values are
+        in x's dtype, the projections in f32."""
+        import torch
+        nh, nkv, hd = self.n_heads, self.n_kv_heads, self.head_dim
+        dt, dev = torch.float32, x.device
+        xf = x.float()
+        q, k, v = ((xf @ self._w(n, dev, dt)).to(x.dtype).view(-1, h, hd) for n, h in (("wq", nh), ("wk", nkv), ("wv", nkv)))
+        q = cache.append(k, v, rows.block_table, rows.kv_lens, rows.cu_rows, rotary=rope.rotary(dev.index), q=q)
+        o = cache.attention(q, rows.block_table, rows.kv_lens, rows.cu_rows, rows.max_rows,
+                            scale=float(np.float32(1.0) / np.sqrt(np.float32(hd))), window=self.sliding_window, out=q)
+        return (o.reshape(-1, nh * hd).float() @ self._w("wo", dev, dt)).to(x.dtype)
+
     def param_count(self) -> int:
         return self.wq.size + self.wk.size + self.wv.size + self.wo.size
+
+
+class CacheRows:
+    """The new tokens of one step over a batch of sequences (device metadata of
+    noor_kv_batch)."""
+
+    def __init__(self, block_table, lens: Sequence[int], news: Sequence[int]):
+        import torch
+        dev = block_table.device
+        self.block_table = block_table
+        self.kv_lens = torch.tensor(list(lens), dtype=torch.int32, device=dev)
+        self.cu_rows = torch.tensor([0] + list(np.cumsum(news)), dtype=torch.int32, device=dev)
+        self.max_rows = max(news)
+
+
+class StackCache:
+    """The caches of a NoorStack's layers for a batch of sequences of up to
+    max_tokens each: one paged 8-bit cache for every layer, the same pages of
+    each for a sequence."""
+
+    def __init__(self, stack: "NoorStack", batch: int, max_tokens: int, block: int = 64, fmt: str = "int8"):
+        import torch
+        if batch <= 0 or max_tokens <= 0:
+            raise ValueError("batch and max_tokens must be positive")
+        per = (max_tokens + block - 1) // block
+        att = stack.blocks[0].attention
+        self.layers = [_attn.KVCache(batch * per, att.n_kv_heads, att.head_dim, block, fmt, stack.device)
+                       for _ in stack.blocks]
+        self.block_table = torch.arange(batch * per, dtype=torch.int32,
+                                        device=torch.device("cuda", stack.device)).view(batch, per)
+        self.lens = [0] * batch
+        self.max_tokens = max_tokens
+
+    def step(self, news: Sequence[int]) -> CacheRows:
+        """Make room for news[b] more tokens of each sequence."""
+        if len(news) != len(self.lens) or min(news) < 0 or max(news) == 0:
+            raise ValueError(f"expected {len(self.lens)} token counts, at least one above 0, got {list(news)}")
+        lens = [o + n for o, n in zip(self.lens, news)]
+        if max(lens) > self.max_tokens:
+            raise ValueError(f"a sequence would hold {max(lens)} tokens, the cache {self.max_tokens}")
+        self.lens = lens
+        return CacheRows(self.block_table, lens, news)
+
+    def reset(self, sequence: int) -> None:
+        """Start sequence `sequence` over (its pages are written afresh)."""
+        self.lens[sequence] = 0
+
+    def check(self) -> None:
+        """Raise if a kernel found a mistake in device metadata."""
+        for c in self.layers:
+            c.check()
 
 
 def _rms_norm_torch(x, w, eps: float, depth_scale: float):
@@ -153,12 +232,24 @@ class MoEBlock:
     def forward(self, x, rope: RoPE, want_max_logit: bool = True):
         """x: (seq, d_model) torch tensor on the layer's device.  Returns
         (hidden, max_attn_logit)."""
-        import torch
         an = self.attn_norm
         normed = _rms_norm_torch(x, self._norm_w(an.pre_norm, x), an.pre_norm.eps, float(an.depth_scale))
         attn_out, max_logit = self.attention.forward(normed, rope, want_max_logit)
         attn_out = _rms_norm_torch(attn_out, self._norm_w(an.post_norm, x), an.post_norm.eps, float(an.depth_scale))
         h = (x.float() + attn_out.float()).to(x.dtype)  # tensor::add, in f32
+        return self._ffn_sublayer(h), max_logit
+
+    def forward_cached(self, x, rope: RoPE, cache: "_attn.KVCache", rows: CacheRows):
+        """The block over new tokens x (rows, d_model) with its cache."""
+        an = self.attn_norm
+        normed = _rms_norm_torch(x, self._norm_w(an.pre_norm, x), an.pre_norm.eps, float(an.depth_scale))
+        attn_out = self.attention.forward_cached(normed, rope, cache, rows)
+        attn_out = _rms_norm_torch(attn_out, self._norm_w(an.post_norm, x), an.post_norm.eps, float(an.depth_scale))
+        return self._ffn_sublayer((x.float() + attn_out.float()).to(x.dtype))
+
+    def _ffn_sublayer(self, h):
+        """h + post(ParallelFFN(pre(h))), one library call (block.rs:87-90)."""
+        import torch
         moe = self.parallel_ffn.moe
         dev = moe._device_handle()
         fn = self.ffn_norm
@@ -171,7 +262,7 @@ class MoEBlock:
         stream = torch.cuda.current_stream(h.device).cuda_stream
         dev.ffn_sublayer_device(h.data_ptr(), out.data_ptr(), h.shape[0], stream, counts_ptr=counts.data_ptr())
         moe.utilization.record_batch(counts.cpu().numpy(), h.shape[0])
-        return out, max_logit
+        return out
 
     def _norm_w(self, norm: "api.RMSNorm", like):
         import torch
@@ -231,3 +322,29 @@ class NoorStack:
         h = _rms_norm_torch(h, w, self.final_norm.eps, 1.0)
         logits = h.float() @ torch.from_numpy(self.output_proj).to(dev)
         return logits, max_logit, util
+
+    def new_cache(self, batch: int, max_tokens: int, block: int = 64, fmt: str = "int8") -> StackCache:
+        """Caches for serving `batch` sequences of up to max_tokens tokens."""
+        return StackCache(self, batch, max_tokens, block, fmt)
+
+    def forward_cached(self, token_ids: Sequence[Sequence[int]], cache: StackCache):
+        """The next tokens of each sequence (a prompt, one token, or none), on top
+        of what the cache holds.  Returns (logits [rows, vocab] f32, per-layer
+        expert utilization fractions), rows in sequence order."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        tdt = torch.bfloat16 if self.dtype == api.DTYPE_BF16 else torch.float32
+        flat = np.concatenate([np.asarray(t, np.int64).reshape(-1) for t in token_ids])
+        if flat.size and (flat.max() >= self.embedding.shape[0] or flat.min() < 0):
+            raise ValueError("token id out of vocab range")
+        rows = cache.step([len(t) for t in token_ids])
+        h = torch.from_numpy(self.embedding[flat]).to(dev).to(tdt)
+        util = []
+        for b, layer in zip(self.blocks, cache.layers):
+            rope = self.prope if (b.is_global and self.prope is not None) else self.rope
+            h = b.forward_cached(h, rope, layer, rows)
+            util.append(b.parallel_ffn.moe.utilization.fractions())
+            b.parallel_ffn.moe.utilization.reset()
+        w = torch.from_numpy(self.final_norm.weight).to(dev)
+        h = _rms_norm_torch(h, w, self.final_norm.eps, 1.0)
+        return h.float() @ torch.from_numpy(self.output_proj).to(dev), util

@@ -92,7 +92,8 @@ class RefCache:
 
 def attend(q, k, v, pos, scale, window):
     """q [n, Hq, D] at positions pos [n] over k, v [L, Hkv, D], all f64.
-    Returns out, lse, mag (sum p |v| / sum p) and smax (largest scale |q|.|k|)."""
+    Returns out, lse, mag (sum p |v| / sum p), smax (largest scale |q|.|k|) and
+    vsum (sum |v| over the tokens that any row sees)."""
     n, Hq, D = q.shape
     L, Hkv, _ = k.shape
     g = Hq // Hkv
@@ -113,17 +114,21 @@ def attend(q, k, v, pos, scale, window):
     mag = torch.einsum("hnl,lhd->nhd", w, vz.abs())
     lse = (top.squeeze(-1) + torch.log(tot.squeeze(-1))).transpose(0, 1)
     smax = (torch.einsum("nhd,lhd->hnl", q.abs(), kk.abs()) * abs(scale)).masked_fill(hidden[None], 0).nan_to_num().amax(-1)
-    return out, lse, mag, smax.transpose(0, 1)
+    return out, lse, mag, smax.transpose(0, 1), vz.abs().sum(0)
 
 
-def attend_tolerance(dtype, out, mag, smax, D, L):
+def attend_tolerance(dtype, out, mag, smax, vsum, D, L):
     """Largest error of one output.  Its own rounding; each p off by its f16
     parts (one part 2^-11, two 2^-21), and by its score: a sum of D + 8 products
     and factors in f32, whose error (2^-23 a step, the tensor core cuts rather than
     rounds) is relative to scale |q|.|k| and doubles through the quotient; the
-    sums over L tokens."""
+    sums over L tokens.  And f16's own floor: a p below 2^-14 of its format is off by
+up to 2^-25 whatever its size, and the largest p is at least 2^7 there (2^7 in
+the many-row kernel, 2^14 in the other, where F32's second part reaches as
+far), so each token adds up to 2^-32 |v| (F32 2^-39 |v|) of the row's largest
+weight, which is at most 1."""
     bf = dtype == torch.bfloat16
     own = 2.0 ** -8 if bf else 2.0 ** -24
     p = 2.0 ** -11 if bf else 2.0 ** -21
     rel = p + 2 * (D + 8) * 2.0 ** -23 * smax[..., None] + (L + 64) * 2.0 ** -23
-    return own * out.abs() + mag * rel + 1e-30
+    return own * out.abs() + mag * rel + (2.0 ** -32 if bf else 2.0 ** -39) * vsum + 1e-30

@@ -279,9 +279,9 @@ def check_attention(pkg, c, rk, rv, tab, lens, news, Hq, dtype, window=0, seed=0
         if n == 0:
             continue
         pos = torch.arange(L - n, L)
-        o, ls, mag, smax = ref.attend(q[row:row + n].double(), rk.tokens(tab[b], L), rv.tokens(tab[b], L), pos, sc, window)
+        o, ls, mag, smax, vsum = ref.attend(q[row:row + n].double(), rk.tokens(tab[b], L), rv.tokens(tab[b], L), pos, sc, window)
         g = got[row:row + n].cpu().double()
-        tol = ref.attend_tolerance(DT[dtype], o, mag, smax, D, L)
+        tol = ref.attend_tolerance(DT[dtype], o, mag, smax, vsum, D, L)
         bad = torch.isnan(g) | ((g - o).abs() > tol)
         assert not bool(bad.any()), (b, L, n, float(((g - o).abs() / tol).max()))
         gl = lse[row:row + n].cpu().double()
@@ -350,3 +350,302 @@ def test_attention_magnitudes(pkg, cuda_device, dtype, qgain, gain):
     rk, rv = fill(c, 9, gain)
     s = 0.125 if gain == 1.0 or qgain != 1.0 else 0.125 / gain
     check_attention(pkg, c, rk, rv, tables(lens, blk, P, 7), lens, [1, 2], 4, dtype, seed=7, qgain=qgain, scale=s)
+
+
+@pytest.mark.parametrize("D,blk,fmt", [(64, 16, "int8"), (96, 32, "e4m3"), (128, 64, "int8"), (128, 64, "e4m3"), (16, 64, "int8")])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attention_many_rows(pkg, cuda_device, D, blk, fmt, window):
+    """The tensor-core kernel: chunks on cached context, part row tiles, one and
+    two row tiles of a block, rows that begin a tile, queries off the vector's
+    alignment; sequences with few rows beside them."""
+    lens, news = [500, 129, 1, 700, 64, 400], [300, 65, 1, 257, 64, 3]
+    P = sum(-(-n // blk) for n in lens) + 1
+    c, _, _ = make_cache(pkg, P, 2, blk, D, fmt)
+    rk, rv = fill(c, 21)
+    tab = tables(lens, blk, P, 8)
+    for g in (1, 3, 8):
+        check_attention(pkg, c, rk, rv, tab, lens, news, 2 * g, "bf16", window=window, seed=20 + g, strided=g == 3, qgain=2.0)
+    N = sum(news)
+    q = randn((N, 4, D), 30, torch.bfloat16).cuda()
+    flat = torch.empty(N * 4 * D + 1, dtype=torch.bfloat16, device="cuda")
+    off = flat[1:].view(N, 4, D)
+    off.copy_(q)
+    args = (i32(tab.tolist()), i32(lens), cu_of(news), max(news))
+    assert torch.equal(c.attention(off, *args, out=torch.empty_like(off)), c.attention(q, *args))
+    # a wrong hint costs time, not results: both kernels answer alike but for their sums' order
+    a, b = c.attention(q, *args).float(), c.attention(q, *args[:3], 1).float()
+    assert float((a - b).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
+    assert torch.equal(c.attention(q, *args, scale=-0.07), c.attention(-q, *args, scale=0.07))
+
+
+@pytest.mark.parametrize("news", [1, 200])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_attention_masked_blocks_may_hold_anything(pkg, cuda_device, news, fmt):
+    """A block whose scale is NaN or infinite (or that names no page) spoils the
+    rows that see it and no others; memory past the last token is never used."""
+    L, blk, D = 640, 64, 64
+    c, _, _ = make_cache(pkg, 11, 1, blk, D, fmt)
+    rk, rv = fill(c, 31)
+    tab = np.arange(10)[None]
+    q = randn((news, 4, D), 32, torch.bfloat16).cuda()
+    args = (i32([L - 30]), i32([0, news]), news)
+    want = {w: c.attention(q, i32(tab.tolist()), *args, window=w) for w in (0, 100)}
+    keep = [t.clone() for t in (c.k_scale, c.v_scale)]
+    for bad in (float("nan"), float("inf")):
+        for which in ("k_scale", "v_scale"):
+            getattr(c, which)[1, 0] = bad  # tokens 64 .. 127
+            assert torch.isnan(c.attention(q, i32(tab.tolist()), *args)).all()
+            got = c.attention(q, i32(tab.tolist()), *args, window=100)
+            sees = torch.tensor([(L - 30 - news + i) - 100 <= 127 for i in range(news)])
+            assert torch.equal(torch.isnan(got).all(-1).all(-1).cpu(), sees) and torch.equal(torch.isnan(got).any(-1).any(-1).cpu(), sees)
+            assert torch.equal(got[~sees], want[100][~sees])
+            c.k_scale.copy_(keep[0])
+            c.v_scale.copy_(keep[1])
+    # the last page past its 34 tokens: junk codes; a later page that no row sees: junk scale
+    for t in (c.k_codes.view(torch.uint8)[9, :, 34:], c.v_codes.view(torch.uint8)[9, :, :, 34:]):
+        t.fill_(0x7F)
+    c.k_scale[10] = c.v_scale[10] = float("nan")
+    assert torch.equal(c.attention(q, i32(tab.tolist()), *args), want[0])
+    c.check()
+    # pages outside the cache
+    for page in (-1, 11, 2 ** 31 - 1):
+        t = tab.copy()
+        t[0, 0] = page
+        assert torch.isnan(c.attention(q, i32(t.tolist()), *args)).all()
+        with pytest.raises(pkg.api.NoorMoEError):
+            c.check()
+        got = c.attention(q, i32(t.tolist()), *args, window=100)
+        sees = torch.tensor([(L - 30 - news + i) - 100 <= 63 for i in range(news)])
+        assert torch.equal(torch.isnan(got).any(-1).any(-1).cpu(), sees) and torch.equal(got[~sees], want[100][~sees])
+        k, v = c.read(i32(t.tolist()), None, i32([0, 70]), 70)
+        assert torch.isnan(k[:64]).all() and torch.isnan(v[:64]).all() and torch.isfinite(k[64:].float()).all()
+        c.status.zero_()
+    c.check()
+
+
+def test_bad_metadata_is_reported_and_touches_nothing(pkg, cuda_device):
+    D, blk = 64, 32
+    c, _, _ = make_cache(pkg, 6, 1, blk, D, "int8")
+    fill(c, 33)
+    tab = i32([[0, 1], [2, 3]])
+    before = [t.clone() for t in (c.k_codes, c.v_codes, c.k_scale, c.v_scale)]
+    x = randn((4, 1, D), 34, torch.bfloat16).cuda()
+    for lens, cu in (([65, 2], [0, 2, 4]), ([-1, 2], [0, 2, 2]), ([1, 2], [0, 2, 2]), ([2, 2], [0, 5, 5]), ([2, 2], [3, 1, 1]),
+                     ([2, 2], [-2, 0, 0]), ([2 ** 31 - 1, 2], [0, 2, 2])):
+        out = torch.full_like(x, 3.0)
+        c.attention(x, tab, i32(lens), i32(cu), 4, out=out)
+        with pytest.raises(pkg.api.NoorMoEError):
+            c.check()
+        if lens[0] != 1:  # (rows at positions below 0 see nothing)
+            assert torch.all(out[:2] == 3.0)
+        c.append(x, x, i32([[0, 1], [2, 3]]), i32(lens), i32([min(max(v, -5), 9) for v in cu]))
+        torch.cuda.synchronize()
+        # sequence 1 is sound in the first case alone
+        pages = [0, 1, 4, 5] if lens[0] == 65 else range(6)
+        for t, b in zip((c.k_codes, c.v_codes, c.k_scale, c.v_scale), before):
+            assert torch.equal(t.view(torch.int8)[list(pages)] if t.dtype == torch.int8 else t[list(pages)], b[list(pages)])
+        with pytest.raises(pkg.api.NoorMoEError):
+            c.check()
+        for t, b in zip((c.k_codes, c.v_codes, c.k_scale, c.v_scale), before):
+            t.copy_(b)
+    c.read(tab, i32([60, 0]), i32([0, 8, 9]), 9)  # past the pages
+    with pytest.raises(pkg.api.NoorMoEError):
+        c.check()
+    c.append(x, x, i32([[6, -1], [2, 3]]), i32([2, 2]), i32([0, 2, 4]))
+    with pytest.raises(pkg.api.NoorMoEError):
+        c.check()
+    assert torch.equal(c.k_codes[:2], before[0][:2])
+    c.check()
+
+
+def test_attention_in_place_and_shared_pages(pkg, cuda_device):
+    """out may be q; sequences may share pages (a common prefix)."""
+    blk, D = 16, 48
+    c, _, _ = make_cache(pkg, 8, 2, blk, D, "e4m3")
+    rk, rv = fill(c, 35)
+    tab = np.array([[3, 5, 0, 1], [3, 5, 2, 6], [3, 3, 3, 3]])
+    lens, news = [50, 61, 64], [1, 40, 2]
+    for dt in ("bf16", "f32"):
+        check_attention(pkg, c, rk, rv, tab, lens, news, 6, dt, seed=36)
+        q = randn((43, 6, D), 37, DT[dt]).cuda()
+        args = (i32(tab.tolist()), i32(lens), cu_of(news), 40)
+        want = c.attention(q, *args)
+        assert c.attention(q, *args, out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_offsets_past_32_bits(pkg, cuda_device, fmt):
+    """Pages whose byte offsets pass 2^32 are written, read and attended to."""
+    P, H, blk, D = 33000, 8, 64, 256  # 4.3 GB a pool
+    c, rk_, rv_ = make_cache(pkg, P, H, blk, D, fmt, junk=False)
+    pages = [P - 1, 5, P - 2]
+    tab = i32([pages])
+    n = 130
+    k, v = randn((n, H, D), 41, torch.bfloat16), randn((n, H, D), 42, torch.bfloat16)
+    rk, rv = (ref.RefCache(3, H, blk, D, fmt) for _ in range(2))
+    rk.append(k.double(), 0, n, n, [0, 1, 2])
+    rv.append(v.double(), 0, n, n, [0, 1, 2])
+    c.append(k.cuda(), v.cuda(), tab, i32([n]), i32([0, n]))
+    gk, gv = c.read(tab, None, i32([0, n]), n)
+    assert torch.equal(gk.cpu().double(), rk.tokens([0, 1, 2], n)) and torch.equal(gv.cpu().double(), rv.tokens([0, 1, 2], n))
+    q = randn((3, 16, D), 43, torch.bfloat16)
+    got = c.attention(q.cuda(), tab, i32([n]), i32([0, 3]), 3).cpu().double()
+    o, _, mag, smax, vsum = ref.attend(q.double(), rk.tokens([0, 1, 2], n), rv.tokens([0, 1, 2], n), torch.arange(n - 3, n), D ** -0.5, 0)
+    assert bool(((got - o).abs() <= ref.attend_tolerance(torch.bfloat16, o, mag, smax, vsum, D, n)).all())
+    c.check()
+
+
+def test_graphs_and_streams(pkg, cuda_device):
+    """One captured decode step replays over growing lengths; two graphs and two
+    streams do not disturb one another; calls run on the current stream."""
+    A = pkg.attention
+    D, blk, H, Hq, B = 64, 16, 2, 4, 3
+    r = A.Rotary.create(D, device=0)
+
+    class Side:
+        def __init__(self, seed):
+            self.c, _, _ = make_cache(pkg, 24, H, blk, D, "e4m3")
+            self.tab = i32(np.arange(24).reshape(3, 8).tolist())
+            self.lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+            self.cu = i32([0, 1, 2, 3])
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            self.xs = [[torch.randn((B, h, D), device="cuda", generator=g).bfloat16() for h in (Hq, H, H)] for _ in range(40)]
+            self.q, self.k, self.v = (t.clone() for t in self.xs[0])
+
+        def step(self):
+            self.lens += 1
+            q = self.c.append(self.k, self.v, self.tab, self.lens, self.cu, rotary=r, q=self.q)
+            return self.c.attention(q, self.tab, self.lens, self.cu, 1)
+
+        def eager(self):
+            outs = []
+            for x in self.xs:
+                for d, s in zip((self.q, self.k, self.v), x):
+                    d.copy_(s)
+                outs.append(self.step().clone())
+            return outs
+
+    want = [Side(s).eager() for s in (1, 2)]
+    sides = [Side(1), Side(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    for s, st in zip(sides, streams):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            s.step()
+            s.lens.zero_()
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(s.step())
+        s.lens.zero_()
+        graphs.append(g)
+    torch.cuda.synchronize()
+    got = [[], []]
+    for i in range(40):
+        for j, (s, st, g) in enumerate(zip(sides, streams, graphs)):  # both at once, each on its stream
+            with torch.cuda.stream(st):
+                for d, x in zip((s.q, s.k, s.v), s.xs[i]):
+                    d.copy_(x)
+                g.replay()
+                got[j].append(outs[j].clone())
+    torch.cuda.synchronize()
+    for j in range(2):
+        sides[j].c.check()
+        for i in range(40):
+            assert torch.equal(got[j][i], want[j][i]), (j, i)
+
+
+def test_rope_gradient_in_a_graph_and_twice(pkg, cuda_device):
+    """Forward and backward captured together; the gradient's own gradient."""
+    A = pkg.attention
+    r = A.Rotary.create(32, device=0, layout="half")
+    pos = i32([3, 9, 1])
+    w = randn((3, 2, 32), 51).cuda()
+    x = randn((3, 2, 32), 52).cuda().requires_grad_()
+    (want,) = torch.autograd.grad((A.rope_apply(x, pos, r) * w).sum(), x)
+    y = randn((3, 2, 32), 52).cuda().requires_grad_()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        torch.autograd.grad((A.rope_apply(y, pos, r) * w).sum(), y)
+    torch.cuda.current_stream().wait_stream(st)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        (got,) = torch.autograd.grad((A.rope_apply(y, pos, r) * w).sum(), y)
+    got.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    # d/dx of sum(R^T(w x) v): R^T differentiates to R again
+    v = randn((3, 2, 32), 53).cuda()
+    z = randn((3, 2, 32), 54).cuda().requires_grad_()
+    (g1,) = torch.autograd.grad((A.rope_apply(z, pos, r) ** 2).sum(), z, create_graph=True)
+    (g2,) = torch.autograd.grad((g1 * v).sum(), z)
+    assert float((g2 - 2 * v).abs().max()) <= 1e-5  # R^T R = 1
+
+
+def test_stack_served_from_the_cache(pkg, cuda_device):
+    """NoorStack.forward_cached: the attention half against its plain form (the
+    projections, the cache and the attention of one layer), and a prompt at once
+    against the same tokens a few at a time.  e4m3 blocks grow without loss but
+    for codes under 2^-6 of a step's scale (2^-19 of the block's largest
+    value), so both ways agree to f32's sums: 1e-4."""
+    api, S = pkg.api, pkg.stack
+    rng = np.random.default_rng(5)
+    att = S.GQAAttention(64, 4, 2, 32, 24, 0.3, rng)
+    rope = S.RoPE(32, 10000.0)
+    x = randn((50, 64), 61)
+
+    class One:
+        blocks, device = [type("B", (), {"attention": att})], 0
+
+    cache = S.StackCache(One, 1, 96, block=16, fmt="int8")
+    rows = cache.step([50])
+    got = att.forward_cached(x.cuda(), rope, cache.layers[0], rows).cpu().double()
+    w = {n: torch.from_numpy(getattr(att, n)).double() for n in ("wq", "wk", "wv", "wo")}
+    q, k, v = ((x.double() @ w[n]).view(50, -1, 32) for n in ("wq", "wk", "wv"))
+    pos, inv = torch.arange(50), torch.from_numpy(rope.inv_freq)
+    rk, rv = ref.RefCache(6, 2, 16, 32, "int8"), ref.RefCache(6, 2, 16, 32, "int8")
+    rk.append(ref.rotate(k, pos, inv, "interleaved"), 0, 50, 50, range(6))
+    rv.append(v, 0, 50, 50, range(6))
+    o, _, mag, smax, vsum = ref.attend(ref.rotate(q, pos, inv, "interleaved"), rk.tokens(range(6), 50), rv.tokens(range(6), 50), pos,
+                                 32 ** -0.5, 24)
+    want = o.reshape(50, -1) @ w["wo"]
+    # a projection off by 2^-20 may round a code the other way: one step of its
+    # block for such a token, in k (through the score) and v
+    step = float(torch.maximum(rk.scale.max(), rv.scale.max()))
+    tol = (ref.attend_tolerance(torch.float32, o, mag, smax, vsum, 32, 50) + 2.0 ** -14 * mag).reshape(50, -1) @ w["wo"].abs() + 1e-5
+    bad = (got - want).abs() > tol
+    assert float(bad.double().mean()) <= 0.02 and float((got - want).abs().max()) <= 4 * step, (float(bad.double().mean()), step)
+
+    st = S.NoorStack(vocab_size=61, d_model=64, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=32, dense_ffn_dim=128,
+                     expert_ffn_dim=64, n_experts=4, n_active_experts=2, sliding_window=8, global_every_n=2, prope_fraction=0.25,
+                     dtype=api.DTYPE_F32, rng=rng)
+    ids = [list(rng.integers(0, 61, 37)), list(rng.integers(0, 61, 20))]
+    c1 = st.new_cache(2, 64, block=16, fmt="e4m3")
+    full, util = st.forward_cached(ids, c1)
+    c1.check()
+    assert full.shape == (57, 61) and torch.isfinite(full).all() and len(util) == 2
+    c2 = st.new_cache(2, 64, block=16, fmt="e4m3")
+    last = {}
+    at = [0, 0]
+    for n in ([30, 1], [1, 0], [0, 12], [5, 1], [1, 6]):
+        out, _ = st.forward_cached([ids[b][at[b]:at[b] + n[b]] for b in range(2)], c2)
+        rows = [0, n[0], n[0] + n[1]]
+        for b in range(2):
+            at[b] += n[b]
+            if n[b]:
+                last[b] = out[rows[b + 1] - 1]
+    assert at == [37, 20]
+    for b, row in ((0, 36), (1, 56)):
+        assert float((last[b] - full[row]).norm() / full[row].norm()) <= 1e-4
+    with pytest.raises(ValueError):
+        st.forward_cached([[1] * 30, []], c2)  # past max_tokens
+    with pytest.raises(ValueError):
+        st.forward_cached([[99], [1]], c2)
+    c2.reset(0)
+    again, _ = st.forward_cached([ids[0], []], c2)
+    assert float((again[-1] - full[36]).norm() / full[36].norm()) <= 1e-4
+    for b in st.blocks:
+        b.parallel_ffn.moe.invalidate()
