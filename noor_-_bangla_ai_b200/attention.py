@@ -37,9 +37,15 @@ _HEADS = struct.Struct("Pqq")
 _BATCH = struct.Struct("PqPPqii")
 
 
+_T = None
+
+
 def _torch():
-    import torch
-    return torch
+    global _T
+    if _T is None:
+        import torch
+        _T = torch
+    return _T
 
 
 def _code_dtype(fmt: str):
@@ -71,13 +77,16 @@ def _heads(t, what: str, device: int, dim: int) -> bytes:
 
 def _ints(t, what: str, n: int, device: int) -> int:
     """Data pointer of a contiguous int32 tensor [n] on `device`."""
-    if t.dtype is not _torch().int32 or t.get_device() != device:
-        raise ValueError(f"{what} must be an int32 tensor on cuda:{device}, got {t.dtype} on {t.device}")
-    if t.dim() != 1 or t.size(0) != n:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({n},)")
-    if n > 1 and t.stride(0) != 1:
-        raise ValueError(f"{what} must be contiguous")
+    st = t.stride()
+    if t.dtype is not _T.int32 or t.get_device() != device or len(st) != 1 or t.size(0) != n or (st[0] != 1 and n > 1):
+        raise ValueError(f"{what} must be a contiguous int32 tensor ({n},) on cuda:{device}, got {t.dtype} {tuple(t.shape)} "
+                         f"on {t.device}")
     return t.data_ptr()
+
+
+def _empty_like(t):
+    """Contiguous output of t's shape."""
+    return _T.empty_like(t, memory_format=_T.contiguous_format)
 
 
 def _stream(device: int) -> int:
@@ -165,7 +174,7 @@ def _rope_call(q, k, positions, rotary: Rotary, inverse: bool):
     if rotary.device != dev:
         raise ValueError(f"the rotary table is on cuda:{rotary.device}, q on cuda:{dev}")
     pos = _ints(positions, "positions", T, dev)
-    q_out = torch.empty((T, nq, D), dtype=q.dtype, device=q.device)
+    q_out = _empty_like(q)
     k_out = hk = hk_out = None
     nk = 0
     if k is not None:
@@ -173,7 +182,7 @@ def _rope_call(q, k, positions, rotary: Rotary, inverse: bool):
         nk = k.size(1)
         if k.dtype is not q.dtype or k.size(0) != T:
             raise ValueError("k must have q's tokens and type")
-        k_out = torch.empty((T, nk, D), dtype=q.dtype, device=q.device)
+        k_out = _empty_like(k)
         hk_out = _HEADS.pack(k_out.data_ptr(), nk * D, D)
     rc = api.lib().noor_rope_apply(rotary.ref, hq, _HEADS.pack(q_out.data_ptr(), nq * D, D), nq, hk, hk_out, nk, pos, T, D,
                                    dt, inverse, dev, _stream(dev))
@@ -348,7 +357,7 @@ class KVCache:
             nq = q.size(1)
             if q.size(0) != rows or q.dtype is not k.dtype:
                 raise ValueError("q must have k's rows and type")
-            q_out = torch.empty((rows, nq, D), dtype=q.dtype, device=q.device)
+            q_out = _empty_like(q)
             hq_out = _HEADS.pack(q_out.data_ptr(), nq * D, D)
         rc = api.lib().noor_kv_append(self._ref, batch, hk, hv, rot, hq, hq_out, nq, dt, _stream(dev))
         if rc:
@@ -366,7 +375,7 @@ class KVCache:
         shape = (rows, self.n_kv_heads, self.head_dim)
         dtype = torch.bfloat16 if dtype is None else dtype
         k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         rc = api.lib().noor_kv_read(self._ref, batch, st, k.data_ptr(), v.data_ptr(), _dtype_code(k), _stream(self._dev))
         if rc:
             api.check(rc)
@@ -388,7 +397,7 @@ class KVCache:
             raise ValueError(f"{nq} query heads over {self.n_kv_heads} kv heads")
         batch = self._batch(block_table, kv_lens, cu_rows, rows)
         if out is None:
-            out = torch.empty((rows, nq, D), dtype=q.dtype, device=q.device)
+            out = _empty_like(q)
             ho = _HEADS.pack(out.data_ptr(), nq * D, D)
         else:
             if out.shape != q.shape or out.dtype is not q.dtype:

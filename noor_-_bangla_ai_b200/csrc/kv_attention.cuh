@@ -286,6 +286,26 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
     const int tb = max(w.t0 + (int)(at - u0), lo_tok / kTile);
     const int te = min(w.t0 + (int)(stop - u0), (hi_tok + kTile - 1) / kTile);
 
+    // Query rows: lane (row gr of each group of 8, c) loads dims d0 .. d0 + 3 of
+    // step ks = 4 j + s, d0 = 16 (4 j + c) + 4 s, so that the quad's four lanes
+    // hold the whole row between them; the loads are in flight together and
+    // with those of the page table.
+    kv::Raw4<T> raw[NB][DP / 16];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = 8 * nb + gr, e = e0 + r;
+      const T* qp = nullptr;
+      if (r < nrows)
+        qp = static_cast<const T*>(a.q.p) + (int64_t)(w.s.row0 + e / a.g) * a.q.st + (int64_t)(h * a.g + e % a.g) * a.q.sh;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
+        raw[nb][ks] = kv::Raw4<T>{};
+        if (qp != nullptr && d0 < D)
+          raw[nb][ks] = a.qvec ? *reinterpret_cast<const kv::Raw4<T>*>(qp + d0)
+                               : kv::four(qp[d0], qp[d0 + 1], qp[d0 + 2], qp[d0 + 3]);
+      }
+    }
     // Page numbers and scales of 32 pages at a time, a page for each lane: the
     // list in use and the one after it, loaded a list ahead, so that no tile
     // waits for the page table.  -1: past the visible tokens; -2: unreadable
@@ -350,31 +370,15 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         if (tb + i < te) issue(pg, i * tile_pages, i);
     }
 
-    // ---- query fragments: this lane holds row gr of each group of 8, dims
-    // d0 .. d0 + 3 of step ks = 4 j + s, d0 = 16 (4 j + c) + 4 s
+    // ---- query fragments
     uint2 qreg[Sh::kQShared ? 1 : PARTS * DP / 16 * NB];
     float qfac[NB][2];  // score factors of rows 2c, 2c + 1 of each group
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int r = 8 * nb + gr, e = e0 + r;
-      const T* qp = nullptr;
-      if (r < nrows)
-        qp = static_cast<const T*>(a.q.p) + (int64_t)(w.s.row0 + e / a.g) * a.q.st + (int64_t)(h * a.g + e % a.g) * a.q.sh;
-      // the quad's four lanes hold the whole row between them; all its loads are
-      // in flight together
-      kv::Raw4<T> raw[DP / 16];
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        const int d0 = 16 * (4 * (ks >> 2) + qc) + 4 * (ks & 3);
-        raw[ks] = kv::Raw4<T>{};
-        if (qp != nullptr && d0 < D)
-          raw[ks] = a.qvec ? *reinterpret_cast<const kv::Raw4<T>*>(qp + d0)
-                           : kv::four(qp[d0], qp[d0 + 1], qp[d0 + 2], qp[d0 + 3]);
-      }
       float mx = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        const float4 v = kv::widen4(raw[ks], false);
+        const float4 v = kv::widen4(raw[nb][ks], false);
         mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       qfac[nb][1] = __shfl_sync(0xffffffffu, down, 8 * qc + 4);
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        const float4 v = kv::widen4(raw[ks], false);
+        const float4 v = kv::widen4(raw[nb][ks], false);
         const uint2 hi = make_uint2(pack_half(v.x * up, v.y * up), pack_half(v.z * up, v.w * up));
         const uint2 lo = make_uint2(pack_rest(v.x * up, v.y * up, hi.x), pack_rest(v.z * up, v.w * up, hi.y));
         if constexpr (Sh::kQShared) {
@@ -697,46 +701,70 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   }
 }
 
-// Join the parts of one cut unit's row: block (pair that holds the first
-// part, row).  The first pair's part may be its last piece (slot 1); every
-// later pair's is its first (slot 0).
+// Join the parts of one cut unit: a block for the pair that holds the first
+// part and 8 of its rows, a warp for each row.  The first pair's part may be
+// its last piece (slot 1); every later pair's is its first (slot 0).  A lane
+// weighs one part (32 at a time), then all lanes sum 4 dims each over the
+// parts, in the parts' order.
+constexpr int kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) combine_kernel(const Args a) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) combine_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched while the streamed kernel still runs)
-  const int wid = blockIdx.x, r = blockIdx.y;
-  const int4 d = a.desc[wid];
+  const int wid = blockIdx.x, lane = threadIdx.x & 31;
+  const int4 d = __ldg(a.desc + wid);
   if (d.x < 0) return;
+  const int r = min(blockIdx.y * kJoinWarps + (threadIdx.x >> 5), (unsigned)a.rows - 1u);
+  const int D = a.c.D, parts = (d.w >> 1) - wid + 1;
+  auto slot = [&](int i) -> int64_t {  // row r of part i
+    return (2 * ((int64_t)wid + i) + (i == 0 ? (d.w & 1) : 0)) * a.rows + r;
+  };
+  // (rows past the unit's read their slots and write nothing: the loads need not
+  // wait for the sequence's)
+  const float2 none = make_float2(-INFINITY, 0.f);
+  auto part = [&](int i) { return i < parts ? *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2) : none; };
+  const float2 ml0 = part(lane);
   const kv::Seq s = kv::sequence(a.b, a.b.cu, a.b.lens, a.c.blk, d.x, nullptr);
-  const int64_t e = (int64_t)a.rows * d.z + r;
-  if (e >= (int64_t)s.n * a.g) return;
-  const int D = a.c.D, last = d.w >> 1;
-  const int64_t slot0 = 2 * (int64_t)wid + (d.w & 1);
-  float m = -INFINITY;
-  for (int i = wid + threadIdx.x; i <= last; i += blockDim.x)
-    m = fmaxf(m, a.part_ml[((i == wid ? slot0 : 2 * (int64_t)i) * a.rows + r) * 2]);
-  __shared__ float s_m[4];
+  float m = ml0.x;
+  for (int i = lane + 32; i < parts; i += 32) m = fmaxf(m, part(i).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int base = 0; base < parts; base += 32) {
+    const int n = min(32, parts - base);
+    const float2 ml = base == 0 ? ml0 : part(base + lane);
+    const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - m), wl = ml.y * w;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float f = __shfl_sync(0xffffffffu, w, i);
+      l += __shfl_sync(0xffffffffu, wl, i);
+      const float* po = a.part_o + slot(base + i) * D;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int c = 4 * lane + 128 * y;
+        if (c < D) {
+          const float4 v = *reinterpret_cast<const float4*>(po + c);
+          acc[4 * y] = fmaf(v.x, f, acc[4 * y]);
+          acc[4 * y + 1] = fmaf(v.y, f, acc[4 * y + 1]);
+          acc[4 * y + 2] = fmaf(v.z, f, acc[4 * y + 2]);
+          acc[4 * y + 3] = fmaf(v.w, f, acc[4 * y + 3]);
+        }
+      }
+    }
+  }
+  const int64_t e = (int64_t)a.rows * d.z + r;
+  if (blockIdx.y * kJoinWarps + (threadIdx.x >> 5) >= (unsigned)a.rows || e >= (int64_t)s.n * a.g) return;
   const int row = s.row0 + (int)(e / a.g), head = d.y * a.g + (int)(e % a.g);
   T* op = static_cast<T*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
-  for (int c = threadIdx.x; c < D; c += blockDim.x) {
-    float acc = 0.f, l = 0.f;
-#pragma unroll 4
-    for (int i = wid; i <= last; ++i) {
-      const int64_t slot = (i == wid ? slot0 : 2 * (int64_t)i) * a.rows + r;
-      const float mi = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1];
-      if (li == 0.f) continue;
-      const float f = exp2_approx(mi - m);
-      l += li * f;
-      acc += a.part_o[slot * D + c] * f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int y = 0; y < 2; ++y)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int c = 4 * lane + 128 * y + x;
+      if (c < D) op[c] = rope::from_f32<T>(acc[4 * y + x] * inv);
     }
-    op[c] = rope::from_f32<T>(l == 0.f ? 0.f : acc / l);
-    if (a.lse != nullptr && c == 0)
-      a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m - kPShift + log2f(l)) * 0.69314718055994531f;
-  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m - kPShift + log2f(l)) * 0.69314718055994531f;
 }
 
 }  // namespace attn

@@ -453,14 +453,14 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     else
       CKR(c->format == NOOR_KV_INT8 ? attn::stream_f32_int8(a, p.nb, p.grid, s) : attn::stream_f32_e4m3(a, p.nb, p.grid, s));
     return by_dtype(dtype, [&](auto t) -> int {
-      const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g);
+      const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g), per = attn::kJoinWarps;
       // launched behind the streamed kernel without waiting for its end
       cudaLaunchAttribute attr{};
       attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
       attr.val.programmaticStreamSerializationAllowed = 1;
       cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3((unsigned)p.pairs, (unsigned)rows);
-      cfg.blockDim = dim3(128);
+      cfg.gridDim = dim3((unsigned)p.pairs, (unsigned)((rows + per - 1) / per));
+      cfg.blockDim = dim3(attn::kJoinWarps * 32);
       cfg.stream = s;
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
