@@ -260,19 +260,33 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
   return codes2<FMT>(a * ratio, b * ratio) | (codes2<FMT>(c * ratio, d * ratio) << 16);
 }
 
-// x rounded to f32 such that rounding that to a code gives what rounding x
-// would: where the nearest f32 could be a border of a code or of a scale (they
-// have at most 9 significant bits) and x is not it, the neighbour on x's side.
-// Powers of two scale both alike, so this can come before the scale is known.
-__device__ __forceinline__ float toward(double x) {
-  float h = (float)x;
-  if ((__float_as_uint(h) & 0x7FFFu) == 0) {
-    const double r = x - (double)h;
-    if (r != 0.0 && h == h) {
-      const bool up = (r > 0.0) == (h > 0.0);  // away from zero
-      if (h == 0.f) h = r > 0.0 ? 1e-45f : -1e-45f;
-      else h = __uint_as_float(__float_as_uint(h) + (up ? 1 : -1));
-    }
+// Larger magnitude, NaN if either is.
+__device__ __forceinline__ float max_abs(float m, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+  return r;
+}
+
+// f64 values rounded to f32 such that rounding those to codes gives what
+// rounding the values would: where the nearest f32 could be a border of a code
+// or of a scale (they have at most 9 significant bits) and the value is not it,
+// the neighbour on the value's side.  Powers of two scale both alike, so this
+// can come before the scale is known.
+__device__ __forceinline__ float toward(double x, float h) {
+  const double r = x - (double)h;
+  if ((__float_as_uint(h) & 0x7FFFu) != 0 || r == 0.0 || !(fabsf(h) <= 3.4028235e38f)) return h;
+  if (h == 0.f) return r > 0.0 ? 1e-45f : -1e-45f;
+  return __uint_as_float(__float_as_uint(h) + ((r > 0.0) == (h > 0.0) ? 1 : -1));
+}
+__device__ __forceinline__ float4 toward4(const double (&x)[4]) {
+  float4 h = make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+  const uint32_t low = min(min(__float_as_uint(h.x) & 0x7FFFu, __float_as_uint(h.y) & 0x7FFFu),
+                           min(__float_as_uint(h.z) & 0x7FFFu, __float_as_uint(h.w) & 0x7FFFu));
+  if (low == 0) {  // one in thousands, but for values that the rotation leaves as they are
+    h.x = toward(x[0], h.x);
+    h.y = toward(x[1], h.y);
+    h.z = toward(x[2], h.z);
+    h.w = toward(x[3], h.w);
   }
   return h;
 }
@@ -319,14 +333,14 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
   Raw4<T> raw[TPT];
   auto load = [&](int hb) {
     const bool live = thread_live && hb + hl < h1;
-    const T* kp = static_cast<const T*>(a.k.p) + (int64_t)k.row0 * a.k.st + (hb + hl) * a.k.sh;
+    const T* p = static_cast<const T*>(a.k.p) + (int64_t)(k.row0 + g) * a.k.st + (hb + hl) * a.k.sh;
+    const int64_t step = G * a.k.st;
 #pragma unroll
-    for (int j = 0; j < TPT; ++j) {
+    for (int j = 0; j < TPT; ++j, p += step) {
       if (G * j >= k.n) break;
       const int s = g + G * j;
       raw[j] = Raw4<T>{};
       if (live && s < k.n) {
-        const T* p = kp + s * a.k.st;
         if (a.kvec && run)
           raw[j] = *reinterpret_cast<const Raw4<T>*>(p + d0);
         else if (a.kvec && split)
@@ -350,26 +364,29 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
     }
     if (hb + at_once < h1) load(hb + at_once);  // the next heads', while these are worked on
     // ---- rotate; the largest magnitude chooses the scale
-    uint32_t amax = 0;
+    float fmx = 0.f;
     double c1[2] = {c0[0], c0[1]}, s1[2] = {s0[0], s0[1]};
 #pragma unroll
     for (int j = 0; j < TPT; ++j) {
       if (G * j >= k.n) break;
-      auto turn = [&](float& u, float& v, int y) {
-        if (turned[y]) {
-          const double a0 = u, a1 = v;
-          u = toward(a0 * c1[y] - a1 * s1[y]);
-          v = toward(a0 * s1[y] + a1 * c1[y]);
-          const double cn = c1[y] * cg[y] - s1[y] * sg[y];
-          s1[y] = s1[y] * cg[y] + c1[y] * sg[y];
-          c1[y] = cn;
+      if (turned[0]) {  // (both pairs or, where rot / 2 is odd, the first)
+        double y[4];
+        const double x0 = x[j].x, x1 = x[j].y, x2 = x[j].z, x3 = x[j].w;
+        y[0] = x0 * c1[0] - x1 * s1[0];
+        y[1] = x0 * s1[0] + x1 * c1[0];
+        y[2] = x2 * c1[1] - x3 * s1[1];
+        y[3] = x2 * s1[1] + x3 * c1[1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const double cn = c1[e] * cg[e] - s1[e] * sg[e];
+          s1[e] = s1[e] * cg[e] + c1[e] * sg[e];
+          c1[e] = cn;
         }
-        amax = max(amax, max(__float_as_uint(fabsf(u)), __float_as_uint(fabsf(v))));
-      };
-      turn(x[j].x, x[j].y, 0);
-      turn(x[j].z, x[j].w, 1);
+        x[j] = toward4(y);
+      }
+      fmx = max_abs(max_abs(max_abs(max_abs(fmx, x[j].x), x[j].y), x[j].z), x[j].w);
     }
-    amax = head_max(amax, live ? hl : kHeadsAtOnce, s_max, pass);
+    const uint32_t amax = head_max(__float_as_uint(fmx), live ? hl : kHeadsAtOnce, s_max, pass);
     if (!live) continue;
     const float scale = k.first > 0 ? grown_scale(s_old, scale_for<FMT>(amax)) : scale_for<FMT>(amax);
     const bool poisoned = scale != scale;
@@ -388,9 +405,9 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
     for (int j = 0; j < TPT; ++j) {
       const int s = g + G * j;
       if (s >= k.n) break;
-      const uint32_t e = poisoned ? 0 : codes2<FMT>(x[j].x * inv, x[j].y * inv),
-                     f = poisoned ? 0 : codes2<FMT>(x[j].z * inv, x[j].w * inv);
-      uint8_t* o = kc + (int64_t)(k.first + s) * D;
+      uint32_t e = codes2<FMT>(x[j].x * inv, x[j].y * inv), f = codes2<FMT>(x[j].z * inv, x[j].w * inv);
+      if (poisoned) e = f = 0;
+      uint8_t* o = kc + (k.first + s) * D;
       if (run) {
         *reinterpret_cast<uint32_t*>(o + d0) = e | (f << 16);
       } else if (split && d1 % 2 == 0) {
@@ -425,14 +442,29 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
   uint32_t next[16][W];
   auto load = [&](int hb) {
     const bool live = hl < at_once && hb + hl < h1;
-    const T* vp = static_cast<const T*>(a.v.p) + (int64_t)k.row0 * a.v.st + (hb + hl) * a.v.sh + d;
+    const int s0 = lo - k.first;
+    const T* p = static_cast<const T*>(a.v.p) + ((int64_t)k.row0 + s0) * a.v.st + (hb + hl) * a.v.sh + d;
+    if (live && all_new && a.vvec) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int s = lo + i - k.first;
+      for (int i = 0; i < 16; ++i, p += a.v.st) {
+        if constexpr (W == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          next[i][0] = u.x; next[i][1] = u.y; next[i][2] = u.z; next[i][3] = u.w;
+        } else if constexpr (W == 2) {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          next[i][0] = u.x; next[i][1] = u.y;
+        } else {
+          next[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i, p += a.v.st) {
+      const int s = s0 + i;
 #pragma unroll
       for (int x = 0; x < W; ++x) next[i][x] = 0;
       if (live && s >= 0 && s < k.n) {
-        const T* p = vp + s * a.v.st;
         if constexpr (W == 4) {
           if (a.vvec) {
             const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -511,13 +543,14 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
         uint32_t t[4];  // a token's 2 codes
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          t[i] = poisoned ? 0 : codes2<FMT>(value(4 * z + i, y) * inv, value(4 * z + i, y + 1) * inv);
+          t[i] = codes2<FMT>(value(4 * z + i, y) * inv, value(4 * z + i, y + 1) * inv);
         const uint32_t lo2 = __byte_perm(t[0], t[1], 0x5410), hi2 = __byte_perm(t[2], t[3], 0x5410);
         w[0][z] = __byte_perm(lo2, hi2, 0x6420);
         w[1][z] = __byte_perm(lo2, hi2, 0x7531);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        if (poisoned) w[e][0] = w[e][1] = w[e][2] = w[e][3] = 0;
         uint4* dst = reinterpret_cast<uint4*>(vc + (int64_t)(y + e) * blk);
         if (!all_new) {
           const uint4 was = *dst;
