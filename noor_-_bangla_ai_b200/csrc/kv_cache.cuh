@@ -81,18 +81,19 @@ struct Task {
   int64_t page;
 };
 
-// The t-th touched block in batch order, found by one warp: each sequence
-// touches the blocks of its tokens [pos0, pos0 + n).  starts: pos0 of each
-// sequence (reading), or NULL for the last n tokens (writing).  Returned in
-// every lane.
-__device__ __forceinline__ Task find_task(const Cache& c, const Batch& b, const int32_t* starts, bool write, int32_t t,
-                                          int lane) {
-  Task k;
-  k.b = -1;
-  const int blk = c.blk;
-  int32_t before = 0;
-  for (int base = 0; base < b.B; base += 32) {
-    const int i = base + lane;
+// The t-th touched block in batch order, found by the whole block of THREADS
+// threads, a sequence for each at a time: each sequence touches the blocks of
+// its tokens [pos0, pos0 + n).  starts: pos0 of each sequence (reading), or
+// NULL for the last n tokens (writing).  All threads call it and get it.
+template <int THREADS>
+__device__ __forceinline__ Task find_task(const Cache& c, const Batch& b, const int32_t* starts, bool write, int32_t t) {
+  __shared__ Task s_task;
+  __shared__ int32_t s_warp[THREADS / 32];
+  const int blk = c.blk, lblk = 31 - __clz(blk), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) s_task.b = -1;
+  int32_t before = 0;  // touched blocks of earlier sequences
+  for (int base = 0; base < b.B; base += THREADS) {
+    const int i = base + threadIdx.x;
     int32_t pos0 = 0, touched = 0;
     Seq s{0, 0, 0};
     if (i < b.B) {
@@ -102,7 +103,7 @@ __device__ __forceinline__ Task find_task(const Cache& c, const Batch& b, const 
         flag(c.status, NOOR_KV_BAD_LENGTH);
         s.n = 0;
       }
-      if (s.n > 0) touched = (pos0 + s.n - 1) / blk - pos0 / blk + 1;
+      if (s.n > 0) touched = ((pos0 + s.n - 1) >> lblk) - (pos0 >> lblk) + 1;
     }
     int32_t incl = touched;
 #pragma unroll
@@ -110,31 +111,36 @@ __device__ __forceinline__ Task find_task(const Cache& c, const Batch& b, const 
       const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const int32_t local = t - before;
-    const unsigned hit = __ballot_sync(0xffffffffu, local >= incl - touched && local < incl);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int32_t e0 = __shfl_sync(0xffffffffu, incl - touched, src);
-      const int32_t p0 = __shfl_sync(0xffffffffu, pos0, src);
-      const int32_t n = __shfl_sync(0xffffffffu, s.n, src);
-      const int32_t r0 = __shfl_sync(0xffffffffu, s.row0, src);
-      k.b = base + src;
-      k.j = p0 / blk + (local - e0);
-      const int32_t lo = max(p0, k.j * blk), hi = min(p0 + n, (k.j + 1) * blk);
-      k.first = lo - k.j * blk;
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int32_t mine = before, total = before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) mine += s_warp[w];
+      total += s_warp[w];
+    }
+    const int32_t local = t - (mine + incl - touched);  // which of this sequence's blocks
+    if (local >= 0 && local < touched) {
+      Task k;
+      k.b = i;
+      k.j = (pos0 >> lblk) + local;
+      const int32_t lo = max(pos0, k.j << lblk), hi = min(pos0 + s.n, (k.j + 1) << lblk);
+      k.first = lo - (k.j << lblk);
       k.n = hi - lo;
-      k.row0 = r0 + (lo - p0);
+      k.row0 = s.row0 + (lo - pos0);
       const int32_t page = __ldg(b.table + (int64_t)k.b * b.tstride + k.j);
       k.page = page;
       if (page < 0 || (int64_t)page >= c.P) {
-        if (lane == 0) flag(c.status, NOOR_KV_BAD_PAGE);
+        flag(c.status, NOOR_KV_BAD_PAGE);
         k.page = -1;
       }
-      return k;
+      s_task = k;
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    before = total;
+    __syncthreads();
+    if (t < before) break;
   }
-  return k;
+  return s_task;
 }
 
 // ------------------------------------------------------------- codes
@@ -613,7 +619,6 @@ template <typename T, int FMT, int TPT>
 __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kernel(const AppendArgs a) {
   extern __shared__ __align__(16) uint8_t s_append[];
   __shared__ Maxima s_max;
-  __shared__ Task s_task;
   if ((int)blockIdx.x >= a.kv_blocks) {
     if (a.qvec)
       append_rotate_q<T, true>(a, s_append);
@@ -624,12 +629,7 @@ __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kern
   if (threadIdx.x < kHeadsAtOnce) s_max.m[0][threadIdx.x] = 0;
   const int groups = (a.c.H + a.heads - 1) / a.heads;
   const int t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
-  if (threadIdx.x < 32) {
-    const Task f = find_task(a.c, a.b, nullptr, true, t, threadIdx.x);
-    if (threadIdx.x == 0) s_task = f;
-  }
-  __syncthreads();
-  const Task k = s_task;
+  const Task k = find_task<kAppendThreads>(a.c, a.b, nullptr, true, t);
   if (k.b < 0 || k.page < 0) return;
   const int h0 = (r >> 1) * a.heads, h1 = min(h0 + a.heads, a.c.H);
   if (r & 1)
@@ -703,13 +703,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
   const int D = c.D, blk = c.blk, tid = threadIdx.x;
   const int groups = (c.H + a.heads - 1) / a.heads, t = blockIdx.x / (2 * groups), r = blockIdx.x - t * 2 * groups;
   const int h0 = (r >> 1) * a.heads, nh = min(a.heads, c.H - h0);
-  __shared__ Task s_task;
-  if (tid < 32) {
-    const Task f = find_task(c, a.b, a.starts, false, t, tid);
-    if (tid == 0) s_task = f;
-  }
-  __syncthreads();
-  const Task k = s_task;
+  const Task k = find_task<kReadThreads>(c, a.b, a.starts, false, t);
   if (k.b < 0) return;
   const bool bad = k.page < 0;
   const float nan = __uint_as_float(0x7FC00000u);
