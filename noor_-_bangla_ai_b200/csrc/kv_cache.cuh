@@ -615,6 +615,7 @@ __device__ void append_rotate_q(const AppendArgs& a, uint8_t* smem) {
   }
 }
 
+// Keys and values in one launch: blocks alternate between them.
 template <typename T, int FMT, int TPT>
 __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kernel(const AppendArgs a) {
   extern __shared__ __align__(16) uint8_t s_append[];
@@ -636,6 +637,28 @@ __global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : 2) append_kern
     append_values<T, FMT, TPT == 16 ? 4 : 2>(a, k, h0, h1, s_max);
   else
     append_keys<T, FMT, TPT>(a, k, h0, h1, s_max);
+}
+
+// The same as two launches of half the grid, for batches with enough blocks to
+// fill the GPU: apart, keys and values need fewer registers each, so that more
+// blocks run at once.
+template <typename T, int FMT, int TPT>
+__global__ void __launch_bounds__(kAppendThreads, TPT == 16 ? 1 : TPT == 8 || sizeof(T) == 4 ? 2 : 3) keys_kernel(const AppendArgs a) {
+  __shared__ Maxima s_max;
+  if (threadIdx.x < kHeadsAtOnce) s_max.m[0][threadIdx.x] = 0;
+  const int groups = (a.c.H + a.heads - 1) / a.heads, t = blockIdx.x / groups, h0 = (blockIdx.x - t * groups) * a.heads;
+  const Task k = find_task<kAppendThreads>(a.c, a.b, nullptr, true, t);
+  if (k.b < 0 || k.page < 0) return;
+  append_keys<T, FMT, TPT>(a, k, h0, min(h0 + a.heads, a.c.H), s_max);
+}
+template <typename T, int FMT, int DPT>
+__global__ void __launch_bounds__(kAppendThreads, DPT * sizeof(T) == 4 ? 3 : DPT * sizeof(T) == 8 ? 2 : 1) values_kernel(const AppendArgs a) {
+  __shared__ Maxima s_max;
+  if (threadIdx.x < kHeadsAtOnce) s_max.m[0][threadIdx.x] = 0;
+  const int groups = (a.c.H + a.heads - 1) / a.heads, t = blockIdx.x / groups, h0 = (blockIdx.x - t * groups) * a.heads;
+  const Task k = find_task<kAppendThreads>(a.c, a.b, nullptr, true, t);
+  if (k.b < 0 || k.page < 0) return;
+  append_values<T, FMT, DPT>(a, k, h0, min(h0 + a.heads, a.c.H), s_max);
 }
 
 // The rotation of q by itself, for batches whose q would wait for the few

@@ -155,7 +155,7 @@ int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
   return NOOR_MOE_OK;
 }
 
-// Rows of q from which its rotation gets its own launch.
+// Rows from which q, k and v get a launch each.
 constexpr int64_t kApartRows = 1024;
 
 // Four elements of a head can be loaded at once from any multiple of four.
@@ -263,11 +263,11 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     a.qvec = q && vector_heads(a.r, dtype, {a.r.q, a.r.q_out});
     const size_t smem = q ? (size_t)a.q_tok * (a.r.rot / 2) * sizeof(float2) : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // q in blocks of the same launch, or where there is much of it in its own
-    const bool apart = q && b->n_rows >= kApartRows;
+    // one launch, or for many rows one each for q, k and v
+    const bool apart = b->n_rows >= kApartRows;
     return by_dtype(dtype, [&](auto t) -> int {
       using T = decltype(t);
-      if (apart) {
+      if (apart && q) {
         kv::AppendArgs alone = a;
         alone.kv_blocks = 0;
         if (a.qvec)
@@ -276,17 +276,22 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
           kv::rotate_q_kernel<T, false><<<(unsigned)qb, kv::kAppendThreads, smem, s>>>(alone);
         CK(cudaGetLastError());
       }
-      auto go = [&](auto kern) -> int {
-        kern<<<(unsigned)(kvb + (apart ? 0 : qb)), kv::kAppendThreads, smem, s>>>(a);
+      // tokens a thread can own: a block's over the 256 / (head_dim / 4) that share a pair
+      const int share = kv::kAppendThreads / (c->head_dim / 4), own = (c->block + share - 1) / share;
+      auto go = [&](auto fmt, auto tpt) -> int {
+        if (apart) {
+          kv::keys_kernel<T, fmt(), tpt()><<<(unsigned)(kvb / 2), kv::kAppendThreads, 0, s>>>(a);
+          kv::values_kernel<T, fmt(), tpt() == 16 ? 4 : 2><<<(unsigned)(kvb / 2), kv::kAppendThreads, 0, s>>>(a);
+        } else {
+          kv::append_kernel<T, fmt(), tpt()><<<(unsigned)(kvb + qb), kv::kAppendThreads, smem, s>>>(a);
+        }
         CK(cudaGetLastError());
         return NOOR_MOE_OK;
       };
-      // tokens a thread can own: a block's over the 256 / (head_dim / 4) that share a pair
-      const int share = kv::kAppendThreads / (c->head_dim / 4), own = (c->block + share - 1) / share;
       auto by_own = [&](auto fmt) -> int {
-        if (own <= 4 && c->head_dim <= 128) return go(kv::append_kernel<T, fmt(), 4>);
-        if (c->head_dim <= 128) return go(kv::append_kernel<T, fmt(), 8>);
-        return go(kv::append_kernel<T, fmt(), 16>);
+        if (own <= 4 && c->head_dim <= 128) return go(fmt, std::integral_constant<int, 4>{});
+        if (c->head_dim <= 128) return go(fmt, std::integral_constant<int, 8>{});
+        return go(fmt, std::integral_constant<int, 16>{});
       };
       return c->format == NOOR_KV_INT8 ? by_own(std::integral_constant<int, kv::INT8>{})
                                        : by_own(std::integral_constant<int, kv::E4M3>{});
