@@ -59,11 +59,13 @@ struct Args {
   bool qvec;       // q can be read four elements at a time
   float scale2;    // scale * log2(e)
   int32_t window;
-  // partial results: [2 * pairs] slots of `rows` rows of D o's, and of `rows` (m, l)
+  // partial results: [slots * pairs] slots of `rows` rows of D o's, and of `rows` (m, l)
   float* part_o;
   float* part_ml;
   int4* desc;      // [pairs] the cut unit that starts in a pair's share: (sequence or -1, head, row tile,
                    // last pair << 1 | slot of its part)
+  int32_t slots;   // 2: a pair's first and last piece
+  int32_t parts;   // tensor-core kernel: parts of a unit, each a block with one slot (it has no pairs)
   int32_t pairs;   // warp pairs of the grid that share the work
   int32_t rows;    // query rows of a row tile
   int64_t min_e, max_e;  // sequences with min_e <= rows * g < max_e are this launch's
@@ -716,7 +718,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) combine_kernel(const Args 
   const int r = min(blockIdx.y * kJoinWarps + (threadIdx.x >> 5), (unsigned)a.rows - 1u);
   const int D = a.c.D, parts = (d.w >> 1) - wid + 1;
   auto slot = [&](int i) -> int64_t {  // row r of part i
-    return (2 * ((int64_t)wid + i) + (i == 0 ? (d.w & 1) : 0)) * a.rows + r;
+    return (a.slots * ((int64_t)wid + i) + (i == 0 ? (d.w & 1) : 0)) * a.rows + r;
   };
   // (rows past the unit's read their slots and write nothing: the loads need not
   // wait for the sequence's)

@@ -6,24 +6,26 @@ namespace noor {
 namespace attn {
 namespace {
 
-template <int DP, int FMT>
-int launch(const Args& a, int units, cudaStream_t s) {
-  auto kern = prompt::prompt_kernel<DP, FMT>;
+template <int DP, int FMT, bool PARTS>
+int launch(const Args& a, int blocks, cudaStream_t s) {
+  auto kern = prompt::prompt_kernel<DP, FMT, PARTS>;
   constexpr int smem = prompt::Smem<DP>::kBytes;
   CKR(ensure_smem_limit(kern, smem));
-  kern<<<units, prompt::kThreads, smem, s>>>(a);
+  kern<<<blocks, prompt::kThreads, smem, s>>>(a);
   CK(cudaGetLastError());
   return NOOR_MOE_OK;
 }
 
+template <int FMT>
+int by_dim(const Args& a, int blocks, cudaStream_t s) {
+  if (a.c.D <= 64) return a.parts > 1 ? launch<64, FMT, true>(a, blocks, s) : launch<64, FMT, false>(a, blocks, s);
+  return a.parts > 1 ? launch<128, FMT, true>(a, blocks, s) : launch<128, FMT, false>(a, blocks, s);
+}
+
 }  // namespace
 
-int prompt_int8(const Args& a, int units, cudaStream_t s) {
-  return a.c.D <= 64 ? launch<64, kv::INT8>(a, units, s) : launch<128, kv::INT8>(a, units, s);
-}
-int prompt_e4m3(const Args& a, int units, cudaStream_t s) {
-  return a.c.D <= 64 ? launch<64, kv::E4M3>(a, units, s) : launch<128, kv::E4M3>(a, units, s);
-}
+int prompt_int8(const Args& a, int blocks, cudaStream_t s) { return by_dim<kv::INT8>(a, blocks, s); }
+int prompt_e4m3(const Args& a, int blocks, cudaStream_t s) { return by_dim<kv::E4M3>(a, blocks, s); }
 
 }  // namespace attn
 }  // namespace noor

@@ -2,8 +2,9 @@
 // tcgen05 tensor cores (BF16 activations, head_dim up to 128).
 //
 // A block takes one unit: 256 rows (query row, query head of the group) of one
-// kv head, as two row tiles of 128, and all their visible tokens in tiles of
-// 128.  The same sums as the streamed kernel (kv_attention.cuh):
+// kv head, as two row tiles of 128, and their visible tokens in tiles of 128:
+// all of them, or one of `parts` equal runs where there are fewer units than
+// SMs; combine_kernel then joins a unit's parts.  The same sums as the streamed kernel (kv_attention.cuh):
 //   s = q.k (f16 codes and f16 queries, f32 sums), p = 2^(s f - m + shift) in
 //   f16, o += p v, with f = scale log2(e) 2^e(row) k scale(block).
 // Roles:
@@ -22,7 +23,7 @@
 // when the maximum has grown by more than 2^8, so most tiles never touch o.
 // p <= 2^15 then fits f16; shift 7 keeps p down to 2^-31 of the largest.
 // A block's v scale is applied while widening, relative to the largest v scale
-// of the unit's pages (exact for powers of two).
+// so far (exact for powers of two); o follows when that grows.
 #pragma once
 
 #include "kv_attention.cuh"
@@ -109,7 +110,8 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
-template <int DP, int FMT>
+// PARTS: whether units are cut (compiled apart: the tests cost registers, 8% of the time)
+template <int DP, int FMT, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   using S = Smem<DP>;
   extern __shared__ uint8_t s_raw_base[];
@@ -122,18 +124,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   __shared__ __align__(8) Bars bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ uint32_t s_vref;
   __shared__ float s_kf[kMeta][8], s_vf[kMeta][8];  // factors of each 16 tokens
+  __shared__ float s_vref[kMeta], s_vstep[kMeta];   // the v reference, and the last one over it
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.c.D, blk = a.c.blk;
 
   // ---- the block's unit: last row tiles first, they see the most tokens
-  const int h = blockIdx.x % a.c.H;
+  const int parts = PARTS ? a.parts : 1;
+  const int part = blockIdx.x % parts, unit = blockIdx.x / parts, h = unit % a.c.H;
   int sb = -1, rt = 0;
   {
     int32_t before = 0;
-    const int32_t t = blockIdx.x / a.c.H;
+    const int32_t t = unit / a.c.H;
     for (int base = 0; base < a.b.B && sb < 0; base += 32) {
       int32_t n = 0;
       if (base + lane < a.b.B) n = attn::seq_work(a, base + lane).rtiles;
@@ -152,13 +155,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
+  if (PARTS && threadIdx.x == 0)
+    a.desc[blockIdx.x] = make_int4(part == 0 ? sb : -1, h, rt, (int)(blockIdx.x + parts - 1) << 1);
   if (sb < 0) return;
   const attn::SeqWork w = attn::seq_work(a, sb);
   const int e0 = 256 * rt, nrows = min(256, w.s.n * a.g - e0), nw = nrows > 128 ? 2 : 1;
   const int pos0 = w.s.len - w.s.n;
   const int p_first = pos0 + e0 / a.g, p_last = pos0 + (e0 + nrows - 1) / a.g;
   const int lo_tok = a.window > 0 ? max(p_first - a.window, 0) : 0, hi_tok = p_last + 1;
-  const int tb = lo_tok / kTok, te = (hi_tok + kTok - 1) / kTok, T = max(te - tb, 0);
+  const int first = lo_tok / kTok, count = max((hi_tok + kTok - 1) / kTok - first, 0);
+  const int tb = first + (int)((int64_t)count * part / parts);
+  const int T = first + (int)((int64_t)count * (part + 1) / parts) - tb;
   const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
 
   if (threadIdx.x == 0) {
@@ -176,7 +183,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     }
     tc::mbar_init(&bar.drain, 1);
     abort_flag = 0;
-    s_vref = 0x00800000u;  // the smallest normal number
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     async_fence();
   }
@@ -189,21 +195,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // largest finite v scale of the unit's pages
-  {
-    uint32_t mx = 0;
-    for (int64_t p = lo_tok / blk + threadIdx.x; p * blk < hi_tok; p += kThreads) {
-      const int32_t page = __ldg(table + p);
-      if (page >= 0 && (int64_t)page < a.c.P) {
-        const uint32_t b = __float_as_uint(fabsf(__ldg(a.c.vs + (int64_t)page * a.c.H + h)));
-        if (b < 0x7F800000u) mx = max(mx, b);
-      }
-    }
-    mx = __reduce_max_sync(0xffffffffu, mx);
-    if (lane == 0) atomicMax(&s_vref, mx);
-  }
-  __syncthreads();
-
   // Bounded wait: false once a wait anywhere in the block gave up.
   auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
     if (tc::mbar_try_wait(b, parity)) return true;
@@ -220,9 +211,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   };
 
   // Registers: 128 a thread at launch (512 x 128, the whole file); the eight
-  // softmax warps take 176, the other eight keep 80: 256 x 176 + 256 x 80 = 65536.
+  // softmax warps take 160, the other eight keep 96 (256 x 160 + 256 x 96 =
+  // 65536): neither spills.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     // ------------------------------------------------------- softmax
     const int wg = warp >> 2, r = (warp & 3) * 32 + lane;  // row of this row tile
     const int e = e0 + 128 * wg + r;
@@ -234,36 +226,39 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       // the row's queries, scaled by a power of two (negative if the scale is)
       // so that the largest is in 2^14 .. 2^15
       const bf16* qp = static_cast<const bf16*>(a.q.p) + (int64_t)row * a.q.st + (int64_t)head * a.q.sh;
-      const bool vec = (reinterpret_cast<uintptr_t>(a.q.p) | (uintptr_t)(a.q.st * 2) | (uintptr_t)(a.q.sh * 2)) % 16 == 0;
-      auto load8 = [&](int d, float (&v)[8]) {
-        if (vec) {
-          rope::Vec<bf16>::load(qp + d, v);
-        } else {
+      const bool qvec = (reinterpret_cast<uintptr_t>(a.q.p) | (uintptr_t)(a.q.st * 2) | (uintptr_t)(a.q.sh * 2)) % 16 == 0;
+      uint4 qr[DP / 8];  // all loads in flight together
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = __bfloat162float(qp[d + x]);
+      for (int d = 0; d < DP / 8; ++d) {
+        qr[d] = make_uint4(0, 0, 0, 0);
+        if (live && 8 * d < D) {
+          if (qvec) {
+            qr[d] = *reinterpret_cast<const uint4*>(qp + 8 * d);
+          } else {
+            const uint16_t* e16 = reinterpret_cast<const uint16_t*>(qp + 8 * d);
+            qr[d] = make_uint4(e16[0] | (uint32_t)e16[1] << 16, e16[2] | (uint32_t)e16[3] << 16,
+                               e16[4] | (uint32_t)e16[5] << 16, e16[6] | (uint32_t)e16[7] << 16);
+          }
         }
-      };
-      float mx = 0.f;
-      if (live)
-        for (int d = 0; d < D; d += 8) {
-          float v[8];
-          load8(d, v);
+      }
+      uint32_t mb = 0;  // magnitudes, two at a time
 #pragma unroll
-          for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(v[x]));
-        }
-      const int ex = max(min((int)(__float_as_uint(mx) >> 23) - 127, 127), -112);
+      for (int d = 0; d < DP / 8; ++d)
+        mb = __vmaxu2(mb, __vmaxu2(__vmaxu2(qr[d].x & 0x7FFF7FFFu, qr[d].y & 0x7FFF7FFFu),
+                                   __vmaxu2(qr[d].z & 0x7FFF7FFFu, qr[d].w & 0x7FFF7FFFu)));
+      const int ex = max(min((int)(max(mb & 0x7FFF0000u, mb << 16) >> 23) - 127, 127), -112);
       float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
       const float fac = fabsf(a.scale2) * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
       if (a.scale2 < 0.f) up = -up;
-      for (int d = 0; d < D; d += 8) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) load8(d, v);
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        if (8 * d >= D) break;
         uint4 u;
-        u.x = attn::pack_half(v[0] * up, v[1] * up);
-        u.y = attn::pack_half(v[2] * up, v[3] * up);
-        u.z = attn::pack_half(v[4] * up, v[5] * up);
-        u.w = attn::pack_half(v[6] * up, v[7] * up);
-        *reinterpret_cast<uint4*>(s_q + wg * S::kQ + (d >> 6) * (128 * 128) + swizzled(r, (d & 63) >> 3)) = u;
+        u.x = attn::pack_half(bf16_lo(qr[d].x) * up, bf16_hi(qr[d].x) * up);
+        u.y = attn::pack_half(bf16_lo(qr[d].y) * up, bf16_hi(qr[d].y) * up);
+        u.z = attn::pack_half(bf16_lo(qr[d].z) * up, bf16_hi(qr[d].z) * up);
+        u.w = attn::pack_half(bf16_lo(qr[d].w) * up, bf16_hi(qr[d].w) * up);
+        *reinterpret_cast<uint4*>(s_q + wg * S::kQ + (d >> 3) * (128 * 128) + swizzled(r, d & 7)) = u;
       }
       async_fence();
       __syncwarp();
@@ -310,11 +305,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         const bool grow = mx2 > m + kLazy || (m == -INFINITY && mx2 > -INFINITY);
         if (i == 0) {
           m = mx2;
-        } else if (__any_sync(0xffffffffu, grow)) {
+        } else if (__any_sync(0xffffffffu, grow) || s_vstep[i % kMeta] != 1.f) {
           // (o holds all earlier tiles: its last product ran before this s)
-          const float alpha = grow ? attn::exp2_approx(m - mx2) : 1.f;
+          float alpha = grow ? attn::exp2_approx(m - mx2) : 1.f;
           if (grow) m = mx2;
           l *= alpha;
+          alpha *= s_vstep[i % kMeta];
           for (int c = 0; c < D; c += 16) {
             uint32_t v[16];
             asm volatile(
@@ -379,7 +375,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         tc::tc_fence_after();
       }
       if (ok) {
-        const float inv = l == 0.f ? 0.f : 1.f / l * __uint_as_float(s_vref);
+        const float vref = T > 0 ? s_vref[(T - 1) % kMeta] : 0.f;
+        // a part leaves its sums as they are, with the reference of the join's shift
+        const float inv = PARTS ? vref : l == 0.f ? 0.f : 1.f / l * vref;
+        const int64_t slot = (int64_t)blockIdx.x * 256 + 128 * wg + r;
         bf16* op = static_cast<bf16*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
         const bool ovec = (reinterpret_cast<uintptr_t>(a.out.p) | (uintptr_t)(a.out.st * 2) | (uintptr_t)(a.out.sh * 2)) % 16 == 0;
         for (int c = 0; c < D; c += 16) {
@@ -398,7 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           float z[16];
 #pragma unroll
           for (int x = 0; x < 16; ++x) z[x] = __uint_as_float(v[x]) * inv;
-          if (live && ovec) {
+          if constexpr (PARTS) {
+            if (live)
+#pragma unroll
+              for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + c + x) = make_float4(z[x], z[x + 1], z[x + 2], z[x + 3]);
+          } else if (live && ovec) {
 #pragma unroll
             for (int y = 0; y < 2; ++y)
               *reinterpret_cast<uint4*>(op + c + 8 * y) =
@@ -410,12 +413,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           }
           __syncwarp();
         }
-        if (live && a.lse != nullptr)
+        if (PARTS && live)
+          *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m + (attn::kPShift - kShift), l);
+        else if (live && a.lse != nullptr)
           a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * 0.69314718055994531f;
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------- widen
     // Each thread keeps its 16-byte piece and walks down the rows, so that
     // addresses (and the swizzle, rows 16 or 32 apart) only advance; four
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       if (!ok) break;
       uint8_t* dk = s_k + slot * S::kK;
       if (kin) {
-#pragma unroll
+#pragma unroll 1
         for (int it = 0; it < kTok / kRowStep; it += 4) {
           uint4 c[4];
 #pragma unroll
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         const int n = min(max(nv - 4 * y, 0), 4);
         keep[y] = n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
       }
-#pragma unroll
+#pragma unroll 1
       for (int it = 0; it < DP / 16; it += 4) {
         uint4 c[4];
 #pragma unroll
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       }
     }
   } else if (warp == 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------- mma
     // The whole warp runs the loop, so that descriptors and TMEM addresses stay
     // in uniform registers; one elected thread issues.
@@ -587,13 +592,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     }
     __syncwarp();
   } else if (warp > 13) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------- loader
     const int pages = kTok / blk;
     const uint32_t bytes = (uint32_t)blk * D;
-    const float vref = __uint_as_float(s_vref), nan = __uint_as_float(0x7FC00000u);
+    const float nan = __uint_as_float(0x7FC00000u);
+    float vref = 1.17549435e-38f;  // the largest v scale so far
     int issued = 0;  // tiles whose copies were issued (k, and v one step later)
     bool ok = true, vpending = false;
     for (int i = 0; i < T && ok; ++i) {
@@ -614,13 +620,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       ks = __shfl_sync(0xffffffffu, ks, src);
       vs = __shfl_sync(0xffffffffu, vs, src);
       const bool fin = fabsf(vs) <= 3.4028235e38f;
+      const float vnew = fmaxf(vref, __uint_as_float(__reduce_max_sync(0xffffffffu, fin ? __float_as_uint(fabsf(vs)) : 0u)));
       ok = wait(&bar.raw_empty[0], (i & 1) ^ 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane < 8) {
         s_kf[i % kMeta][lane] = fin ? ks : nan;
-        s_vf[i % kMeta][lane] = fin ? vs / vref : 0.f;
+        s_vf[i % kMeta][lane] = fin ? vs / vnew : 0.f;
+        s_vref[i % kMeta] = vnew;
+        s_vstep[i % kMeta] = vref / vnew;
       }
+      vref = vnew;
       const unsigned who = __ballot_sync(0xffffffffu, page >= 0);
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_expect_tx(&bar.raw_full[0], __popc(who) * bytes);

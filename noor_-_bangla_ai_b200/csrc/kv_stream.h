@@ -34,8 +34,8 @@ int stream_launch(const Args& a, int nb, int grid, cudaStream_t s) {
 }
 
 // The tensor-core kernel for many rows (kv_prompt.cuh).
-int prompt_int8(const Args& a, int units, cudaStream_t s);
-int prompt_e4m3(const Args& a, int units, cudaStream_t s);
+int prompt_int8(const Args& a, int blocks, cudaStream_t s);
+int prompt_e4m3(const Args& a, int blocks, cudaStream_t s);
 
 int stream_bf16_int8(const Args& a, int nb, int grid, cudaStream_t s);
 int stream_bf16_e4m3(const Args& a, int nb, int grid, cudaStream_t s);

@@ -337,14 +337,42 @@ namespace {
 
 struct StreamPlan {
   int grid = 0, pairs = 0, nb = 1;
-  int64_t off_ml = 0, off_desc = 0, bytes = 0;
+  int prompt = 0, parts = 1;  // units of the tensor-core kernel (0: not launched) and parts of each
+  int64_t off_ml = 0, off_desc = 0, off_prompt = 0, off_prompt_ml = 0, off_prompt_desc = 0, bytes = 0;
 };
+
+// Rows (times query heads of a group) from which a sequence runs on the
+// tensor-core kernel.
+constexpr int64_t kPromptRows = 128;
+
+bool prompt_fits(const noor_kv_cache* c, const noor_kv_batch* b, int g, int max_rows, int dtype) {
+  return dtype == NOOR_DTYPE_BF16 && c->head_dim <= 128 && (int64_t)max_rows * g >= kPromptRows &&
+         b->n_rows * g >= kPromptRows;
+}
+
+// Parts of each of the tensor-core kernel's units: those with the shortest time
+// for the last SM, in tiles of 128 tokens (2.2 us); a block's start and end cost
+// some six of them, the join four.  BF16 over int8, 512 rows of 16 / 4 heads of
+// 128 dims: 8192 tokens 162 us whole, 77 us in four parts; 1024 tokens (1024
+// rows) 43 us whole, 49 us in two.
+int prompt_parts(int64_t units, int64_t tiles, int sms) {
+  int best = 1;
+  double time = (double)((units + sms - 1) / sms) * (tiles + 6);
+  for (int s = 2; s <= tiles / 4 && s * units <= 2 * sms; ++s) {
+    const double t = (double)((s * units + sms - 1) / sms) * ((double)tiles / s + 6) + 4;
+    if (t < 0.95 * time) {
+      best = s;
+      time = t;
+    }
+  }
+  return best;
+}
 
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
 // have that many tiles.  Up to 8 query rows for a kv head use one column group
 // of the mma; more use as many as the registers hold, so that a tile's codes
 // are widened once for 32 rows (16 at more than 128 dims).
-int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int dtype, StreamPlan* p) {
+int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int window, int dtype, StreamPlan* p) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
   const int64_t g = Hq / c->n_kv_heads;
@@ -363,16 +391,38 @@ int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_
   p->off_ml = (int64_t)p->pairs * 2 * R * c->head_dim * 4;
   p->off_desc = p->off_ml + (int64_t)p->pairs * 2 * R * 2 * 4;
   p->bytes = p->off_desc + (int64_t)p->pairs * 16;
+  if (prompt_fits(c, b, (int)g, max_rows, dtype)) {
+    const int64_t units = std::min(b->n_rows * g, b->n_rows * g / 256 + b->batch) * c->n_kv_heads;
+    if (units > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
+    p->prompt = (int)units;
+    // a unit's rows see at most that many tiles
+    int64_t seen = (tiles + 1) / 2;
+    if (window > 0) seen = std::min(seen, ((int64_t)window + 256 / g) / 128 + 2);
+    p->parts = prompt_parts(units, seen, sms);
+    const int64_t n = p->parts > 1 ? units * p->parts : 0;
+    p->off_prompt = (p->bytes + 15) / 16 * 16;
+    p->off_prompt_ml = p->off_prompt + n * 256 * c->head_dim * 4;
+    p->off_prompt_desc = p->off_prompt_ml + n * 256 * 2 * 4;
+    p->bytes = p->off_prompt_desc + n * 16;
+  }
   return NOOR_MOE_OK;
 }
 
-// Rows (times query heads of a group) from which a sequence runs on the
-// tensor-core kernel.
-constexpr int64_t kPromptRows = 128;
-
-bool prompt_fits(const noor_kv_cache* c, const noor_kv_batch* b, int g, int max_rows, int dtype) {
-  return dtype == NOOR_DTYPE_BF16 && c->head_dim <= 128 && (int64_t)max_rows * g >= kPromptRows &&
-         b->n_rows * g >= kPromptRows;
+// The join of the `n` slots' cut units, launched behind the kernel that leaves
+// the parts without waiting for its end.  rows: the most rows a unit can have.
+template <typename T>
+int launch_join(const attn::Args& a, int n, int rows, cudaStream_t s) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)n, (unsigned)((rows + attn::kJoinWarps - 1) / attn::kJoinWarps));
+  cfg.blockDim = dim3(attn::kJoinWarps * 32);
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  CK(cudaLaunchKernelEx(&cfg, attn::combine_kernel<T>, a));
+  return NOOR_MOE_OK;
 }
 
 int check_heads(const noor_kv_cache* c, int Hq) {
@@ -394,7 +444,7 @@ int noor_kv_attention_workspace(const noor_kv_cache* c, const noor_kv_batch* b, 
     CKR(check_heads(c, q_heads));
     if (!bytes || max_rows < 0) return fail(NOOR_MOE_ERR_INVALID, "null bytes or negative max_rows");
     StreamPlan p;
-    CKR(stream_plan(c, b, q_heads, max_rows, dtype, &p));
+    CKR(stream_plan(c, b, q_heads, max_rows, 0, dtype, &p));  // (a window never needs more)
     *bytes = p.bytes;
     return NOOR_MOE_OK;
   });
@@ -416,7 +466,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
       return fail(NOOR_MOE_ERR_INVALID, "workspace is null or not 16-byte aligned");
     StreamPlan p;
-    CKR(stream_plan(c, b, q_heads, max_rows, dtype, &p));
+    CKR(stream_plan(c, b, q_heads, max_rows, window, dtype, &p));
     if (workspace_bytes < p.bytes)
       return fail(NOOR_MOE_ERR_INVALID, "workspace of %lld bytes, needs %lld", (long long)workspace_bytes,
                   (long long)p.bytes);
@@ -435,42 +485,37 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     a.scale2 = scale * 1.4426950408889634f;
     a.window = window;
     a.pairs = p.pairs;
+    a.slots = 2;
+    a.parts = 1;
     a.rows = 8 * p.nb;
     a.min_e = 0;
     a.max_e = INT64_MAX;
-    // Sequences with many rows go to the tensor-core kernel, the others to the
-    // streamed one (only the device knows which a batch has).
-    if (prompt_fits(c, b, a.g, max_rows, dtype)) {
-      attn::Args t = a;
-      t.rows = 256;
-      t.min_e = kPromptRows;
-      const int64_t units = std::min(b->n_rows * a.g, b->n_rows * a.g / 256 + b->batch) * c->n_kv_heads;
-      if (units > INT32_MAX) return fail(NOOR_MOE_ERR_INVALID, "too many rows");
-      CKR(c->format == NOOR_KV_INT8 ? attn::prompt_int8(t, (int)units, s) : attn::prompt_e4m3(t, (int)units, s));
-      a.max_e = kPromptRows;
-    }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float*>(ws + p.off_ml);
     a.desc = reinterpret_cast<int4*>(ws + p.off_desc);
+    // Sequences with many rows go to the tensor-core kernel, the others to the
+    // streamed one (only the device knows which a batch has).
+    if (p.prompt) {
+      attn::Args t = a;
+      t.rows = 256;
+      t.min_e = kPromptRows;
+      t.slots = 1;
+      t.parts = p.parts;
+      const int64_t blocks = (int64_t)p.prompt * p.parts;
+      t.part_o = reinterpret_cast<float*>(ws + p.off_prompt);
+      t.part_ml = reinterpret_cast<float*>(ws + p.off_prompt_ml);
+      t.desc = reinterpret_cast<int4*>(ws + p.off_prompt_desc);
+      CKR(c->format == NOOR_KV_INT8 ? attn::prompt_int8(t, (int)blocks, s) : attn::prompt_e4m3(t, (int)blocks, s));
+      if (p.parts > 1) CKR(launch_join<bf16>(t, (int)blocks, 256, s));
+      a.max_e = kPromptRows;
+    }
     if (dtype == NOOR_DTYPE_BF16)
       CKR(c->format == NOOR_KV_INT8 ? attn::stream_bf16_int8(a, p.nb, p.grid, s) : attn::stream_bf16_e4m3(a, p.nb, p.grid, s));
     else
       CKR(c->format == NOOR_KV_INT8 ? attn::stream_f32_int8(a, p.nb, p.grid, s) : attn::stream_f32_e4m3(a, p.nb, p.grid, s));
     return by_dtype(dtype, [&](auto t) -> int {
-      const int64_t rows = std::min<int64_t>(a.rows, b->n_rows * a.g), per = attn::kJoinWarps;
-      // launched behind the streamed kernel without waiting for its end
-      cudaLaunchAttribute attr{};
-      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr.val.programmaticStreamSerializationAllowed = 1;
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3((unsigned)p.pairs, (unsigned)((rows + per - 1) / per));
-      cfg.blockDim = dim3(attn::kJoinWarps * 32);
-      cfg.stream = s;
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      CK(cudaLaunchKernelEx(&cfg, attn::combine_kernel<decltype(t)>, a));
-      return NOOR_MOE_OK;
+      return launch_join<decltype(t)>(a, a.pairs, (int)std::min<int64_t>(a.rows, b->n_rows * a.g), s);
     });
   });
 }

@@ -205,6 +205,36 @@ def test_append_and_read(pkg, cuda_device, fmt, dtype, H, D, blk, layout, rot):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype,H,D,blk,layout", [("bf16", 2, 128, 64, "half"), ("f32", 1, 64, 16, "interleaved"),
+                                                  ("bf16", 1, 256, 32, "interleaved"), ("f32", 2, 144, 64, "half")])
+def test_append_long_prompts(pkg, cuda_device, fmt, dtype, H, D, blk, layout):
+    """Prompts of more than a thousand rows, which keys, values and queries are
+    written for in a launch each: a fresh sequence, one that goes on inside a
+    block with larger values, an idle one."""
+    A = pkg.attention
+    P = -(-1200 // blk) + -(-90 // blk) + 1
+    c, rk, rv = make_cache(pkg, P, H, blk, D, fmt)
+    tab = tables([1200, 90, 0], blk, P, 11)[:, :-(-1200 // blk)]
+    inv = torch.from_numpy((10000.0 ** (-2.0 * np.arange(D // 2) / D)).astype(np.float32))
+    r = A.Rotary(inv.cuda(), layout, 1.0)
+    lens = np.zeros(3, int)
+    for si, n in enumerate(([5, 0, 0], [1100, 77, 0], [3, 13, 0])):
+        N, cu = sum(n), np.concatenate([[0], np.cumsum(n)])
+        k, v = randn((N, H, D), 50 + si, DT[dtype], 1.0 + si), randn((N, H, D), 60 + si, DT[dtype], 1.0 + si)
+        q = randn((N, 3 * H, D), 70 + si, DT[dtype])
+        lens = lens + np.array(n)
+        pos = torch.tensor([p for b in range(3) for p in range(lens[b] - n[b], lens[b])], dtype=torch.int64)
+        kr = ref.rotate(k, pos, inv, layout)
+        for b in range(3):
+            rk.append(kr, int(cu[b]), n[b], int(lens[b]), tab[b])
+            rv.append(v.double(), int(cu[b]), n[b], int(lens[b]), tab[b])
+        q_out = c.append(k.cuda(), v.cuda(), i32(tab.tolist()), i32(lens.tolist()), cu_of(n), rotary=r, q=q.cuda())
+        c.check()
+        cache_equal(c, rk, rv, [(tab[b], int(lens[b])) for b in range(3)], blk)
+        check_rope(q_out, q, pos, inv, layout, 1.0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_append_values_at_the_edges(pkg, cuda_device, fmt):
     """Zeros, subnormals, values at the scale's border, the largest floats, and
     values that are not finite; a poisoned block reads NaN until it starts over."""
@@ -376,6 +406,60 @@ def test_attention_many_rows(pkg, cuda_device, D, blk, fmt, window):
     a, b = c.attention(q, *args).float(), c.attention(q, *args[:3], 1).float()
     assert float((a - b).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
     assert torch.equal(c.attention(q, *args, scale=-0.07), c.attention(-q, *args, scale=0.07))
+
+
+@pytest.mark.parametrize("D,blk,fmt", [(64, 64, "int8"), (128, 16, "e4m3"), (80, 32, "int8")])
+@pytest.mark.parametrize("lens,news", [([3000], [200]), ([2500, 1, 0, 70], [130, 1, 0, 33]), ([130], [130])])
+def test_attention_many_rows_in_parts(pkg, cuda_device, D, blk, fmt, lens, news):
+    """Few rows over a long context: the tensor-core kernel cuts the context and
+    joins the parts.  Parts without a tile (the table has room for more than the
+    sequences hold), windows inside one part and over several, a page that
+    cannot be read."""
+    P = sum(-(-n // blk) for n in lens) + 1
+    c, _, _ = make_cache(pkg, P, 1, blk, D, fmt)
+    rk, rv = fill(c, 22)
+    tab = tables(lens, blk, P, 9)
+    tab = np.concatenate([tab, np.full((len(lens), 3000 // blk), -1, np.int64)], 1)
+    for window in (0, 90, 1500):
+        check_attention(pkg, c, rk, rv, tab, lens, news, 4, "bf16", window=window, seed=40 + window, qgain=2.0, strided=window == 90)
+    q = randn((news[0], 4, D), 41, torch.bfloat16).cuda()
+    bad = tab[:1].copy()
+    at = (lens[0] - news[0]) // blk + 1  # some rows see it, those before do not
+    bad[0, at] = P + 5
+    got, lse = c.attention(q, i32(bad.tolist()), i32(lens[:1]), cu_of(news[:1]), news[0], return_lse=True)
+    with pytest.raises(RuntimeError, match="page"):
+        c.check()
+    want = c.attention(q, i32(tab[:1].tolist()), i32(lens[:1]), cu_of(news[:1]), news[0])
+    n = max(at * blk - (lens[0] - news[0]), 0)
+    assert torch.equal(got[:n], want[:n]) and torch.isnan(got[n:]).all() and torch.isnan(lse[n:]).all()
+    c.check()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows", [16, 128])
+@pytest.mark.parametrize("down", [20, 60])
+def test_attention_value_scales_far_apart(pkg, cuda_device, fmt, rows, down):
+    """Values of the first 128 tokens 2^20 or 2^60 times smaller than the later
+    ones: rows that see only the first keep their precision, whether they run
+    beside rows that see the others or not."""
+    blk, D, L = 32, 64, 700
+    P = -(-L // blk)
+    c, _, _ = make_cache(pkg, P, 1, blk, D, fmt)
+    rk, rv = fill(c, 23)
+    tab = tables([L], blk, P, 10)
+    first = torch.from_numpy(tab[0, :128 // blk])
+    rv.scale[first] *= 2.0 ** -down
+    c.v_scale.copy_(rv.scale.float())
+    q = randn((L, 2, D), 42, torch.bfloat16)
+    got = c.attention(q.cuda(), i32(tab.tolist()), i32([L]), i32([0, L]), L)
+    few = torch.cat([c.attention(q[i:i + rows].cuda(), i32(tab.tolist()), i32([i + rows]), i32([0, rows]), rows)
+                     for i in range(0, 640, rows)])
+    for beg, end in ((0, 128), (128, 640)):
+        o, _, mag, smax, vsum = ref.attend(q[beg:end].double(), rk.tokens(tab[0], end), rv.tokens(tab[0], end),
+                                           torch.arange(beg, end), D ** -0.5, 0)
+        tol = ref.attend_tolerance(torch.bfloat16, o, mag, smax, vsum, D, L)
+        for x in (got, few):
+            assert bool(((x[beg:end].cpu().double() - o).abs() <= tol).all())
 
 
 @pytest.mark.parametrize("news", [1, 200])
