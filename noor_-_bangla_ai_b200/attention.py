@@ -84,6 +84,14 @@ def _ints(t, what: str, n: int, device: int) -> int:
     return t.data_ptr()
 
 
+def _no_grad(*tensors) -> None:
+    """The cache rounds to 8 bits and holds no graph: refuse what wants a gradient."""
+    if _T.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("the cached path has no gradient: call it under torch.no_grad() or detach its inputs")
+
+
 def _empty_like(t):
     """Contiguous output of t's shape."""
     return _T.empty_like(t, memory_format=_T.contiguous_format)
@@ -338,6 +346,7 @@ class KVCache:
         dt = _dtype_code(k)
         dev, D = self._dev, self.head_dim
         hk, hv = _heads(k, "k", dev, D), _heads(v, "v", dev, D)
+        _no_grad(k, v, q)
         rows = k.size(0)
         if k.size(1) != self.n_kv_heads or v.size(1) != self.n_kv_heads:
             raise ValueError(f"k and v must have {self.n_kv_heads} heads")
@@ -392,6 +401,7 @@ class KVCache:
         dt = _dtype_code(q)
         dev, D = self._dev, self.head_dim
         hq = _heads(q, "q", dev, D)
+        _no_grad(q, out)
         rows, nq = q.size(0), q.size(1)
         if nq % self.n_kv_heads != 0:
             raise ValueError(f"{nq} query heads over {self.n_kv_heads} kv heads")
@@ -410,10 +420,12 @@ class KVCache:
         if need is None:
             n = ctypes.c_int64()
             api.check(lib.noor_kv_attention_workspace(self._ref, batch, nq, max_rows, dt, ctypes.byref(n)))
+            if len(self._workspace) >= 1024:  # a server's prompts come in any number of rows
+                self._workspace.clear()
             need = self._workspace[key] = n.value
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         rc = lib.noor_kv_attention(self._ref, batch, hq, ho, lse.data_ptr() if return_lse else None, nq, max_rows,
-                                   D ** -0.5 if scale is None else scale, window, dt, ws.data_ptr(), need, _stream(dev))
+                                   D ** -0.5 if scale is None else scale, min(window, 2 ** 31 - 1), dt, ws.data_ptr(), need, _stream(dev))
         if rc:
             api.check(rc)
         return (out, lse) if return_lse else out

@@ -158,6 +158,17 @@ __device__ __forceinline__ void pair_sync(int pair) {
   asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory");
 }
 
+// After a wait gave up: the copies still in flight land before the block can
+// end (a stage without any only waits the limit out).
+static __device__ __noinline__ void drain(uint64_t* bars, int stages, uint32_t kphase, uint32_t vphase) {
+  const long long start = clock64();
+  for (int i = 0; i < 2 * stages; ++i) {
+    const uint32_t parity = ((i < stages ? kphase : vphase) >> (i % stages)) & 1;
+    while (!tc::mbar_try_wait(bars + i, parity) && clock64() - start < kWaitLimitCycles) {
+    }
+  }
+}
+
 // Pairs per block and shared memory: a ring of two tiles (k and v) for each
 // pair, and the query fragments where they do not fit into registers.
 template <int DP, int PARTS, int NB>
@@ -361,6 +372,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         if (clock64() - start > kWaitLimitCycles) {
           dead = true;
           kv::flag(a.c.status, NOOR_KV_TIMEOUT);
+          drain(bars, NST, kphase, vphase);
           break;
         }
       dead = __any_sync(0xffffffffu, dead);

@@ -459,6 +459,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     CKR(check_dtype(dtype));
     CKR(check_heads(c, q_heads));
     if (max_rows < 0 || window < 0) return fail(NOOR_MOE_ERR_INVALID, "negative max_rows or window");
+    if (window >= (int64_t)b->max_blocks * c->block) window = 0;  // longer than any sequence (positions less it stay in 32 bits)
     if (!std::isfinite(scale)) return fail(NOOR_MOE_ERR_INVALID, "scale is not finite");
     if (b->n_rows == 0) return NOOR_MOE_OK;
     CKR(check_view(q, dtype, "q"));

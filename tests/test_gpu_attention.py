@@ -733,3 +733,21 @@ def test_stack_served_from_the_cache(pkg, cuda_device):
     assert float((again[-1] - full[36]).norm() / full[36].norm()) <= 1e-4
     for b in st.blocks:
         b.parallel_ffn.moe.invalidate()
+
+
+def test_cached_path_refuses_gradients_and_takes_any_window(pkg, cuda_device):
+    c = pkg.attention.KVCache(4, 1, 16, 16)
+    x = torch.ones((1, 1, 16), device="cuda", requires_grad=True)
+    args = (i32([[2, 1, -1, -1]]), i32([20]), i32([0, 1]))
+    for call in (lambda: c.append(x, x.detach(), *args), lambda: c.append(x.detach(), x, *args), lambda: c.attention(x, *args, 1)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+    rk, rv = fill(c, 30)
+    want = c.attention(x.detach(), *args, 1)
+    with torch.no_grad():
+        for window in (20, 2 ** 31 - 1, 2 ** 31, 2 ** 40 + 5):
+            assert torch.equal(c.attention(x, *args, 1, window=window), want)
+        rows = torch.ones((20, 1, 16), device="cuda", dtype=torch.bfloat16)
+        many = c.attention(rows.repeat(1, 8, 1), args[0], args[1], i32([0, 20]), 20)
+        assert torch.equal(c.attention(rows.repeat(1, 8, 1), args[0], args[1], i32([0, 20]), 20, window=2 ** 31 - 1), many)
+    c.check()
