@@ -205,10 +205,10 @@ def test_append_and_read(pkg, cuda_device, fmt, dtype, H, D, blk, layout, rot):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
-@pytest.mark.parametrize("dtype,H,D,blk,layout", [("bf16", 2, 128, 64, "half"), ("f32", 1, 64, 16, "interleaved"),
-                                                  ("bf16", 1, 256, 32, "interleaved"), ("f32", 2, 144, 64, "half")])
+@pytest.mark.parametrize("dtype,H,D,blk,layout", [("bf16", 11, 128, 64, "half"), ("f32", 22, 64, 16, "interleaved"),
+                                                  ("bf16", 6, 256, 32, "interleaved"), ("f32", 10, 144, 64, "half")])
 def test_append_long_prompts(pkg, cuda_device, fmt, dtype, H, D, blk, layout):
-    """Prompts of more than a thousand rows, which keys, values and queries are
+    """Prompts of more than 1.5 M elements, which keys, values and queries are
     written for in a launch each: a fresh sequence, one that goes on inside a
     block with larger values, an idle one."""
     A = pkg.attention
@@ -221,7 +221,7 @@ def test_append_long_prompts(pkg, cuda_device, fmt, dtype, H, D, blk, layout):
     for si, n in enumerate(([5, 0, 0], [1100, 77, 0], [3, 13, 0])):
         N, cu = sum(n), np.concatenate([[0], np.cumsum(n)])
         k, v = randn((N, H, D), 50 + si, DT[dtype], 1.0 + si), randn((N, H, D), 60 + si, DT[dtype], 1.0 + si)
-        q = randn((N, 3 * H, D), 70 + si, DT[dtype])
+        q = randn((N, 2 * H, D), 70 + si, DT[dtype])
         lens = lens + np.array(n)
         pos = torch.tensor([p for b in range(3) for p in range(lens[b] - n[b], lens[b])], dtype=torch.int64)
         kr = ref.rotate(k, pos, inv, layout)
@@ -409,7 +409,7 @@ def test_attention_many_rows(pkg, cuda_device, D, blk, fmt, window):
 
 
 @pytest.mark.parametrize("D,blk,fmt", [(64, 64, "int8"), (128, 16, "e4m3"), (80, 32, "int8")])
-@pytest.mark.parametrize("lens,news", [([3000], [200]), ([2500, 1, 0, 70], [130, 1, 0, 33]), ([130], [130])])
+@pytest.mark.parametrize("lens,news", [([3000], [200]), ([2900, 40, 300], [8, 1, 7]), ([2500, 1, 0, 70], [130, 1, 0, 33]), ([130], [130])])
 def test_attention_many_rows_in_parts(pkg, cuda_device, D, blk, fmt, lens, news):
     """Few rows over a long context: the tensor-core kernel cuts the context and
     joins the parts.  Parts without a tile (the table has room for more than the
@@ -424,7 +424,7 @@ def test_attention_many_rows_in_parts(pkg, cuda_device, D, blk, fmt, lens, news)
         check_attention(pkg, c, rk, rv, tab, lens, news, 4, "bf16", window=window, seed=40 + window, qgain=2.0, strided=window == 90)
     q = randn((news[0], 4, D), 41, torch.bfloat16).cuda()
     bad = tab[:1].copy()
-    at = (lens[0] - news[0]) // blk + 1  # some rows see it, those before do not
+    at = (lens[0] - 1) // blk  # the last page: rows before it do not see it
     bad[0, at] = P + 5
     got, lse = c.attention(q, i32(bad.tolist()), i32(lens[:1]), cu_of(news[:1]), news[0], return_lse=True)
     with pytest.raises(RuntimeError, match="page"):
