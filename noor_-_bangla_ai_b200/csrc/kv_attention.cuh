@@ -27,6 +27,12 @@
 // scaled by 2^14 so that p down to 2^-38 counts in a long context.  A block's
 // v scale multiplies its p, relative to the largest scale so far.
 //
+// Measured at 32 / 8 heads of 128 dims: 64 ragged sequences of up to 8192
+// tokens, a row each, e4m3, 120 us = 5.6 TB/s of codes; 4 x 131072 tokens, int8,
+// 213 us = 5.0 TB/s.  int8 takes four instructions to widen a word where e4m3
+// takes two, and is bound by them; e4m3 by memory.  One stream of 1000 tokens
+// takes 14 us, the chain of its loads (lengths, page table, codes) and the join.
+//
 // The contraction index of an mma may be permuted at will if both operands
 // agree: thread c of a quad takes 16 consecutive bytes of a key row and feeds
 // them to four mma steps, so keys come straight from the stored layout with
@@ -719,7 +725,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 // part and 8 of its rows, a warp for each row.  The first pair's part may be
 // its last piece (slot 1); every later pair's is its first (slot 0).  A lane
 // weighs one part (32 at a time), then all lanes sum 4 dims each over the
-// parts, in the parts' order.
+// parts, in the parts' order.  Bound by latency: it adds some 4 us.
 constexpr int kJoinWarps = 8;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32, 4) combine_kernel(const Args a) {

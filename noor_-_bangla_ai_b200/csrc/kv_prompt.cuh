@@ -22,6 +22,11 @@
 // m is a reference that follows the row's maximum lazily: o is rescaled only
 // when the maximum has grown by more than 2^8, so most tiles never touch o.
 // p <= 2^15 then fits f16; shift 7 keeps p down to 2^-31 of the largest.
+//
+// Measured: 2 sequences of 2048 rows on 8192 tokens, 32 / 8 heads of 128 dims,
+// 549 us = 876 TFLOP/s of visible products.  Bound by the softmax warps: an
+// exponential, its scaling and the sums for each score, beside TMEM reads; the
+// tensor core waits for p.
 // A block's v scale is applied while widening, relative to the largest v scale
 // so far (exact for powers of two); o follows when that grows.
 #pragma once

@@ -146,8 +146,9 @@ int64_t most_tasks(const noor_kv_cache* c, const noor_kv_batch* b) {
 
 // kv heads that one grid block takes in turn, so that finding its place and
 // (for keys) the angles is paid for once: as many as leave eight blocks for
-// every SM, at most 8.  Against one head: 16384 rows of 8 kv heads written in
-// 145 us instead of 201, 120k tokens read back in 94 instead of 115.
+// every SM, at most 8.  Against one head, at 8 kv heads of 128
+// dims: 8 ragged prompts of up to 4096 tokens written in 145 us instead of 201,
+// 32 ragged prefixes of up to 4096 read back in 94 instead of 115.
 int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
@@ -378,12 +379,15 @@ int prompt_parts(int64_t units, int64_t tiles, int sms) {
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
 // have that many tiles.  Up to 8 query rows for a kv head use one column group
 // of the mma; more use as many as the registers hold, so that a tile's codes
-// are widened once for 32 rows (16 at more than 128 dims).
+// are widened once for 32 rows (16 at more than 128 dims).  16 sequences of
+// 4096 tokens, 16 / 4 heads: 2 rows 29 us with one group, 3 rows 55 us with
+// four.  Beside prompts, which go to the other kernel, the rest are taken to
+// have one row: a prompt of 256 beside 32 single rows 133 us, 173 with four.
 int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int window, int dtype, StreamPlan* p) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
   const int64_t g = Hq / c->n_kv_heads;
-  p->nb = max_rows * g <= 8 ? 1 : c->head_dim <= 128 ? 4 : 2;
+  p->nb = (prompt_fits(c, b, (int)g, max_rows, dtype) ? g : max_rows * g) <= 8 ? 1 : c->head_dim <= 128 ? 4 : 2;
   const int64_t R = 8 * p->nb;
   int per = 0;
   CKR(attn::by_shape(c->head_dim, p->nb, [&](auto dp, auto nb) -> int {
