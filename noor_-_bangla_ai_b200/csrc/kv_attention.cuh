@@ -70,12 +70,26 @@ struct Args {
   float* part_ml;
   int4* desc;      // [pairs] the cut unit that starts in a pair's share: (sequence or -1, head, row tile,
                    // last pair << 1 | slot of its part)
-  int32_t slots;   // 2: a pair's first and last piece
-  int32_t parts;   // tensor-core kernel: parts of a unit, each a block with one slot (it has no pairs)
-  int32_t pairs;   // warp pairs of the grid that share the work
+  int32_t slots;   // 2: a pair's first and last piece; tensor-core kernel 1: a block's part of a unit
+  int32_t pairs;   // warp pairs of the grid that share the work; tensor-core kernel: blocks with a slot (0: none)
+  int32_t sms, seen;  // tensor-core kernel: SMs, and most tiles of 128 tokens that a unit sees
   int32_t rows;    // query rows of a row tile
   int64_t min_e, max_e;  // sequences with min_e <= rows * g < max_e are this launch's
 };
+
+// Time of the tensor-core kernel's last SM with each unit cut in s parts, in
+// sixteenths of a tile of 128 tokens (2.2 us): a block's start and end cost some
+// six tiles, the join four.  BF16 over int8, 512 rows of 16 / 4 heads of
+// 128 dims: 8192 tokens 162 us whole, 81 us in four parts; 1024 tokens (1024
+// rows) 43 us whole, 49 us in two.
+__host__ __device__ inline int part_cost(int units, int tiles, int s, int sms) {
+  return (s * units + sms - 1) / sms * (16 * tiles / s + 96) + (s > 1 ? 64 : 0);
+}
+// Most parts: at least four tiles each, two blocks for an SM, a slot for each.
+__host__ __device__ inline int most_parts(int units, int tiles, int sms, int slots) {
+  const int blocks = 2 * sms < slots ? 2 * sms : slots, by_blocks = units > 0 ? blocks / units : 0;
+  return by_blocks < tiles / 4 ? by_blocks : tiles / 4;
+}
 
 // ------------------------------------------------------------ mma pieces
 

@@ -18,8 +18,8 @@ int launch(const Args& a, int blocks, cudaStream_t s) {
 
 template <int FMT>
 int by_dim(const Args& a, int blocks, cudaStream_t s) {
-  if (a.c.D <= 64) return a.parts > 1 ? launch<64, FMT, true>(a, blocks, s) : launch<64, FMT, false>(a, blocks, s);
-  return a.parts > 1 ? launch<128, FMT, true>(a, blocks, s) : launch<128, FMT, false>(a, blocks, s);
+  if (a.c.D <= 64) return a.pairs > 0 ? launch<64, FMT, true>(a, blocks, s) : launch<64, FMT, false>(a, blocks, s);
+  return a.pairs > 0 ? launch<128, FMT, true>(a, blocks, s) : launch<128, FMT, false>(a, blocks, s);
 }
 
 }  // namespace

@@ -3,7 +3,7 @@
 //
 // A block takes one unit: 256 rows (query row, query head of the group) of one
 // kv head, as two row tiles of 128, and their visible tokens in tiles of 128:
-// all of them, or one of `parts` equal runs where there are fewer units than
+// all of them, or one of several equal runs where there are fewer units than
 // SMs; combine_kernel then joins a unit's parts.  The same sums as the streamed kernel (kv_attention.cuh):
 //   s = q.k (f16 codes and f16 queries, f32 sums), p = 2^(s f - m + shift) in
 //   f16, o += p v, with f = scale log2(e) 2^e(row) k scale(block).
@@ -24,7 +24,7 @@
 // p <= 2^15 then fits f16; shift 7 keeps p down to 2^-31 of the largest.
 //
 // Measured: 2 sequences of 2048 rows on 8192 tokens, 32 / 8 heads of 128 dims,
-// 549 us = 876 TFLOP/s of visible products.  Bound by the softmax warps: an
+// 547 us = 880 TFLOP/s of visible products.  Bound by the softmax warps: an
 // exponential, its scaling and the sums for each score, beside TMEM reads; the
 // tensor core waits for p.
 // A block's v scale is applied while widening, relative to the largest v scale
@@ -115,7 +115,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
   return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
-// PARTS: whether units are cut (compiled apart: the tests cost registers, 8% of the time)
+// PARTS: whether units may be cut (compiled apart: the tests cost registers, 8% of the time)
 template <int DP, int FMT, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   using S = Smem<DP>;
@@ -136,7 +136,30 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   const int D = a.c.D, blk = a.c.blk;
 
   // ---- the block's unit: last row tiles first, they see the most tokens
-  const int parts = PARTS ? a.parts : 1;
+  // ---- parts of each unit, from the units that the batch has
+  int parts = 1;
+  if constexpr (PARTS) {
+    __shared__ int32_t s_units;
+    if (threadIdx.x == 0) s_units = 0;
+    __syncthreads();
+    int32_t n = 0;
+    for (int i = threadIdx.x; i < a.b.B; i += kThreads) n += attn::seq_work(a, i).rtiles;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0 && n > 0) atomicAdd(&s_units, n);
+    __syncthreads();
+    const int32_t units = s_units * a.c.H;
+    if (units < a.sms) {
+      const int most = attn::most_parts(units, a.seen, a.sms, a.pairs);
+      uint32_t best = 0xFFFFFFFFu;  // cost, then parts
+      for (int s = 2 + lane; s <= most; s += 32) {
+        const uint32_t cost = attn::part_cost(units, a.seen, s, a.sms);
+        best = min(best, min(cost, (1u << 22) - 1) << 10 | (uint32_t)s);
+      }
+      best = __reduce_min_sync(0xffffffffu, best);
+      if (best != 0xFFFFFFFFu && 20 * (best >> 10) < 19 * (uint32_t)attn::part_cost(units, a.seen, 1, a.sms)) parts = best & 1023;
+    }
+  }
+  const bool cut = PARTS && parts > 1;
   const int part = blockIdx.x % parts, unit = blockIdx.x / parts, h = unit % a.c.H;
   int sb = -1, rt = 0;
   {
@@ -160,8 +183,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
-  if (PARTS && threadIdx.x == 0)
-    a.desc[blockIdx.x] = make_int4(part == 0 ? sb : -1, h, rt, (int)(blockIdx.x + parts - 1) << 1);
+  // (row offsets that overlap may count more units than there are slots)
+  if (cut && (int64_t)unit * parts + parts > a.pairs) sb = -1;
+  if (PARTS && threadIdx.x == 0 && blockIdx.x < a.pairs)
+    a.desc[blockIdx.x] = make_int4(cut && part == 0 ? sb : -1, h, rt, (int)(blockIdx.x + parts - 1) << 1);
   if (sb < 0) return;
   const attn::SeqWork w = attn::seq_work(a, sb);
   const int e0 = 256 * rt, nrows = min(256, w.s.n * a.g - e0), nw = nrows > 128 ? 2 : 1;
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       if (ok) {
         const float vref = T > 0 ? s_vref[(T - 1) % kMeta] : 0.f;
         // a part leaves its sums as they are, with the reference of the join's shift
-        const float inv = PARTS ? vref : l == 0.f ? 0.f : 1.f / l * vref;
+        const float inv = cut ? vref : l == 0.f ? 0.f : 1.f / l * vref;
         const int64_t slot = (int64_t)blockIdx.x * 256 + 128 * wg + r;
         bf16* op = static_cast<bf16*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
         const bool ovec = (reinterpret_cast<uintptr_t>(a.out.p) | (uintptr_t)(a.out.st * 2) | (uintptr_t)(a.out.sh * 2)) % 16 == 0;
@@ -402,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           float z[16];
 #pragma unroll
           for (int x = 0; x < 16; ++x) z[x] = __uint_as_float(v[x]) * inv;
-          if constexpr (PARTS) {
+          if (cut) {
             if (live)
 #pragma unroll
               for (int x = 0; x < 16; x += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + c + x) = make_float4(z[x], z[x + 1], z[x + 2], z[x + 3]);
@@ -418,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           }
           __syncwarp();
         }
-        if (PARTS && live)
+        if (cut && live)
           *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m + (attn::kPShift - kShift), l);
         else if (live && a.lse != nullptr)
           a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * 0.69314718055994531f;

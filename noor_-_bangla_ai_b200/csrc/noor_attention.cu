@@ -342,7 +342,7 @@ namespace {
 
 struct StreamPlan {
   int grid = 0, pairs = 0, nb = 1;
-  int prompt = 0, parts = 1;  // units of the tensor-core kernel (0: not launched) and parts of each
+  int prompt = 0, slots = 0, seen = 0, sms = 0;  // tensor-core kernel: most units (0: not launched), slots of parts, Args
   int64_t off_ml = 0, off_desc = 0, off_prompt = 0, off_prompt_ml = 0, off_prompt_desc = 0, bytes = 0;
 };
 
@@ -358,22 +358,13 @@ bool prompt_fits(const noor_kv_cache* c, const noor_kv_batch* b, int g, int max_
          b->n_rows * g >= kPromptRows;
 }
 
-// Parts of each of the tensor-core kernel's units: those with the shortest time
-// for the last SM, in tiles of 128 tokens (2.2 us); a block's start and end cost
-// some six of them, the join four.  BF16 over int8, 512 rows of 16 / 4 heads of
-// 128 dims: 8192 tokens 162 us whole, 77 us in four parts; 1024 tokens (1024
-// rows) 43 us whole, 49 us in two.
-int prompt_parts(int64_t units, int64_t tiles, int sms) {
-  int best = 1;
-  double time = (double)((units + sms - 1) / sms) * (tiles + 6);
-  for (int s = 2; s <= tiles / 4 && s * units <= 2 * sms; ++s) {
-    const double t = (double)((s * units + sms - 1) / sms) * ((double)tiles / s + 6) + 4;
-    if (t < 0.95 * time) {
-      best = s;
-      time = t;
-    }
-  }
-  return best;
+// Whether that many of the tensor-core kernel's units are better cut (the
+// kernel counts the units that there are, and chooses the parts).
+bool cut_pays(int units, int tiles, int sms) {
+  const int64_t whole = attn::part_cost(units, tiles, 1, sms);
+  for (int s = 2; s <= attn::most_parts(units, tiles, sms, INT32_MAX); ++s)
+    if (20 * (int64_t)attn::part_cost(units, tiles, s, sms) < 19 * whole) return true;
+  return false;
 }
 
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
@@ -382,7 +373,7 @@ int prompt_parts(int64_t units, int64_t tiles, int sms) {
 // are widened once for 32 rows (16 at more than 128 dims).  16 sequences of
 // 4096 tokens, 16 / 4 heads: 2 rows 29 us with one group, 3 rows 55 us with
 // four.  Beside prompts, which go to the other kernel, the rest are taken to
-// have one row: a prompt of 256 beside 32 single rows 133 us, 173 with four.
+// have one row: a prompt of 256 beside 32 single rows gains 40 us of 173 by it.
 int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int window, int dtype, StreamPlan* p) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
@@ -409,8 +400,13 @@ int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_
     // a unit's rows see at most that many tiles
     int64_t seen = (tiles + 1) / 2;
     if (window > 0) seen = std::min(seen, ((int64_t)window + 256 / g) / 128 + 2);
-    p->parts = prompt_parts(units, seen, sms);
-    const int64_t n = p->parts > 1 ? units * p->parts : 0;
+    // The fewest units, were all rows prompts' but those of sequences just below
+    // the limit: where they would not be cut, none is.
+    const int64_t least = std::max<int64_t>((b->n_rows * g - (kPromptRows - 1) * b->batch) / 256, 1) * c->n_kv_heads;
+    p->sms = sms;
+    p->seen = (int)seen;
+    if (least < sms && cut_pays((int)least, (int)seen, sms)) p->slots = (int)std::min<int64_t>(2 * sms, units * (seen / 4));
+    const int64_t n = p->slots;
     p->off_prompt = (p->bytes + 15) / 16 * 16;
     p->off_prompt_ml = p->off_prompt + n * 256 * c->head_dim * 4;
     p->off_prompt_desc = p->off_prompt_ml + n * 256 * 2 * 4;
@@ -498,7 +494,6 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     a.window = window;
     a.pairs = p.pairs;
     a.slots = 2;
-    a.parts = 1;
     a.rows = 8 * p.nb;
     a.min_e = 0;
     a.max_e = INT64_MAX;
@@ -513,13 +508,15 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
       t.rows = 256;
       t.min_e = kPromptRows;
       t.slots = 1;
-      t.parts = p.parts;
-      const int64_t blocks = (int64_t)p.prompt * p.parts;
+      t.pairs = p.slots;
+      t.sms = p.sms;
+      t.seen = p.seen;
+      const int blocks = std::max(p.prompt, p.slots);
       t.part_o = reinterpret_cast<float*>(ws + p.off_prompt);
       t.part_ml = reinterpret_cast<float*>(ws + p.off_prompt_ml);
       t.desc = reinterpret_cast<int4*>(ws + p.off_prompt_desc);
-      CKR(c->format == NOOR_KV_INT8 ? attn::prompt_int8(t, (int)blocks, s) : attn::prompt_e4m3(t, (int)blocks, s));
-      if (p.parts > 1) CKR(launch_join<bf16>(t, (int)blocks, 256, s));
+      CKR(c->format == NOOR_KV_INT8 ? attn::prompt_int8(t, blocks, s) : attn::prompt_e4m3(t, blocks, s));
+      if (p.slots) CKR(launch_join<bf16>(t, p.slots, 256, s));
       a.max_e = kPromptRows;
     }
     if (dtype == NOOR_DTYPE_BF16)

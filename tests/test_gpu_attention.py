@@ -435,6 +435,28 @@ def test_attention_many_rows_in_parts(pkg, cuda_device, D, blk, fmt, lens, news)
     c.check()
 
 
+@pytest.mark.parametrize("L", [350, 5000])
+def test_overlapping_row_offsets_stay_in_bounds(pkg, cuda_device, L):
+    """Offsets that go back: one sequence is skipped, two share rows, and the
+    batch has more row tiles than its rows allow."""
+    blk, P = 64, -(-5000 // 64)
+    c, _, _ = make_cache(pkg, P, 1, blk, 64, "int8")
+    fill(c, 24)
+    q = torch.cat([randn((300, 4, 64), 43, torch.bfloat16), torch.full((40, 4, 64), 3.0, dtype=torch.bfloat16)]).cuda()
+    out = torch.full_like(q, 7.5)
+    tab = i32(np.broadcast_to(np.arange(P), (3, P)).tolist())
+    got = c.attention(q[:300], tab, i32([L] * 3), i32([0, 300, 100, 300]), 300, out=out[:300])
+    with pytest.raises(RuntimeError, match="offsets"):
+        c.check()
+    assert torch.all(out[300:] == 7.5) and torch.isfinite(got[:100]).all()
+    c.read(tab, None, i32([0, 300, 100, 300]), 300)
+    with pytest.raises(RuntimeError, match="offsets"):
+        c.check()
+    want = c.attention(q[:300], tab[:1], i32([L]), i32([0, 300]), 300)  # the cache still answers
+    assert torch.isfinite(want).all()
+    c.check()
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("rows", [16, 128])
 @pytest.mark.parametrize("down", [20, 60])
