@@ -18,7 +18,7 @@
 // for p v, head dims) as the 16 rows and 8 query rows as the columns: a decode
 // step has 1 to 8 query rows for a kv head, which tcgen05's 128-row tiles would
 // leave nearly empty, and at one pass per byte the tensor work is far below
-// the memory time.  More rows (NB = 4: 32) share each widened code.
+// the memory time.  F32 with many rows (NB = 4: 32) shares each widened code.
 // Codes (|int8| <= 127, e4m3) are exact in f16.  Queries are
 // scaled by a power of two for each row so that f16 holds them: exactly for BF16
 // (elements under 2^-38 of the row's largest aside), and for F32 as a sum of

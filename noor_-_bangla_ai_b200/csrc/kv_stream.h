@@ -10,19 +10,21 @@
 namespace noor {
 namespace attn {
 
-// Calls f(bound of head_dim, column groups) as integral constants.
-template <typename F>
+// Calls f(bound of head_dim, column groups) as integral constants.  BF16 (one
+// f16 part) up to 128 dims always has one group.
+template <int PARTS, typename F>
 int by_shape(int D, int nb, F&& f) {
   using std::integral_constant;
   using One = integral_constant<int, 1>;
-  if (D <= 64) return nb == 1 ? f(integral_constant<int, 64>{}, One{}) : f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  if (D <= 128) return nb == 1 ? f(integral_constant<int, 128>{}, One{}) : f(integral_constant<int, 128>{}, integral_constant<int, 4>{});
+  using More = integral_constant<int, PARTS == 1 ? 1 : 4>;
+  if (D <= 64) return nb == 1 ? f(integral_constant<int, 64>{}, One{}) : f(integral_constant<int, 64>{}, More{});
+  if (D <= 128) return nb == 1 ? f(integral_constant<int, 128>{}, One{}) : f(integral_constant<int, 128>{}, More{});
   return nb == 1 ? f(integral_constant<int, 256>{}, One{}) : f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
 }
 
 template <int FMT, int PARTS>
 int stream_launch(const Args& a, int nb, int grid, cudaStream_t s) {
-  return by_shape(a.c.D, nb, [&](auto dp, auto n) -> int {
+  return by_shape<PARTS>(a.c.D, nb, [&](auto dp, auto n) -> int {
     using Sh = Shape<dp(), PARTS, n()>;
     auto kern = stream_kernel<dp(), FMT, PARTS, n()>;
     const int smem = Sh::smem_bytes(a.c.D);

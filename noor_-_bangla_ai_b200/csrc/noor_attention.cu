@@ -347,10 +347,9 @@ struct StreamPlan {
 };
 
 // Rows (times query heads of a group) from which a sequence runs on the
-// tensor-core kernel.  4 kv heads of 128 dims, int8, groups of 4: 8 new rows
-// of 1 / 16 / 64 sequences of 4096 / 4096 / 2048 tokens take 27 / 65 / 96 us
-// there and 31 / 62 / 96 us on the streamed kernel, 4 rows 25 / 62 / 97 and
-// 27 / 55 / 88, 12 rows 27 / 78 / 97 and 32 / 86 / 147.
+// tensor-core kernel.  4 kv heads of 128 dims, int8, groups of 4, for 1 / 16 / 64
+// sequences of 4096 / 4096 / 2048 tokens: 4 new rows 25 / 62 / 97 us there and
+// 22 / 40 / 65 us on the streamed kernel, 7 rows 26 / 64 / 96 and 24 / 63 / 114.
 constexpr int64_t kPromptRows = 32;
 
 bool prompt_fits(const noor_kv_cache* c, const noor_kv_batch* b, int g, int max_rows, int dtype) {
@@ -368,23 +367,31 @@ bool cut_pays(int units, int tiles, int sms) {
 }
 
 // Grid of the streamed kernel: one block per SM, fewer where the batch cannot
-// have that many tiles.  Up to 8 query rows for a kv head use one column group
-// of the mma; more use as many as the registers hold, so that a tile's codes
-// are widened once for 32 rows (16 at more than 128 dims).  16 sequences of
-// 4096 tokens, 16 / 4 heads: 2 rows 29 us with one group, 3 rows 55 us with
-// four.  Beside prompts, which go to the other kernel, the rest are taken to
-// have one row: a prompt of 256 beside 32 single rows gains 40 us of 173 by it.
+// have that many tiles.  With one column group of the mma a row tile is 8 query
+// rows, and more rows read a tile's codes again (from L2); with as many as the
+// registers hold, codes are widened once for 32 rows (16 at more than 128 dims),
+// but a tile's chain is longer and less runs beside it.  16 sequences of 4096
+// tokens, 4 kv heads, one group / many: F32 at 128 dims 12 rows 41 / 69 us,
+// 48 rows 91 / 108, 64 rows 113 / 114; at 256 dims 12 rows 101 / 101, 32 rows
+// 177 / 154 (BF16 154 / 128).  BF16 up to 128 dims has the other kernel for
+// more rows.
 int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int window, int dtype, StreamPlan* p) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
   const int64_t g = Hq / c->n_kv_heads;
-  p->nb = (prompt_fits(c, b, (int)g, max_rows, dtype) ? g : max_rows * g) <= 8 ? 1 : c->head_dim <= 128 ? 4 : 2;
+  if (c->head_dim > 128)
+    p->nb = max_rows * g <= 8 ? 1 : 2;
+  else
+    p->nb = dtype == NOOR_DTYPE_BF16 || max_rows * g <= 48 ? 1 : 4;
   const int64_t R = 8 * p->nb;
   int per = 0;
-  CKR(attn::by_shape(c->head_dim, p->nb, [&](auto dp, auto nb) -> int {
-    per = dtype == NOOR_DTYPE_F32 ? attn::Shape<dp(), 2, nb()>::kPairs : attn::Shape<dp(), 1, nb()>::kPairs;
-    return NOOR_MOE_OK;
-  }));
+  auto pairs_of = [&](auto parts) {
+    return attn::by_shape<parts()>(c->head_dim, p->nb, [&](auto dp, auto nb) -> int {
+      per = attn::Shape<dp(), parts(), nb()>::kPairs;
+      return NOOR_MOE_OK;
+    });
+  };
+  CKR(dtype == NOOR_DTYPE_F32 ? pairs_of(std::integral_constant<int, 2>{}) : pairs_of(std::integral_constant<int, 1>{}));
   const int64_t rtiles = std::min(b->n_rows * g, b->n_rows * g / R + b->batch);
   const int64_t tiles = ((int64_t)b->max_blocks * c->block + attn::kTile - 1) / attn::kTile;
   const double most = (double)rtiles * c->n_kv_heads * tiles;
