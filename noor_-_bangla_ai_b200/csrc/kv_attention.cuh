@@ -28,9 +28,10 @@
 // v scale multiplies its p, relative to the largest scale so far.
 //
 // Measured at 32 / 8 heads of 128 dims: 64 ragged sequences of up to 8192
-// tokens, a row each, e4m3, 120 us = 5.6 TB/s of codes; 4 x 131072 tokens, int8,
-// 213 us = 5.0 TB/s.  int8 takes four instructions to widen a word where e4m3
-// takes two, and is bound by them; e4m3 by memory.  One stream of 1000 tokens
+// tokens, a row each, e4m3, 120-124 us = 5.5 TB/s of codes; 4 x 131072 tokens,
+// int8, 213-218 us = 5.0 TB/s.  int8 takes five instructions to widen a word, e4m3
+// two: e4m3 is bound by memory, int8 by its pairs' chains (0.47 instructions a
+// cycle and scheduler, between waits on shared loads and fixed latencies).  One stream of 1000 tokens
 // takes 14 us, the chain of its loads (lengths, page table, codes) and the join.
 //
 // The contraction index of an mma may be permuted at will if both operands
