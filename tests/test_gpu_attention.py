@@ -773,3 +773,37 @@ def test_cached_path_refuses_gradients_and_takes_any_window(pkg, cuda_device):
         many = c.attention(rows.repeat(1, 8, 1), args[0], args[1], i32([0, 20]), 20)
         assert torch.equal(c.attention(rows.repeat(1, 8, 1), args[0], args[1], i32([0, 20]), 20, window=2 ** 31 - 1), many)
     c.check()
+
+
+def test_one_graph_serves_changing_prompts(pkg, cuda_device):
+    """The kernels cut contexts by what the device metadata says at replay: one
+    captured call over prompts, single rows and idle sequences as they change,
+    beside the same call on another stream."""
+    blk, P = 32, 3 * (2000 // 32 + 1)
+    c, _, _ = make_cache(pkg, P, 1, blk, 64, "int8")
+    fill(c, 26)
+    tab = i32(np.arange(P).reshape(3, -1).tolist())
+    q = randn((216, 4, 64), 45, torch.bfloat16).cuda()
+    lens, cu = i32([2000, 300, 5]), i32([0, 200, 215, 216])
+    out = torch.empty_like(q)
+    call = lambda out=None: c.attention(q, tab, lens, cu, 216, out=out)
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    side = torch.cuda.Stream()
+    for new_lens, new_cu in (([2000, 300, 5], [0, 200, 215, 216]), ([216, 2000, 2000], [0, 216, 216, 216]),
+                             ([2000, 1999, 1], [0, 1, 2, 3]), ([700, 2000, 40], [0, 8, 176, 216])):
+        lens.copy_(i32(new_lens))
+        cu.copy_(i32(new_cu))
+        out.fill_(7.5)
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            other = call()
+        torch.cuda.current_stream().wait_stream(side)
+        other.record_stream(torch.cuda.current_stream())
+        n = new_cu[-1]
+        assert torch.equal(out[:n], other[:n]) and torch.all(out[n:] == 7.5) and torch.isfinite(out).all()
+        assert torch.equal(call()[:n], out[:n])
+    c.check()
