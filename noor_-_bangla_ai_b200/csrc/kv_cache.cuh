@@ -322,7 +322,9 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
   auto dim0 = [&](int p) { return half && 2 * p < rot ? p : 2 * p; };
   auto dim1 = [&](int p) { return half && 2 * p < rot ? p + (rot >> 1) : 2 * p + 1; };
   const int d0 = dim0(2 * qd), d1 = dim1(2 * qd), d2 = dim0(2 * qd + 1), d3 = dim1(2 * qd + 1);
-  const bool split = d2 == d0 + 1 && d3 == d1 + 1;                  // two runs of two
+  // two runs of two, each on an even element: a half layout with an odd rot / 2
+  // starts the second on an odd one, which a two-element access must not touch
+  const bool split = d2 == d0 + 1 && d3 == d1 + 1 && (d1 & 1) == 0;
   const bool run = d1 == d0 + 1 && d2 == d0 + 2 && d3 == d0 + 3;    // one run of four
   // first angle and step of both pairs
   double c0[2] = {1.0, 1.0}, s0[2] = {0.0, 0.0}, cg[2] = {1.0, 1.0}, sg[2] = {0.0, 0.0};
@@ -420,7 +422,7 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
       uint8_t* o = kc + (k.first + s) * D;
       if (run) {
         *reinterpret_cast<uint32_t*>(o + d0) = e | (f << 16);
-      } else if (split && d1 % 2 == 0) {
+      } else if (split) {
         *reinterpret_cast<uint16_t*>(o + d0) = (uint16_t)((e & 0xFF) | ((f & 0xFF) << 8));
         *reinterpret_cast<uint16_t*>(o + d1) = (uint16_t)((e >> 8) | (f & 0xFF00));
       } else {

@@ -235,6 +235,39 @@ def test_append_long_prompts(pkg, cuda_device, fmt, dtype, H, D, blk, layout):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rot", [2, 6, 18, 50])
+@pytest.mark.parametrize("H,n", [(2, [5, 70, 0]), (17, [900, 600, 1])])
+def test_append_half_layout_with_an_odd_half(pkg, cuda_device, fmt, dtype, rot, H, n):
+    """rotate_dim / 2 odd in the half layout: the second elements of the pairs
+    begin on an odd one, in one launch and in a launch each for q, k and v."""
+    A = pkg.attention
+    D, blk = 64, 32
+    lens_max = [x + 3 for x in n]
+    P = sum(-(-x // blk) for x in lens_max)
+    c, rk, rv = make_cache(pkg, P, H, blk, D, fmt)
+    tab = tables(lens_max, blk, P, 12)
+    inv, _ = A.rotary_frequencies(D, 10000.0, (rot + 0.5) / D)
+    assert inv.size == rot // 2
+    r, inv = A.Rotary(inv, "half"), torch.from_numpy(inv)
+    lens = np.zeros(3, int)
+    for si, m in enumerate((n, [3, 0, 2])):
+        N, cu = sum(m), np.concatenate([[0], np.cumsum(m)])
+        k, v = randn((N, H, D), 80 + si, DT[dtype], 1.0 + si), randn((N, H, D), 90 + si, DT[dtype], 1.0 + si)
+        q = randn((N, H, D), 95 + si, DT[dtype])
+        lens = lens + np.array(m)
+        pos = torch.tensor([p for b in range(3) for p in range(lens[b] - m[b], lens[b])], dtype=torch.int64)
+        kr = ref.rotate(k, pos, inv, "half")
+        for b in range(3):
+            rk.append(kr, int(cu[b]), m[b], int(lens[b]), tab[b])
+            rv.append(v.double(), int(cu[b]), m[b], int(lens[b]), tab[b])
+        q_out = c.append(k.cuda(), v.cuda(), i32(tab.tolist()), i32(lens.tolist()), cu_of(m), rotary=r, q=q.cuda())
+        c.check()
+        cache_equal(c, rk, rv, [(tab[b], int(lens[b])) for b in range(3)], blk)
+        check_rope(q_out, q, pos, inv, "half", 1.0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_append_values_at_the_edges(pkg, cuda_device, fmt):
     """Zeros, subnormals, values at the scale's border, the largest floats, and
     values that are not finite; a poisoned block reads NaN until it starts over."""
