@@ -386,17 +386,20 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         bulk_load(s_v + stage * vbytes + lane * (bytes + 2 * blk), a.c.v + ph, bytes, bars + NST + stage);
       }
     };
+    // Each lane waits for itself; the warp votes once all its lanes are back (a
+    // barrier's test may answer them differently).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (dead || tc::mbar_try_wait(bar, parity)) return;
-      const long long start = clock64();
-      while (!tc::mbar_try_wait(bar, parity))
-        if (clock64() - start > kWaitLimitCycles) {
-          dead = true;
-          kv::flag(a.c.status, NOOR_KV_TIMEOUT);
-          drain(bars, NST, kphase, vphase);
-          break;
-        }
-      dead = __any_sync(0xffffffffu, dead);
+      bool gave_up = false;
+      if (!dead && !tc::mbar_try_wait(bar, parity)) {
+        const long long start = clock64();
+        while (!gave_up && !tc::mbar_try_wait(bar, parity))
+          if (clock64() - start > kWaitLimitCycles) {
+            gave_up = true;
+            kv::flag(a.c.status, NOOR_KV_TIMEOUT);
+            drain(bars, NST, kphase, vphase);
+          }
+      }
+      if (__any_sync(0xffffffffu, gave_up)) dead = true;
     };
 
     if (half == 0) {

@@ -132,3 +132,23 @@ def test_rotary_tables(pkg):
     for bad in (dict(linear=2.0, ntk=2.0), dict(linear=0.0), dict(yarn={"scale": -1.0, "original": 8})):
         with pytest.raises(ValueError):
             A.rotary_frequencies(64, **bad)
+
+
+# ---- what no run can show: rules of the memory model and of warp votes, read from the sources
+
+
+def _source(name):
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "noor_-_bangla_ai_b200", "csrc", name)) as f:
+        return f.read()
+
+
+def test_streamed_wait_votes_with_all_its_lanes():
+    """A barrier's test may answer the lanes of a warp differently, so no lane
+    leaves the wait before the warp's vote."""
+    s = _source("kv_attention.cuh")
+    body = s[s.index("auto wait = [&]"):]
+    body = body[:body.index("    };")]
+    assert "mbar_try_wait" in body and "return" not in body
+    assert body.rstrip().splitlines()[-1].strip().startswith("if (__any_sync(0xffffffffu")
