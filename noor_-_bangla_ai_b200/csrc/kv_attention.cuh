@@ -749,7 +749,7 @@ template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32, 4) combine_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (launched while the streamed kernel still runs)
   const int wid = blockIdx.x, lane = threadIdx.x & 31;
-  const int4 d = __ldg(a.desc + wid);
+  const int4 d = a.desc[wid];  // (written while this grid waits: not a read-only load)
   if (d.x < 0) return;
   const int r = min(blockIdx.y * kJoinWarps + (threadIdx.x >> 5), (unsigned)a.rows - 1u);
   const int D = a.c.D, parts = (d.w >> 1) - wid + 1;

@@ -367,7 +367,7 @@ __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, 
     const int h = hb + hl;
     const bool live = thread_live && h < h1;
     const int64_t ph = k.page * c.H + (live ? h : hb);
-    const float s_old = k.first > 0 ? __ldg(c.ks + ph) : 0.f;
+    const float s_old = k.first > 0 ? c.ks[ph] : 0.f;  // (rewritten below: not a read-only load)
     float4 x[TPT];
 #pragma unroll
     for (int j = 0; j < TPT; ++j) {
@@ -512,7 +512,7 @@ __device__ void append_values(const AppendArgs& a, const Task& k, int h0, int h1
     const int h = hb + hl;
     const bool live = hl < at_once && h < h1;
     const int64_t ph = k.page * c.H + (live ? h : hb);
-    const float s_old = k.first > 0 ? __ldg(c.vs + ph) : 0.f;
+    const float s_old = k.first > 0 ? c.vs[ph] : 0.f;  // (rewritten below: not a read-only load)
     uint8_t* vc = c.v + ph * blk * D + (int64_t)d * blk + lo;
     uint32_t x[16][W], amax = 0;
 #pragma unroll

@@ -152,3 +152,15 @@ def test_streamed_wait_votes_with_all_its_lanes():
     body = body[:body.index("    };")]
     assert "mbar_try_wait" in body and "return" not in body
     assert body.rstrip().splitlines()[-1].strip().startswith("if (__any_sync(0xffffffffu")
+
+
+def test_what_a_running_grid_writes_is_not_loaded_as_read_only():
+    """The read-only path wants data that no resident grid writes: the join waits
+    for a grid that writes its parts' list, and the write replaces the scales
+    that it reads."""
+    join = _source("kv_attention.cuh")
+    join = join[join.index("combine_kernel(const Args a) {"):]
+    assert "a.desc" in join and not [w for w in ("desc", "part_ml", "part_o") if f"__ldg(a.{w}" in join]
+    write = _source("kv_cache.cuh")
+    write = write[write.index("void append_keys"):write.index("// Rotate q_tok rows")]
+    assert "c.ks[" in write and "c.vs[" in write and not [w for w in "kv" if f"__ldg(c.{w}" in write]

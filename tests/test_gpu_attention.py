@@ -268,6 +268,22 @@ def test_append_half_layout_with_an_odd_half(pkg, cuda_device, fmt, dtype, rot, 
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_append_grows_a_scale_with_every_token(pkg, cuda_device, fmt):
+    """Token after token of twice the size: every write reads the scale that the
+    one before left, and rounds all earlier codes again."""
+    D, blk, H = 48, 32, 3
+    c, rk, rv = make_cache(pkg, 2, H, blk, D, fmt)
+    tab = i32([[1, 0]])
+    for n in range(1, 41):
+        k, v = (randn((1, H, D), 200 * i + n, torch.bfloat16, 2.0 ** (n % 33)) for i in (1, 2))
+        rk.append(k.double(), 0, 1, n, [1, 0])
+        rv.append(v.double(), 0, 1, n, [1, 0])
+        c.append(k.cuda(), v.cuda(), tab, i32([n]), i32([0, 1]))
+    cache_equal(c, rk, rv, [([1, 0], 40)], blk)
+    c.check()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_append_values_at_the_edges(pkg, cuda_device, fmt):
     """Zeros, subnormals, values at the scale's border, the largest floats, and
     values that are not finite; a poisoned block reads NaN until it starts over."""
