@@ -155,16 +155,16 @@ struct SeqWork {
 __device__ __forceinline__ SeqWork seq_work(const Args& a, int i) {
   SeqWork w;
   w.s = kv::sequence(a.b, a.b.cu, a.b.lens, a.c.blk, i, a.c.status);
-  if (w.s.n > 0 && w.s.len < w.s.n) kv::flag(a.c.status, NOOR_KV_BAD_LENGTH);
+  if (w.s.len < w.s.n) {  // skipped, as the write does
+    kv::flag(a.c.status, NOOR_KV_BAD_LENGTH);
+    w.s.n = 0;
+  }
   const int64_t e = (int64_t)w.s.n * a.g;
   if (e < a.min_e || e >= a.max_e) w.s.n = 0;
   w.rtiles = (int)(((int64_t)w.s.n * a.g + a.rows - 1) / a.rows);
-  // rows at negative positions see nothing; at least one tile, so that rows
-  // which see nothing are written too
-  const int32_t p0 = max(w.s.len - w.s.n, 0);
-  const int32_t lo = a.window > 0 ? max(p0 - a.window, 0) : 0;
+  const int32_t lo = a.window > 0 ? max(w.s.len - w.s.n - a.window, 0) : 0;
   w.t0 = lo / kTile;
-  w.tiles = max((w.s.len + kTile - 1) / kTile - w.t0, 1);
+  w.tiles = (w.s.len + kTile - 1) / kTile - w.t0;  // at least one if it has rows: a row sees itself
   return w;
 }
 

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   const int pos0 = w.s.len - w.s.n;
   const int p_first = pos0 + e0 / a.g, p_last = pos0 + (e0 + nrows - 1) / a.g;
   const int lo_tok = a.window > 0 ? max(p_first - a.window, 0) : 0, hi_tok = p_last + 1;
-  const int first = lo_tok / kTok, count = max((hi_tok + kTok - 1) / kTok - first, 0);
+  const int first = lo_tok / kTok, count = (hi_tok + kTok - 1) / kTok - first;
   const int tb = first + (int)((int64_t)count * part / parts);
   const int T = first + (int)((int64_t)count * (part + 1) / parts) - tb;
   const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;

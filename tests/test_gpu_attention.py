@@ -613,6 +613,28 @@ def test_bad_metadata_is_reported_and_touches_nothing(pkg, cuda_device):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,L", [(3, 2), (3, 0), (90, 89), (300, 40)])
+@pytest.mark.parametrize("window", [0, 5])
+def test_attention_skips_a_sequence_shorter_than_its_rows(pkg, cuda_device, dtype, n, L, window):
+    """Rows that would lie before the sequence's first token: the sequence is
+    skipped and reported, its rows stay as they were, the others are answered."""
+    blk, D = 32, 64
+    c, _, _ = make_cache(pkg, 24, 1, blk, D, "int8")
+    fill(c, 38)
+    tab = i32(np.arange(24).reshape(2, 12).tolist())
+    q = randn((n + 7, 4, D), 39, DT[dtype]).cuda()
+    out = torch.full_like(q, 7.5)
+    c.attention(q, tab, i32([L, 200]), i32([0, n, n + 7]), n, window=window, out=out)
+    with pytest.raises(pkg.api.NoorMoEError, match="length"):
+        c.check()
+    assert torch.all(out[:n] == 7.5)
+    want = c.attention(q[n:], tab[1:], i32([200]), i32([0, 7]), n, window=window)
+    # the other's context is cut elsewhere beside it: f32 sums in another order, then one rounding
+    assert float((out[n:].float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+    c.check()
+
+
 def test_attention_in_place_and_shared_pages(pkg, cuda_device):
     """out may be q; sequences may share pages (a common prefix)."""
     blk, D = 16, 48
