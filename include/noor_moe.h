@@ -359,8 +359,10 @@ NOOR_MOE_API int noor_rope_apply(const noor_rotary* r, const noor_heads* q, cons
  * k_scale / v_scale [num_blocks][n_kv_heads] f32; value = code * scale.
  * noor_kv_append chooses the scale as the smallest power of two (at least
  * 2^-126) that holds the block's largest magnitude, so growing it later is an
- * exact shift.  block 16, 32 or 64; head_dim a multiple of 16 up to 256; the
- * four arrays 16-byte aligned.
+ * exact shift.  A scale that is negative, not finite or above 2^126 (noor_kv_append
+ * leaves none but NaN) reads as NaN.  Written tokens' codes must be numbers: an
+ * e4m3 code of NaN may reach rows that do not see its token.  block 16, 32 or
+ * 64; head_dim a multiple of 16 up to 256; the four arrays 16-byte aligned.
  * status (one device int32, zero at first, nullable) takes the first mistake
  * that a kernel found in device metadata: NOOR_KV_BAD_*. */
 typedef struct {

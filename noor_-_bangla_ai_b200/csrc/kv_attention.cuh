@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
           ks = vs = nan;
         } else {
           const int64_t ph = (int64_t)pg * a.c.H + h;
-          ks = __ldg(a.c.ks + ph);
-          vs = __ldg(a.c.vs + ph);
+          ks = kv::read_scale(__ldg(a.c.ks + ph));
+          vs = kv::read_scale(__ldg(a.c.vs + ph));
         }
       }
     };
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       }
       // ---- scale, mask, running maximum
       float alpha[NB][2], mref[NB][2];
-      const float vmax = fmaxf(fabsf(vs), __shfl_xor_sync(0xffffffffu, fabsf(vs), 16));
+      const float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 16));
       const float vnew = fmaxf(vref, vmax);
       const float vstep = vref / vnew, vrel = vs / vnew;
       vref = vnew;

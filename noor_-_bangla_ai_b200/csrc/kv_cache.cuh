@@ -174,15 +174,22 @@ __device__ __forceinline__ float scale_for(uint32_t amax_bits) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// A scale as readers take it: one that the write cannot have left (negative,
+// not finite, or above 2^126, beyond which its reciprocal is no normal float)
+// reads as NaN, so that it reaches the rows that see its block and no others.
+constexpr float kMostScale = 8.5070592e37f;
+__device__ __forceinline__ float read_scale(float s) {
+  return s >= 0.f && s <= kMostScale ? s : __uint_as_float(0x7FC00000u);
+}
+
 // The scale of a block that held tokens at s_old and now needs s_new: the
 // larger, as a power of two; NaN stays.  (A poisoned block's codes are stored
 // as zeros: a reader's zero weight times any stored code is zero.)
 __device__ __forceinline__ float grown_scale(float s_old, float s_new) {
-  if (!(s_old > 0.f)) return s_old == 0.f ? s_new : __uint_as_float(0x7FC00000u);
+  if (s_old == 0.f) return s_new;
+  if (!(s_old > 0.f && s_old <= kMostScale) || s_new != s_new) return __uint_as_float(0x7FC00000u);
   uint32_t b = __float_as_uint(s_old);
-  if (b >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
   if (b & 0x7FFFFFu) b = (b & 0x7F800000u) + 0x800000u;  // a scale not written here: up to a power of two
-  if (b >= 0x7F800000u || s_new != s_new) return __uint_as_float(0x7FC00000u);
   return fmaxf(__uint_as_float(b), s_new);
 }
 
@@ -746,7 +753,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
     for (int i = tid; i < nh * per; i += kReadThreads) {
       const int hl = i / per, j = i - hl * per, s = j / pieces, d = (j - s * pieces) * 16;
       const uint4 w = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(kc + hl * head + s * D + d));
-      const float ks = bad ? nan : __ldg(c.ks + ph0 + hl);
+      const float ks = bad ? nan : read_scale(__ldg(c.ks + ph0 + hl));
       const float4 v[4] = {values4<FMT>(w.x, ks), values4<FMT>(w.y, ks), values4<FMT>(w.z, ks), values4<FMT>(w.w, ks)};
       store16(ko + s * row + hl * D + d, v);
     }
@@ -761,7 +768,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         w[x] = bad ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(vc + hl * head + (int64_t)(d + x) * blk + lo));
-      const float vs = bad ? nan : __ldg(c.vs + ph0 + hl);
+      const float vs = bad ? nan : read_scale(__ldg(c.vs + ph0 + hl));
       T* o = vo + hl * D + d;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {

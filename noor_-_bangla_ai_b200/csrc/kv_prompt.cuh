@@ -645,12 +645,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       const int64_t ph = (int64_t)page * a.c.H + h;
       // factors of each 16 tokens: NaN where the page or its values cannot be
       // read (the rows that see them come out NaN), values then zero
-      float ks = page >= 0 ? __ldg(a.c.ks + ph) : nan, vs = page >= 0 ? __ldg(a.c.vs + ph) : nan;
+      float ks = page >= 0 ? kv::read_scale(__ldg(a.c.ks + ph)) : nan, vs = page >= 0 ? kv::read_scale(__ldg(a.c.vs + ph)) : nan;
       const int src = (16 * (lane & 7)) / blk;
       ks = __shfl_sync(0xffffffffu, ks, src);
       vs = __shfl_sync(0xffffffffu, vs, src);
-      const bool fin = fabsf(vs) <= 3.4028235e38f;
-      const float vnew = fmaxf(vref, __uint_as_float(__reduce_max_sync(0xffffffffu, fin ? __float_as_uint(fabsf(vs)) : 0u)));
+      const bool fin = vs == vs;
+      const float vnew = fmaxf(vref, __uint_as_float(__reduce_max_sync(0xffffffffu, fin ? __float_as_uint(vs) & 0x7FFFFFFFu : 0u)));
       ok = wait(&bar.raw_empty[0], (i & 1) ^ 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;

@@ -578,6 +578,44 @@ def test_attention_masked_blocks_may_hold_anything(pkg, cuda_device, news, fmt):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("news,blk,window", [(300, 64, 0), (300, 16, 90), (9, 16, 0), (9, 16, 3), (8, 32, 0)])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_scales_that_no_write_leaves_read_as_nan(pkg, cuda_device, dtype, news, blk, window, which):
+    """A negative, infinite or too large scale spoils the rows that see its
+    block, and no row beside them; reading the block back gives NaN."""
+    D, L = 64, 300 if news == 300 else 70
+    c, _, _ = make_cache(pkg, 20, 1, blk, D, "int8")
+    rk, rv = fill(c, 44)
+    at = 64 // blk  # the block of token 64
+    q = randn((news, 4, D), 46, DT[dtype])
+    args = (i32([list(range(20))]), i32([L]), i32([0, news]), news)
+    pos = torch.arange(L - news, L)
+    o, _, mag, smax, vsum = ref.attend(q.double(), rk.tokens(range(20), L), rv.tokens(range(20), L), pos, D ** -0.5, window)
+    tol = ref.attend_tolerance(DT[dtype], o, mag, smax, vsum, D, L)
+    sees = (pos >= 64) & ((pos - window <= 64 + blk - 1) | (window == 0))
+    assert bool(sees.any()) and not bool(sees.all())
+    scale = getattr(c, which)
+    keep = float(scale[at, 0])
+    for bad in (-keep, -math.inf, math.inf, 2.0 ** 127, math.nan):
+        scale[at, 0] = bad
+        got = c.attention(q.cuda(), *args, window=window).cpu().double()
+        assert torch.isnan(got[sees]).all(), bad
+        assert bool(((got - o).abs() <= tol)[~sees].all()), bad
+        gk, gv = c.read(args[0], None, i32([0, 70]), 70, dtype=DT[dtype])
+        x, y = (gk, gv) if which == "k_scale" else (gv, gk)
+        assert torch.isnan(x[64:64 + blk]).all() and torch.isfinite(x[:64]).all() and torch.isfinite(y).all()
+        if blk * at < 70 < blk * (at + 1):  # a write into the block keeps it spoilt
+            one = torch.ones((1, 1, D), device="cuda")
+            c.append(one, one, args[0], i32([71]), i32([0, 1]))
+            assert math.isnan(float(scale[at, 0]))
+            c.k_codes.view(torch.uint8).copy_(rk.vals.to(c.k_codes.dtype).cuda().view(torch.uint8))
+            c.v_codes.view(torch.uint8).copy_(rv.vals.transpose(2, 3).contiguous().to(c.k_codes.dtype).cuda().view(torch.uint8))
+            c.k_scale.copy_(rk.scale.float())
+            c.v_scale.copy_(rv.scale.float())
+    c.check()
+
+
 def test_bad_metadata_is_reported_and_touches_nothing(pkg, cuda_device):
     D, blk = 64, 32
     c, _, _ = make_cache(pkg, 6, 1, blk, D, "int8")
