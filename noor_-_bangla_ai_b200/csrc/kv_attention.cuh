@@ -424,7 +424,9 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       // 2^e <= mx < 2^(e + 1) becomes 2^14: up = 2^(14 - e), within f32's exponents
       const int ex = max(min((int)(__float_as_uint(mx) >> 23) - 127, 127), -112);
       const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
-      const float down = a.scale2 * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
+      // (an infinite element's scores would be infinities, and a row with none above
+      // -inf would look like one that sees nothing: they are NaN)
+      const float down = mx <= 3.4028235e38f ? a.scale2 * __uint_as_float((uint32_t)(ex - 14 + 127) << 23) : nan;
       qfac[nb][0] = __shfl_sync(0xffffffffu, down, 8 * qc);
       qfac[nb][1] = __shfl_sync(0xffffffffu, down, 8 * qc + 4);
 #pragma unroll

@@ -276,9 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       for (int d = 0; d < DP / 8; ++d)
         mb = __vmaxu2(mb, __vmaxu2(__vmaxu2(qr[d].x & 0x7FFF7FFFu, qr[d].y & 0x7FFF7FFFu),
                                    __vmaxu2(qr[d].z & 0x7FFF7FFFu, qr[d].w & 0x7FFF7FFFu)));
-      const int ex = max(min((int)(max(mb & 0x7FFF0000u, mb << 16) >> 23) - 127, 127), -112);
+      const uint32_t mx = max(mb & 0x7FFF0000u, mb << 16);
+      const int ex = max(min((int)(mx >> 23) - 127, 127), -112);
       float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
-      const float fac = fabsf(a.scale2) * __uint_as_float((uint32_t)(ex - 14 + 127) << 23);
+      // (NaN where an element is not finite, as in the streamed kernel)
+      const float fac = mx < 0x7F800000u ? fabsf(a.scale2) * __uint_as_float((uint32_t)(ex - 14 + 127) << 23)
+                                         : __uint_as_float(0x7FC00000u);
       if (a.scale2 < 0.f) up = -up;
 #pragma unroll
       for (int d = 0; d < DP / 8; ++d) {

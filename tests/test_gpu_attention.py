@@ -616,6 +616,32 @@ def test_scales_that_no_write_leaves_read_as_nan(pkg, cuda_device, dtype, news, 
     c.check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("news", [1, 7, 200])
+@pytest.mark.parametrize("D,blk", [(64, 16), (128, 64), (144, 32)])
+def test_queries_that_are_not_finite(pkg, cuda_device, dtype, news, D, blk):
+    """An infinity or a NaN in a query makes its row NaN, whatever the keys (also
+    where all scores are minus infinity), and no row beside it."""
+    L, P = 260, -(-260 // blk)
+    c, _, _ = make_cache(pkg, P, 1, blk, D, "int8")
+    fill(c, 47)
+    c.k_codes.copy_(torch.where(c.k_codes == 0, torch.ones_like(c.k_codes), c.k_codes))
+    c.k_codes[..., 5] = -3  # an infinite query element 5 has scores of minus infinity
+    q = randn((news, 4, D), 48, DT[dtype])
+    args = (i32([list(range(P))]), i32([L]), i32([0, news]), news)
+    want, lse = c.attention(q.cuda(), *args, return_lse=True)
+    assert torch.isfinite(want).all() and torch.isfinite(lse).all()
+    for bad in (math.inf, -math.inf, math.nan):
+        x = q.clone()
+        x[news // 2, 1, 5] = bad
+        got, gl = c.attention(x.cuda(), *args, return_lse=True)
+        hit = torch.zeros((news, 4), dtype=torch.bool, device="cuda")
+        hit[news // 2, 1] = True
+        assert torch.isnan(got[hit]).all() and torch.isnan(gl[hit]).all(), bad
+        assert torch.equal(got[~hit], want[~hit]) and torch.equal(gl[~hit], lse[~hit])
+    c.check()
+
+
 def test_bad_metadata_is_reported_and_touches_nothing(pkg, cuda_device):
     D, blk = 64, 32
     c, _, _ = make_cache(pkg, 6, 1, blk, D, "int8")
