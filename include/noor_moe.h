@@ -429,9 +429,9 @@ NOOR_MOE_API int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, co
  * that sees nothing gets zeros.  q, out [n_rows][q_heads] (they may be the
  * same); lse [n_rows][q_heads] f32 contiguous, nullable: the natural
  * logarithm of the sum of exponentials, -inf for a row that sees nothing.
- * Values are held in f16 relative to the largest v scale among the
- * tokens met so far by the rows computed together: blocks whose scale is
- * below 2^-24 of it lose bits.
+ * Values are held in f16 relative to the largest v scale among the tokens that
+ * the row itself sees: blocks whose scale is below 2^-15 of it (int8: 2^-24) may
+ * lose bits of their codes.  Tokens that a row does not see never matter to it.
  * max_rows: the most rows of any sequence, a hint that picks the kernels (a
  * wrong value costs time, not results).  The workspace, 16-byte aligned, of
  * at least noor_kv_attention_workspace bytes for the same arguments, is free

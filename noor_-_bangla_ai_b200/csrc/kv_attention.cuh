@@ -25,7 +25,9 @@
 // two f16 parts (22 bits).  Probabilities p are f16 as well, off by 2^-11
 // relative, an eighth of the BF16 output's half step (F32: two parts again),
 // scaled by 2^14 so that p down to 2^-38 counts in a long context.  A block's
-// v scale multiplies its p, relative to the largest scale so far.
+// v scale multiplies its p, relative to the largest scale (up to a power of two)
+// among the tokens that the row has seen so far: what a row does not see leaves
+// its bits alone.
 //
 // Measured at 32 / 8 heads of 128 dims: 64 ragged sequences of up to 8192
 // tokens, a row each, e4m3, 120-124 us = 5.5 TB/s of codes; 4 x 131072 tokens,
@@ -205,7 +207,7 @@ struct Shape {
   // reads of different pages fall into different banks
   static constexpr int kVPad = 128;
   // bytes of the second warp's part when the pair joins (it reuses the ring)
-  static constexpr int kJoin = (DP / 16 * NB * 4 + 4 * NB + 1) * 32 * 4;
+  static constexpr int kJoin = (DP / 16 * NB * 4 + 6 * NB) * 32 * 4;
   static __host__ __device__ int pair_bytes(int D) {
     const int ring = kStages * (2 * kTile * D + kVPad);
     return (ring > kJoin ? ring : kJoin) + kQBytes;
@@ -460,14 +462,15 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][nb][x] = 0.f;
     float m[NB][2], l[NB][2];
+    float vinv[NB][2];  // over each row's largest v scale so far, a power of two
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         m[nb][x] = -INFINITY;
         l[nb][x] = 0.f;
+        vinv[nb][x] = kv::kMostScale;  // (2^126)
       }
-    float vref = 1.17549435e-38f;
 
     // Fixed parts of this lane's addresses: its score tokens' page and rows, its
     // value tokens' page and bytes.
@@ -529,14 +532,12 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       }
       // ---- scale, mask, running maximum
       float alpha[NB][2], mref[NB][2];
-      const float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 16));
-      const float vnew = fmaxf(vref, vmax);
-      const float vstep = vref / vnew, vrel = vs / vnew;
-      vref = vnew;
-      bool moved = vstep != 1.f;
+      const float vmax = fmaxf(fmaxf(vs, 0.f), __shfl_xor_sync(0xffffffffu, vs, 16));
+      bool moved = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float tm[2] = {-INFINITY, -INFINITY};
+        float tm[2] = {-INFINITY, -INFINITY}, vseen[2] = {vmax, vmax};  // largest scale that the row sees here
+        if constexpr (!whole) vseen[0] = vseen[1] = 0.f;
         const float f0 = qfac[nb][0] * ks, f1 = qfac[nb][1] * ks;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -545,7 +546,10 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             float v = sc[i][nb][x] * ((x & 1) ? f1 : f0);
             if constexpr (!whole) {
               const int tok = tok0 + my_tok + 2 * (2 * i + (x >> 1)), p = qpos[nb][x & 1];
-              if (tok > p || (a.window > 0 && p - tok > a.window)) v = -INFINITY;
+              if (tok > p || (a.window > 0 && p - tok > a.window))
+                v = -INFINITY;
+              else
+                vseen[x & 1] = fmaxf(vs, 0.f);
             }
             sc[i][nb][x] = v;
             tm[x & 1] = fmaxf(tm[x & 1], v);
@@ -559,6 +563,15 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
           mref[nb][x] = mn == -INFINITY ? 0.f : mn - kPShift;
           alpha[nb][x] = mn == -INFINITY ? 1.f : exp2_approx(m[nb][x] - mn);
           m[nb][x] = mn;
+          l[nb][x] *= alpha[nb][x];
+          if constexpr (!whole) {
+            vseen[x] = fmaxf(vseen[x], __shfl_xor_sync(0xffffffffu, vseen[x], 4));
+            vseen[x] = fmaxf(vseen[x], __shfl_xor_sync(0xffffffffu, vseen[x], 8));
+            vseen[x] = fmaxf(vseen[x], __shfl_xor_sync(0xffffffffu, vseen[x], 16));
+          }
+          const float vnew = fminf(vinv[nb][x], kv::power_inverse(kv::power_up(vseen[x])));
+          alpha[nb][x] *= vnew * kv::power_inverse(vinv[nb][x]);
+          vinv[nb][x] = vnew;
           moved |= alpha[nb][x] != 1.f;
         }
       }
@@ -574,7 +587,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             const float p = exp2_approx(sc[i][nb][x] - mref[nb][x & 1]);
             sum[x & 1] += p;
             // a masked token's p is zero whatever its block's scale
-            sc[i][nb][x] = !whole && sc[i][nb][x] == -INFINITY ? 0.f : p * vrel;
+            sc[i][nb][x] = !whole && sc[i][nb][x] == -INFINITY ? 0.f : p * (vs * vinv[nb][x & 1]);
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -584,10 +597,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
           }
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          l[nb][x] = l[nb][x] * alpha[nb][x] + sum[x];
-          alpha[nb][x] *= vstep;
-        }
+        for (int x = 0; x < 2; ++x) l[nb][x] += sum[x];
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -672,19 +682,18 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         for (int x = 0; x < 2; ++x) {
           j[(4 * nb + 2 * x) * 32] = m[nb][x];
           j[(4 * nb + 2 * x + 1) * 32] = l[nb][x];
+          j[(4 * NB + 2 * nb + x) * 32] = kv::power_inverse(vinv[nb][x]);
         }
-      j[4 * NB * 32] = vref;
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) j[(4 * NB + 1 + (i * NB + nb) * 4 + x) * 32] = o[i][nb][x];
+          for (int x = 0; x < 4; ++x) j[(6 * NB + (i * NB + nb) * 4 + x) * 32] = o[i][nb][x];
     }
     pair_sync(pair);
     if (half == 0) {
       const float* j = s_join + lane;
-      const float vref1 = j[4 * NB * 32];
       const bool done = at == u0 && stop == u1;
       const int64_t slot = 2 * (int64_t)wid + (piece > 0 ? 1 : 0);
 #pragma unroll
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
           if (r >= nrows) continue;
           const int e = e0 + r, row = w.s.row0 + e / a.g, head = h * a.g + e % a.g;
           const float inv = !done ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
-          const float g0 = f0 * vref * inv, g1 = f1 * vref1 * inv;
+          const float g0 = f0 * kv::power_inverse(vinv[nb][x]) * inv, g1 = f1 * j[(4 * NB + 2 * nb + x) * 32] * inv;
           if (gr == 0) {
             if (!done) {
               a.part_ml[(slot * R + r) * 2] = ll == 0.f ? -INFINITY : mm;
@@ -718,7 +727,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const int d = 16 * i + 8 * y + gr;
-              const float v = o[i][nb][2 * y + x] * g0 + j[(4 * NB + 1 + (i * NB + nb) * 4 + 2 * y + x) * 32] * g1;
+              const float v = o[i][nb][2 * y + x] * g0 + j[(6 * NB + (i * NB + nb) * 4 + 2 * y + x) * 32] * g1;
               if (done)
                 op[d] = rope::from_f32<T>(v);
               else

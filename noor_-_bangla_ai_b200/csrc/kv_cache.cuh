@@ -182,6 +182,13 @@ __device__ __forceinline__ float read_scale(float s) {
   return s >= 0.f && s <= kMostScale ? s : __uint_as_float(0x7FC00000u);
 }
 
+// A readable scale (or the largest of some) up to a power of two, and a power
+// of two's reciprocal; zero counts as 2^-126 or, reciprocally, 2^127.
+__device__ __forceinline__ float power_up(float s) {
+  return __uint_as_float(max((__float_as_uint(s) + 0x7FFFFFu) & 0x7F800000u, 0x800000u));
+}
+__device__ __forceinline__ float power_inverse(float p) { return __uint_as_float(0x7F000000u - __float_as_uint(p)); }
+
 // The scale of a block that held tokens at s_old and now needs s_new: the
 // larger, as a power of two; NaN stays.  (A poisoned block's codes are stored
 // as zeros: a reader's zero weight times any stored code is zero.)

@@ -27,8 +27,15 @@
 // 547 us = 880 TFLOP/s of visible products.  Bound by the softmax warps: an
 // exponential, its scaling and the sums for each score, beside TMEM reads; the
 // tensor core waits for p.
-// A block's v scale is applied while widening, relative to the largest v scale
-// so far (exact for powers of two); o follows when that grows.
+// V scales.  o of a row is held relative to the largest v scale (up to a power
+// of two) among the tokens that the row has seen so far, and follows when that
+// grows; what a row does not see leaves its bits alone.
+//   A tile that every row of the unit sees whole is widened relative to its own
+//   largest scale (exact for powers of two, down to 2^-24 of it for int8 and
+//   2^-15 for e4m3), and its ratio to the row's, a power of two, goes into the
+//   exponential: p comes out scaled, and its sum is scaled back.
+//   In the other tiles (the context's end, a window's start) values are codes
+//   alone, and each p is multiplied by its block's scale over the row's.
 #pragma once
 
 #include "kv_attention.cuh"
@@ -129,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   __shared__ __align__(8) Bars bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ float s_kf[kMeta][8], s_vf[kMeta][8];  // factors of each 16 tokens
-  __shared__ float s_vref[kMeta], s_vstep[kMeta];   // the v reference, and the last one over it
+  // of each 16 tokens: scores' factor, widened values' factor, v scale; and the tile's largest, a power of two
+  __shared__ float s_kf[kMeta][8], s_vf[kMeta][8], s_vs[kMeta][8], s_vc[kMeta];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.c.D, blk = a.c.blk;
@@ -197,6 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   const int tb = first + (int)((int64_t)count * part / parts);
   const int T = first + (int)((int64_t)count * (part + 1) / parts) - tb;
   const int32_t* table = a.b.table + (int64_t)sb * a.b.tstride;
+  // whether every row of the unit sees all of the tile of tokens tok0 ..
+  auto sees_whole = [&](int tok0) { return tok0 + kTok - 1 <= p_first && (a.window <= 0 || p_last - tok0 <= a.window); };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -297,10 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bar.q_full[wg]);
 
-      // rows of this row tile, for the tiles that need no mask
-      const int wfirst = pos0 + (e0 + 128 * wg) / a.g;
-      const int wlast = pos0 + (e0 + min(128 * wg + 127, nrows - 1)) / a.g;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, ref = 1.17549435e-38f;  // ref: the largest v scale so far, a power of two
       bool ok = true;
       // One tile's scores to probabilities, compiled apart for tiles that every
       // row sees whole: a test for each score costs more than its exponential.
@@ -336,14 +342,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           }
         }
         const bool grow = mx2 > m + kLazy || (m == -INFINITY && mx2 > -INFINITY);
+        float vseen = 0.f;  // the largest v scale that the row sees here
+        if constexpr (whole) {
+          vseen = s_vc[i % kMeta];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (16 * j <= chi && 16 * j + 15 >= clo) vseen = fmaxf(vseen, s_vs[i % kMeta][j]);
+          vseen = kv::power_up(vseen);
+        }
+        const float vnew = fmaxf(ref, vseen);
         if (i == 0) {
           m = mx2;
-        } else if (__any_sync(0xffffffffu, grow) || s_vstep[i % kMeta] != 1.f) {
+          ref = vnew;
+        } else if (__any_sync(0xffffffffu, grow || vnew != ref)) {
           // (o holds all earlier tiles: its last product ran before this s)
           float alpha = grow ? attn::exp2_approx(m - mx2) : 1.f;
           if (grow) m = mx2;
           l *= alpha;
-          alpha *= s_vstep[i % kMeta];
+          alpha *= ref * kv::power_inverse(vnew);
+          ref = vnew;
           for (int c = 0; c < D; c += 16) {
             uint32_t v[16];
             asm volatile(
@@ -358,7 +376,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
           }
         }
         const float mref = m == -INFINITY ? 0.f : m - kShift;
-        const uint64_t neg = pair2(-mref, -mref);
+        // the tile's scale over the row's, 2^-down: in the exponent of p (below
+        // 2^-42 no p reaches f16, and the sum keeps its bits)
+        const int down = whole ? min((int)(__float_as_uint(ref) - __float_as_uint(vseen)) >> 23, 42) : 0;
+        const float vi = kv::power_inverse(ref), neg1 = -mref - (float)down;
+        const uint64_t neg = pair2(neg1, neg1);
         uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -378,13 +400,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
               z.y = col + 1 >= clo && col + 1 <= chi ? z.y : 0.f;
             }
             sum[(x >> 1) & 3] = add2(sum[(x >> 1) & 3], pair2(z.x, z.y));
+            if constexpr (!whole) {
+              const float vr = fminf(s_vs[i % kMeta][2 * c + (x >> 4)] * vi, 1.f);  // (above 1: a block it does not see)
+              z.x *= vr;
+              z.y *= vr;
+            }
             p[x >> 1] = attn::pack_half(z.x, z.y);
           }
           // columns 16 c .. of p lie over scores that were read already
           tmem_st16(t_s + 16 * c, p);
         }
         const float2 t2 = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-        l += t2.x + t2.y;
+        l = fmaf(t2.x + t2.y, __uint_as_float((uint32_t)(127 + down) << 23), l);
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -392,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       };
       for (int i = 0; i < T && ok; ++i) {
         const int tok0 = (tb + i) * kTok;
-        const bool whole = tok0 + kTok - 1 <= wfirst && (a.window <= 0 || wlast - tok0 <= a.window);
+        const bool whole = sees_whole(tok0);
         // visible columns of this row
         const int chi = min(pos - tok0, kTok - 1), clo = a.window > 0 ? pos - a.window - tok0 : 0;
         ok = __all_sync(0xffffffffu, wait(&bar.s_full[wg], i & 1));
@@ -408,9 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
         tc::tc_fence_after();
       }
       if (ok) {
-        const float vref = T > 0 ? s_vref[(T - 1) % kMeta] : 0.f;
         // a part leaves its sums as they are, with the reference of the join's shift
-        const float inv = cut ? vref : l == 0.f ? 0.f : 1.f / l * vref;
+        const float inv = cut ? ref : l == 0.f ? 0.f : 1.f / l * ref;
         const int64_t slot = (int64_t)blockIdx.x * 256 + 128 * wg + r;
         bf16* op = static_cast<bf16*>(const_cast<void*>(a.out.p)) + (int64_t)row * a.out.st + (int64_t)head * a.out.sh;
         const bool ovec = (reinterpret_cast<uintptr_t>(a.out.p) | (uintptr_t)(a.out.st * 2) | (uintptr_t)(a.out.sh * 2)) % 16 == 0;
@@ -632,7 +658,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
     const int pages = kTok / blk;
     const uint32_t bytes = (uint32_t)blk * D;
     const float nan = __uint_as_float(0x7FC00000u);
-    float vref = 1.17549435e-38f;  // the largest v scale so far
     int issued = 0;  // tiles whose copies were issued (k, and v one step later)
     bool ok = true, vpending = false;
     for (int i = 0; i < T && ok; ++i) {
@@ -653,17 +678,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       ks = __shfl_sync(0xffffffffu, ks, src);
       vs = __shfl_sync(0xffffffffu, vs, src);
       const bool fin = vs == vs;
-      const float vnew = fmaxf(vref, __uint_as_float(__reduce_max_sync(0xffffffffu, fin ? __float_as_uint(vs) & 0x7FFFFFFFu : 0u)));
+      const float vc = kv::power_up(__uint_as_float(__reduce_max_sync(0xffffffffu, fin ? __float_as_uint(vs) & 0x7FFFFFFFu : 0u)));
       ok = wait(&bar.raw_empty[0], (i & 1) ^ 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (lane < 8) {
         s_kf[i % kMeta][lane] = fin ? ks : nan;
-        s_vf[i % kMeta][lane] = fin ? vs / vnew : 0.f;
-        s_vref[i % kMeta] = vnew;
-        s_vstep[i % kMeta] = vref / vnew;
+        s_vf[i % kMeta][lane] = !fin ? 0.f : sees_whole(tok0) ? vs * kv::power_inverse(vc) : 1.f;
+        s_vs[i % kMeta][lane] = fin ? vs : 0.f;
+        s_vc[i % kMeta] = vc;
       }
-      vref = vnew;
       const unsigned who = __ballot_sync(0xffffffffu, page >= 0);
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_expect_tx(&bar.raw_full[0], __popc(who) * bytes);

@@ -533,6 +533,39 @@ def test_attention_value_scales_far_apart(pkg, cuda_device, fmt, rows, down):
             assert bool(((x[beg:end].cpu().double() - o).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,blk,step", [(64, 16, 80), (128, 32, 96), (96, 64, 64), (144, 16, 48), (256, 64, 128)])
+@pytest.mark.parametrize("up", [12, 25, 40, 100])
+@pytest.mark.parametrize("window", [0, 20])
+def test_hidden_value_scales_leave_a_row_alone(pkg, cuda_device, dtype, fmt, D, blk, step, up, window):
+    """Values 2^up larger from token `step` on (with a window: up to there), the
+    border inside the kernels' tiles: rows that do not see them keep the bits
+    they have without them, beside rows that do, few or many.  f16's floor is
+    relative to the largest scale that the row itself sees."""
+    L, P = 200, -(-200 // blk)
+    c, _, _ = make_cache(pkg, P, 1, blk, D, fmt)
+    rk, rv = fill(c, 49)
+    big = torch.arange(P) >= step // blk if window == 0 else torch.arange(P) < step // blk
+    rv.scale[big] *= 2.0 ** up
+    c.v_scale.copy_(rv.scale.float())
+    tab, g = i32([list(range(P))]), 4
+    k, v = rk.tokens(range(P), L), rv.tokens(range(P), L)
+    size = rv.scale[:, 0].repeat_interleave(blk)[:L]  # of each token
+    for beg, end in ((0, 200), (step - 5, step + 4), (step + 15, step + 25), (step - 2, step + 7)):
+        pos = torch.arange(beg, end)
+        q = randn((end - beg, g, D), 50, DT[dtype])
+        o, _, mag, smax, _ = ref.attend(q.double(), k[:end], v[:end], pos, D ** -0.5, window)
+        sees = (torch.arange(end)[None] <= pos[:, None]) & ((pos[:, None] - torch.arange(end)[None] <= window) | (window == 0))
+        most = (sees * size[:end]).amax(-1)
+        vsum = (sees.double() @ (v[:end, 0].abs() / size[:end, None]) * most[:, None])[:, None]
+        tol = ref.attend_tolerance(DT[dtype], o, mag, smax, vsum, D, end)
+        got = c.attention(q.cuda(), tab, i32([end]), i32([0, end - beg]), end - beg, window=window).cpu().double()
+        bad = torch.isnan(got) | ((got - o).abs() > tol)
+        assert not bool(bad.any()), (beg, end, bad.any(-1).any(-1).nonzero().flatten().tolist())
+    c.check()
+
+
 @pytest.mark.parametrize("news", [1, 200])
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_attention_masked_blocks_may_hold_anything(pkg, cuda_device, news, fmt):
