@@ -146,24 +146,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
   // ---- parts of each unit, from the units that the batch has
   int parts = 1;
   if constexpr (PARTS) {
-    __shared__ int32_t s_units;
-    if (threadIdx.x == 0) s_units = 0;
+    __shared__ int32_t s_units, s_tiles;
+    if (threadIdx.x == 0) s_units = s_tiles = 0;
     __syncthreads();
-    int32_t n = 0;
-    for (int i = threadIdx.x; i < a.b.B; i += kThreads) n += attn::seq_work(a, i).rtiles;
+    int32_t n = 0, longest = 0;  // units of a kv head; most tiles of their sequences
+    for (int i = threadIdx.x; i < a.b.B; i += kThreads) {
+      const attn::SeqWork w = attn::seq_work(a, i);
+      n += w.rtiles;
+      if (w.rtiles > 0) longest = max(longest, (w.s.len + kTok - 1) / kTok);
+    }
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0 && n > 0) atomicAdd(&s_units, n);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0 && n > 0) {
+      atomicAdd(&s_units, n);
+      atomicMax(&s_tiles, longest);
+    }
     __syncthreads();
-    const int32_t units = s_units * a.c.H;
+    // (the host knows the page table's width and the window, not the lengths)
+    const int32_t units = s_units * a.c.H, seen = min(a.seen, s_tiles);
     if (units < a.sms) {
-      const int most = attn::most_parts(units, a.seen, a.sms, a.pairs);
+      const int most = attn::most_parts(units, seen, a.sms, a.pairs);
       uint32_t best = 0xFFFFFFFFu;  // cost, then parts
       for (int s = 2 + lane; s <= most; s += 32) {
-        const uint32_t cost = attn::part_cost(units, a.seen, s, a.sms);
+        const uint32_t cost = attn::part_cost(units, seen, s, a.sms);
         best = min(best, min(cost, (1u << 22) - 1) << 10 | (uint32_t)s);
       }
       best = __reduce_min_sync(0xffffffffu, best);
-      if (best != 0xFFFFFFFFu && 20 * (best >> 10) < 19 * (uint32_t)attn::part_cost(units, a.seen, 1, a.sms)) parts = best & 1023;
+      if (best != 0xFFFFFFFFu && 20 * (best >> 10) < 19 * (uint32_t)attn::part_cost(units, seen, 1, a.sms)) parts = best & 1023;
     }
   }
   const bool cut = PARTS && parts > 1;

@@ -484,6 +484,28 @@ def test_attention_many_rows_in_parts(pkg, cuda_device, D, blk, fmt, lens, news)
     c.check()
 
 
+@pytest.mark.parametrize("lens,news", [([1024], [512]), ([1000, 700], [256, 5]), ([3000, 1, 90], [40, 1, 33]), ([200], [9])])
+@pytest.mark.parametrize("window", [0, 300])
+def test_a_wider_page_table_changes_nothing(pkg, cuda_device, lens, news, window):
+    """How a context is cut goes by the sequences' lengths, not by the room that
+    the page table has for more: the answers are the same to the bit."""
+    blk, H = 64, 4
+    need = [-(-n // blk) for n in lens]
+    c, _, _ = make_cache(pkg, sum(need), H, blk, 128, "int8")
+    fill(c, 51)
+    tab = np.full((len(lens), max(need)), -1, np.int64)
+    for b, n in enumerate(need):
+        tab[b, :n] = np.arange(n) + sum(need[:b])
+    q = randn((sum(news), 4 * H, 128), 52, torch.bfloat16).cuda()
+    out = []
+    for wide in (0, 8, 2048):
+        t = np.concatenate([tab, np.full((len(lens), wide), -1, np.int64)], 1)
+        out.append(c.attention(q, i32(t.tolist()), i32(lens), cu_of(news), max(news), window=window, return_lse=True))
+    for got, lse in out[1:]:
+        assert torch.equal(got, out[0][0]) and torch.equal(lse, out[0][1])
+    c.check()
+
+
 @pytest.mark.parametrize("L", [350, 5000])
 def test_overlapping_row_offsets_stay_in_bounds(pkg, cuda_device, L):
     """Offsets that go back: one sequence is skipped, two share rows, and the
