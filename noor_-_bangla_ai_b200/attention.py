@@ -84,12 +84,23 @@ def _ints(t, what: str, n: int, device: int) -> int:
     return t.data_ptr()
 
 
+def _tangent(t):
+    """t's forward-mode tangent, None without one (and outside of dual levels, at
+    once)."""
+    fw = _T.autograd.forward_ad
+    if t is None or getattr(fw, "_current_level", 0) < 0:
+        return None
+    return fw.unpack_dual(t).tangent
+
+
 def _no_grad(*tensors) -> None:
-    """The cache rounds to 8 bits and holds no graph: refuse what wants a gradient."""
-    if _T.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError("the cached path has no gradient: call it under torch.no_grad() or detach its inputs")
+    """The cache rounds to 8 bits and holds no graph: refuse what wants a gradient
+    or carries a tangent."""
+    grad = _T.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (grad and t.requires_grad or _tangent(t) is not None):
+            raise ValueError("the cached path has no gradient: call it under torch.no_grad() or detach its inputs, without "
+                             "forward-mode tangents")
 
 
 def _empty_like(t):
@@ -233,25 +244,36 @@ def _rope_autograd():
                 if gq is None and gk is None:
                     return None, None, None, None, None
                 first, second = (gq, gk) if gq is not None else (gk, None)
-                if torch.is_grad_enabled():
-                    out = RopeFunction.apply(first, second, positions, rotary, not inverse)
-                    d0, d1 = out if second is not None else (out, None)
-                else:
-                    d0, d1 = _rope_call(first, second, positions, rotary, not inverse)
+                d0, d1 = _rope(first, second, positions, rotary, not inverse)
                 return (d0, d1, None, None, None) if gq is not None else (None, d0, None, None, None)
 
         _rope_function = RopeFunction
     return _rope_function
 
 
+def _rope(q, k, positions, rotary: Rotary, inverse: bool):
+    """(q', k') of q and k (or None), with their derivatives where asked for."""
+    torch = _torch()
+    tq, tk = _tangent(q), _tangent(k)
+    if tq is not None or tk is not None:  # linear in q and k: tangents turn alike
+        fw = torch.autograd.forward_ad
+        out = list(_rope(fw.unpack_dual(q).primal, None if k is None else fw.unpack_dual(k).primal, positions, rotary, inverse))
+        for i, t in enumerate((tq, tk)):
+            if t is not None:
+                t = t if t.stride(-1) == 1 else t.contiguous()
+                out[i] = fw.make_dual(out[i], _rope(t, None, positions, rotary, inverse)[0])
+        return tuple(out)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        out = _rope_autograd().apply(q, k, positions, rotary, inverse)
+        return (out, None) if k is None else out
+    return _rope_call(q, k, positions, rotary, inverse)
+
+
 def rope_apply(q, positions, rotary: Rotary, k=None):
     """Rotate q [tokens, heads, head_dim] (and k beside it, in one launch) to
-    positions [tokens] (int32).  Differentiable in q and k; returns new tensors
-    q', or (q', k')."""
-    torch = _torch()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _rope_autograd().apply(q, k, positions, rotary, False)
-    q_out, k_out = _rope_call(q, k, positions, rotary, False)
+    positions [tokens] (int32).  Differentiable in q and k, backward and forward;
+    returns new tensors q', or (q', k')."""
+    q_out, k_out = _rope(q, k, positions, rotary, False)
     return q_out if k is None else (q_out, k_out)
 
 

@@ -881,6 +881,47 @@ def test_rope_gradient_in_a_graph_and_twice(pkg, cuda_device):
     assert float((g2 - 2 * v).abs().max()) <= 1e-5  # R^T R = 1
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_forward_derivative(pkg, cuda_device, dtype, layout):
+    """Rotation is linear: a tangent comes out rotated as its input is, for q, k
+    or both, also through its gradient and where gradients are off."""
+    A, fw = pkg.attention, torch.autograd.forward_ad
+    inv, factor = A.rotary_frequencies(32, 10000.0, 0.75, yarn={"scale": 4.0, "original": 2048})
+    r, inv = A.Rotary(inv, layout, factor), torch.from_numpy(inv)
+    pos = i32([5, 0, 4096])
+    q, k, tq, tk = (randn((3, h, 32), 110 + i, DT[dtype]) for i, h in enumerate((2, 1, 2, 1)))
+    with fw.dual_level():
+        dq, dk = fw.make_dual(q.cuda(), tq.cuda()), fw.make_dual(k.cuda(), tk.cuda())
+        for gq, gk, with_grad in ((dq, dk, True), (dq, k.cuda(), True), (q.cuda(), dk, False), (dq, None, False)):
+            with torch.set_grad_enabled(with_grad):
+                out = A.rope_apply(gq, pos, r, k=gk)
+            out = out if gk is not None else (out,)
+            for o, x, t, dual in zip(out, (q, k), (tq, tk), (gq is dq, gk is dk)):
+                p, tangent = fw.unpack_dual(o)
+                check_rope(p, x, pos.cpu(), inv, layout, factor)
+                if dual:
+                    check_rope(tangent, t, pos.cpu(), inv, layout, factor)
+                else:
+                    assert tangent is None or not bool(tangent.any())
+        # the tangent of the gradient of sum(w . rope(q) . rope(q)) along tq is R^T(w . 2 R tq)
+        x = fw.make_dual(q.cuda().float().requires_grad_(), tq.cuda().float())
+        y = A.rope_apply(x, pos, r)
+        (g,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        tangent = fw.unpack_dual(g).tangent
+        want = ref.rotate(2 * ref.rotate(tq, pos.cpu(), inv, layout, factor), pos.cpu(), inv, layout, factor, -1.0)
+        assert float((tangent.detach().cpu().double() - want).abs().max()) <= 64 * 2.0 ** -24 * 2 * factor ** 2 * 6
+        c = A.KVCache(2, 1, 32)
+        args = (i32([[0, 1]]), i32([3]), i32([0, 3]))
+        x = k.cuda()
+        for call in (lambda: c.append(dk, x, *args), lambda: c.append(x, dk, *args), lambda: c.append(x, x, *args, rotary=r, q=dq),
+                     lambda: c.attention(dq, *args, 3)):
+            for with_grad in (True, False):
+                with torch.set_grad_enabled(with_grad), pytest.raises(ValueError, match="tangents"):
+                    call()
+    c.check()
+
+
 def test_stack_served_from_the_cache(pkg, cuda_device):
     """NoorStack.forward_cached: the attention half against its plain form (the
     projections, the cache and the attention of one layer), and a prompt at once
