@@ -338,8 +338,9 @@ class KVCache:
         self._workspace = {}  # bytes of attention's workspace by its sizes
 
     def check(self) -> None:
-        """Wait for the device and raise NoorMoEError if a kernel found a
-        mistake in device metadata since the last check; clears it."""
+        """Wait for the device (every stream's calls) and raise NoorMoEError if a
+        kernel found a mistake in device metadata since the last check; clears it."""
+        _torch().cuda.synchronize(self.device)
         code = int(self.status.item())
         if code:
             self.status.zero_()

@@ -754,6 +754,24 @@ def test_attention_skips_a_sequence_shorter_than_its_rows(pkg, cuda_device, dtyp
     c.check()
 
 
+def test_check_waits_for_other_streams(pkg, cuda_device):
+    """A mistake found by a call that is still queued on another stream is not
+    missed."""
+    c, _, _ = make_cache(pkg, 4, 1, 16, 16, "int8", junk=False)
+    x = torch.ones((1, 1, 16), device="cuda")
+    tab, lens, cu = i32([[4]]), i32([1]), i32([0, 1])  # page 4 of 4
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    c.append(x, x, i32([[0]]), lens, cu)
+    c.check()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second of work ahead of it
+        c.append(x, x, tab, lens, cu)
+    with pytest.raises(pkg.api.NoorMoEError, match="page"):
+        c.check()
+    c.check()
+
+
 def test_attention_in_place_and_shared_pages(pkg, cuda_device):
     """out may be q; sequences may share pages (a common prefix)."""
     blk, D = 16, 48
