@@ -189,8 +189,9 @@ class StackCache:
         lens = [o + n for o, n in zip(self.lens, news)]
         if max(lens) > self.max_tokens:
             raise ValueError(f"a sequence would hold {max(lens)} tokens, the cache {self.max_tokens}")
+        rows = CacheRows(self.block_table, lens, news)
         self.lens = lens
-        return CacheRows(self.block_table, lens, news)
+        return rows
 
     def reset(self, sequence: int) -> None:
         """Start sequence `sequence` over (its pages are written afresh)."""
@@ -330,21 +331,28 @@ class NoorStack:
     def forward_cached(self, token_ids: Sequence[Sequence[int]], cache: StackCache):
         """The next tokens of each sequence (a prompt, one token, or none), on top
         of what the cache holds.  Returns (logits [rows, vocab] f32, per-layer
-        expert utilization fractions), rows in sequence order."""
+        expert utilization fractions), rows in sequence order.  If it raises, the
+        cache holds the tokens that it held before."""
         import torch
         dev = torch.device("cuda", self.device)
         tdt = torch.bfloat16 if self.dtype == api.DTYPE_BF16 else torch.float32
         flat = np.concatenate([np.asarray(t, np.int64).reshape(-1) for t in token_ids])
         if flat.size and (flat.max() >= self.embedding.shape[0] or flat.min() < 0):
             raise ValueError("token id out of vocab range")
+        held = cache.lens
         rows = cache.step([len(t) for t in token_ids])
-        h = torch.from_numpy(self.embedding[flat]).to(dev).to(tdt)
-        util = []
-        for b, layer in zip(self.blocks, cache.layers):
-            rope = self.prope if (b.is_global and self.prope is not None) else self.rope
-            h = b.forward_cached(h, rope, layer, rows)
-            util.append(b.parallel_ffn.moe.utilization.fractions())
-            b.parallel_ffn.moe.utilization.reset()
-        w = torch.from_numpy(self.final_norm.weight).to(dev)
-        h = _rms_norm_torch(h, w, self.final_norm.eps, 1.0)
-        return h.float() @ torch.from_numpy(self.output_proj).to(dev), util
+        try:
+            h = torch.from_numpy(self.embedding[flat]).to(dev).to(tdt)
+            util = []
+            for b, layer in zip(self.blocks, cache.layers):
+                rope = self.prope if (b.is_global and self.prope is not None) else self.rope
+                h = b.forward_cached(h, rope, layer, rows)
+                util.append(b.parallel_ffn.moe.utilization.fractions())
+                b.parallel_ffn.moe.utilization.reset()
+            w = torch.from_numpy(self.final_norm.weight).to(dev)
+            h = _rms_norm_torch(h, w, self.final_norm.eps, 1.0)
+            logits = h.float() @ torch.from_numpy(self.output_proj).to(dev)
+        except BaseException:
+            cache.lens = held
+            raise
+        return logits, util

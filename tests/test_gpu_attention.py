@@ -1006,6 +1006,36 @@ def test_stack_served_from_the_cache(pkg, cuda_device):
         b.parallel_ffn.moe.invalidate()
 
 
+def test_stack_step_that_fails_is_not_counted(pkg, cuda_device):
+    """A layer that raises in the middle of a step: the cache holds what it held,
+    and the same tokens again give what they would have given."""
+    S = pkg.stack
+    rng = np.random.default_rng(6)
+    st = S.NoorStack(vocab_size=31, d_model=64, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=32, dense_ffn_dim=128,
+                     expert_ffn_dim=64, n_experts=4, n_active_experts=2, sliding_window=8, global_every_n=2, prope_fraction=0.25,
+                     dtype=pkg.api.DTYPE_F32, rng=rng)
+    ids = [list(rng.integers(0, 31, 20)), list(rng.integers(0, 31, 9))]
+    clean, broken = st.new_cache(2, 32, block=16), st.new_cache(2, 32, block=16)
+    for c in (clean, broken):
+        st.forward_cached([ids[0][:12], ids[1][:8]], c)
+    want, _ = st.forward_cached([ids[0][12:], ids[1][8:]], clean)
+    block, fine = st.blocks[1], st.blocks[1].forward_cached
+
+    def fails(*a):
+        raise RuntimeError("planted")
+
+    block.forward_cached = fails
+    with pytest.raises(RuntimeError, match="planted"):
+        st.forward_cached([ids[0][12:], ids[1][8:]], broken)
+    block.forward_cached = fine
+    assert broken.lens == [12, 8]
+    got, _ = st.forward_cached([ids[0][12:], ids[1][8:]], broken)
+    assert broken.lens == [20, 9] and float((got - want).norm() / want.norm()) <= 1e-4
+    broken.check()
+    for b in st.blocks:
+        b.parallel_ffn.moe.invalidate()
+
+
 def test_cached_path_refuses_gradients_and_takes_any_window(pkg, cuda_device):
     c = pkg.attention.KVCache(4, 1, 16, 16)
     x = torch.ones((1, 1, 16), device="cuda", requires_grad=True)
