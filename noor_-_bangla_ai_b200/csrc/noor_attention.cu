@@ -439,9 +439,13 @@ int launch_join(const attn::Args& a, int n, int rows, cudaStream_t s) {
   return NOOR_MOE_OK;
 }
 
-int check_heads(const noor_kv_cache* c, int Hq) {
+int check_heads(const noor_kv_cache* c, const noor_kv_batch* b, int Hq) {
   if (Hq <= 0 || Hq > 65536 || Hq % c->n_kv_heads != 0)
     return fail(NOOR_MOE_ERR_INVALID, "%d query heads over %d kv heads", Hq, c->n_kv_heads);
+  // the kernels number a kv head's (row, query head) pairs in 32 bits, and round up to a tile of 256
+  if (b->n_rows * (Hq / c->n_kv_heads) > INT32_MAX - 256)
+    return fail(NOOR_MOE_ERR_INVALID, "n_rows %lld times %d query heads of a kv head is past 32 bits", (long long)b->n_rows,
+                Hq / c->n_kv_heads);
   return NOOR_MOE_OK;
 }
 
@@ -455,7 +459,7 @@ int noor_kv_attention_workspace(const noor_kv_cache* c, const noor_kv_batch* b, 
     CKR(check_cache(c));
     CKR(check_batch(c, b));
     CKR(check_dtype(dtype));
-    CKR(check_heads(c, q_heads));
+    CKR(check_heads(c, b, q_heads));
     if (!bytes || max_rows < 0) return fail(NOOR_MOE_ERR_INVALID, "null bytes or negative max_rows");
     StreamPlan p;
     CKR(stream_plan(c, b, q_heads, max_rows, 0, dtype, &p));  // (a window never needs more)
@@ -471,7 +475,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     CKR(check_cache(c));
     CKR(check_batch(c, b));
     CKR(check_dtype(dtype));
-    CKR(check_heads(c, q_heads));
+    CKR(check_heads(c, b, q_heads));
     if (max_rows < 0 || window < 0) return fail(NOOR_MOE_ERR_INVALID, "negative max_rows or window");
     if (window >= (int64_t)b->max_blocks * c->block) window = 0;  // longer than any sequence (positions less it stay in 32 bits)
     if (!std::isfinite(scale)) return fail(NOOR_MOE_ERR_INVALID, "scale is not finite");

@@ -98,6 +98,24 @@ def test_call_refusals(pkg):
     assert api.lib().noor_kv_attention_workspace(ctypes.byref(_cache(api)), ctypes.byref(_batch(api)), 4, 1, 1, None) == INVALID
 
 
+def test_rows_past_32_bits_are_refused(pkg):
+    """Row and query head of a group are numbered in 32 bits."""
+    api = pkg.api
+    n = ctypes.c_int64()
+
+    def need(rows, q_heads, kv_heads):
+        return api.lib().noor_kv_attention_workspace(ctypes.byref(_cache(api, n_kv_heads=kv_heads)),
+                                                     ctypes.byref(_batch(api, n_rows=rows)), q_heads, 1, 1, ctypes.byref(n))
+
+    assert need(1 << 28, 8, 1) == INVALID and need((1 << 25) - 4, 64, 1) == INVALID
+    # (the answer itself needs a device)
+    assert need(1 << 28, 14, 2) != INVALID and need((1 << 25) - 5, 64, 1) != INVALID
+    for rows, heads in ((1 << 28, 16), (1 << 26, 64)):
+        assert _call(api, "attention", cache=_cache(api, n_kv_heads=1), batch=_batch(api, n_rows=rows), q_heads=heads,
+                     bytes=1 << 62) == INVALID
+        assert b"32 bits" in api.lib().noor_moe_last_error()
+
+
 def test_python_refuses_cpu_tensors(pkg):
     A = pkg.attention
     with pytest.raises(ValueError):
