@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <exception>
 #include <initializer_list>
 #include <type_traits>
@@ -77,6 +78,16 @@ int check_view(const noor_heads* v, int dtype, const char* what) {
   if (!v || !v->data) return fail(NOOR_MOE_ERR_INVALID, "null %s", what);
   if (reinterpret_cast<uintptr_t>(v->data) % esize(dtype) != 0)
     return fail(NOOR_MOE_ERR_INVALID, "%s is not aligned to its elements", what);
+  return NOOR_MOE_OK;
+}
+
+// An output's heads lie apart: two of them that share elements would be written
+// by two threads at once.  (Strides that overlap in other ways are the caller's.)
+int check_out(const noor_heads* v, int64_t tokens, int heads, int D, int dtype, const char* what) {
+  CKR(check_view(v, dtype, what));
+  if ((tokens > 1 && std::abs(v->token_stride) < D) || (heads > 1 && std::abs(v->head_stride) < D))
+    return fail(NOOR_MOE_ERR_INVALID, "%s: heads of %d elements overlap (strides %lld and %lld)", what, D,
+                (long long)v->token_stride, (long long)v->head_stride);
   return NOOR_MOE_OK;
 }
 
@@ -186,9 +197,9 @@ int noor_rope_apply(const noor_rotary* r, const noor_heads* q, const noor_heads*
       return fail(NOOR_MOE_ERR_INVALID, "tokens or heads out of range");
     if (tokens == 0) return NOOR_MOE_OK;
     CKR(check_view(q, dtype, "q"));
-    CKR(check_view(q_out, dtype, "q_out"));
+    CKR(check_out(q_out, tokens, q_heads, head_dim, dtype, "q_out"));
     if (k) CKR(check_view(k, dtype, "k"));
-    if (k) CKR(check_view(k_out, dtype, "k_out"));
+    if (k) CKR(check_out(k_out, tokens, k_heads, head_dim, dtype, "k_out"));
     if (!positions) return fail(NOOR_MOE_ERR_INVALID, "null positions");
     CKR(check_device(device));
     DeviceGuard g(device);
@@ -230,8 +241,8 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
     CKR(check_view(v, dtype, "v"));
     if (q) {
       CKR(check_view(q, dtype, "q"));
-      CKR(check_view(q_out, dtype, "q_out"));
       if (q_heads <= 0 || q_heads > 4096) return fail(NOOR_MOE_ERR_INVALID, "q_heads %d out of range", q_heads);
+      CKR(check_out(q_out, b->n_rows, q_heads, c->head_dim, dtype, "q_out"));
     }
     CKR(check_device(c->device));
     DeviceGuard g(c->device);
@@ -481,7 +492,7 @@ int noor_kv_attention(const noor_kv_cache* c, const noor_kv_batch* b, const noor
     if (!std::isfinite(scale)) return fail(NOOR_MOE_ERR_INVALID, "scale is not finite");
     if (b->n_rows == 0) return NOOR_MOE_OK;
     CKR(check_view(q, dtype, "q"));
-    CKR(check_view(out, dtype, "out"));
+    CKR(check_out(out, b->n_rows, q_heads, c->head_dim, dtype, "out"));
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
       return fail(NOOR_MOE_ERR_INVALID, "workspace is null or not 16-byte aligned");
     StreamPlan p;

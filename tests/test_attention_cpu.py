@@ -98,6 +98,18 @@ def test_call_refusals(pkg):
     assert api.lib().noor_kv_attention_workspace(ctypes.byref(_cache(api)), ctypes.byref(_batch(api)), 4, 1, 1, None) == INVALID
 
 
+def test_outputs_whose_heads_overlap_are_refused(pkg):
+    api = pkg.api
+    for st, sh in ((0, 64), (256, 0), (63, 64), (256, 63), (256, -8)):
+        o = api.Heads(P, st, sh)
+        assert _call(api, "attention", out=o) == INVALID and _call(api, "append", out=o) == INVALID
+        assert _call(api, "rope", out=o) == INVALID and _call(api, "rope", rk=_heads(api), rk_out=o, k_heads=2) == INVALID
+        assert b"overlap" in api.lib().noor_moe_last_error()
+    one = api.Heads(P, 0, 0)  # one token, one head: no stride is used
+    assert _call(api, "rope", out=one, tokens=1, q_heads=1) != INVALID
+    assert _call(api, "attention", out=api.Heads(P, 64, 10 ** 6)) != INVALID
+
+
 def test_rows_past_32_bits_are_refused(pkg):
     """Row and query head of a group are numbered in 32 bits."""
     api = pkg.api
