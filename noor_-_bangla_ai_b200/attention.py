@@ -136,8 +136,10 @@ def rotary_frequencies(head_dim: int, theta: float = 10000.0, fraction: Optional
         raise ValueError(f"cannot rotate {rot} of {head_dim} dims")
     if sum((linear != 1.0, ntk != 1.0, yarn is not None)) > 1:
         raise ValueError("at most one of linear, ntk and yarn")
-    if linear <= 0 or ntk <= 0 or (yarn is not None and yarn["scale"] <= 0):
-        raise ValueError("a scale must be positive")
+    for what, x in (("theta", theta), ("linear", linear), ("ntk", ntk), *(() if yarn is None else (
+            ("yarn's scale", yarn["scale"]), ("yarn's original", yarn["original"])))):
+        if not (0 < x < math.inf):
+            raise ValueError(f"{what} must be positive and finite, got {x}")
     if ntk != 1.0 and rot > 2:
         theta = theta * ntk ** (rot / (rot - 2.0))
     inv = theta ** (-2.0 * np.arange(rot // 2, dtype=np.float64) / rot) / linear
@@ -145,6 +147,8 @@ def rotary_frequencies(head_dim: int, theta: float = 10000.0, fraction: Optional
     if yarn is not None:
         s = float(yarn["scale"])
         fast, slow = float(yarn.get("fast", 32.0)), float(yarn.get("slow", 1.0))
+        if not (-math.inf < slow < fast < math.inf):
+            raise ValueError(f"yarn's fast must be above its slow, got {fast} and {slow}")
         turns = float(yarn["original"]) * inv / (2.0 * math.pi)
         keep = np.clip((turns - slow) / (fast - slow), 0.0, 1.0)
         inv = inv / s * (1.0 - keep) + inv * keep

@@ -164,6 +164,16 @@ def test_rotary_tables(pkg):
             A.rotary_frequencies(64, **bad)
 
 
+@pytest.mark.parametrize("bad", [dict(theta=0.0), dict(theta=math.nan), dict(theta=-1e4), dict(linear=math.inf), dict(linear=math.nan),
+                                 dict(ntk=math.nan), dict(yarn={"scale": math.nan, "original": 8}),
+                                 dict(yarn={"scale": 2.0, "original": 0}), dict(yarn={"scale": 2.0, "original": 8, "fast": 1.0}),
+                                 dict(yarn={"scale": 2.0, "original": 8, "slow": 40.0}),
+                                 dict(yarn={"scale": 2.0, "original": 8, "slow": math.nan})])
+def test_rotary_tables_refuse_what_gives_no_frequencies(pkg, bad):
+    with pytest.raises(ValueError):
+        pkg.attention.rotary_frequencies(64, **bad)
+
+
 # ---- what no run can show: rules of the memory model and of warp votes, read from the sources
 
 
