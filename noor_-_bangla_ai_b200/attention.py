@@ -172,6 +172,8 @@ class Rotary:
                 device, int) else device)
         if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_cuda:
             raise ValueError("inv_freq must be a 1-D float32 CUDA tensor")
+        if inv_freq.requires_grad or _tangent(inv_freq) is not None:
+            raise ValueError("the frequencies have no gradient: detach them")
         self.inv_freq = inv_freq.contiguous()
         self.rotate_dim = 2 * inv_freq.numel()
         self.layout, self.factor = layout, float(factor)

@@ -119,6 +119,15 @@ def test_rope_gradient(pkg, cuda_device, layout):
     check_rope(g, torch.ones((3, 1, 32)), pos.cpu(), inv, layout, factor, -1.0)
 
 
+def test_rotary_refuses_frequencies_that_want_a_gradient(pkg, cuda_device):
+    A, f = pkg.attention, torch.ones(4, device="cuda")
+    with pytest.raises(ValueError, match="no gradient"):
+        A.Rotary(f.clone().requires_grad_())
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
+        A.Rotary(torch.autograd.forward_ad.make_dual(f, f))
+    assert A.Rotary(f).rotate_dim == 8
+
+
 # ---------------------------------------------------------------- the cache
 
 
