@@ -277,6 +277,34 @@ def test_append_half_layout_with_an_odd_half(pkg, cuda_device, fmt, dtype, rot, 
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("held", [0, 3, 21])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_poisoned_block_holds_zero_codes(pkg, cuda_device, fmt, dtype, held, bad):
+    """Attention multiplies a masked token's zero weight by its stored code, so a
+    poisoned block's codes are zeros: those written with the bad value, the old
+    ones before it, and those written after it."""
+    D, blk, H = 32, 32, 2
+    for which in ("k", "v"):
+        c, _, _ = make_cache(pkg, 2, H, blk, D, fmt)
+        tab = i32([[1]])
+        write = lambda x, end: c.append(*((x, torch.ones_like(x)) if which == "k" else (torch.ones_like(x), x)), tab, i32([end]),
+                                        i32([0, x.size(0)]))
+        if held:
+            write(randn((held, H, D), 120, DT[dtype]).cuda(), held)
+        x = randn((4, H, D), 121, DT[dtype])
+        x[2, 1, 7] = bad
+        write(x.cuda(), held + 4)
+        for end in (held + 4, held + 6):
+            codes = (c.k_codes[1] if which == "k" else c.v_codes[1].transpose(1, 2)).view(torch.uint8)[:, :end]
+            scale = c.k_scale if which == "k" else c.v_scale
+            assert torch.isnan(scale[1, 1]) and torch.isfinite(scale[1, 0])
+            assert not bool(codes[1].any()) and bool(codes[0].any())
+            write(randn((2, H, D), 122, DT[dtype]).cuda(), end + 2)
+    c.check()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_append_grows_a_scale_with_every_token(pkg, cuda_device, fmt):
     """Token after token of twice the size: every write reads the scale that the
     one before left, and rounds all earlier codes again."""
