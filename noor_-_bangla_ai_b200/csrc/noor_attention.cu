@@ -140,6 +140,13 @@ int check_batch(const noor_kv_cache* c, const noor_kv_batch* b, bool need_lens =
   return NOOR_MOE_OK;
 }
 
+// The write and the read back number the blocks that 256 sequences touch in 32
+// bits; row offsets that overlap may give each of them all the rows.
+int check_touched(const noor_kv_cache* c, const noor_kv_batch* b) {
+  if (b->n_rows / c->block + 2 > INT32_MAX / 256) return fail(NOOR_MOE_ERR_INVALID, "n_rows out of range");
+  return NOOR_MOE_OK;
+}
+
 kv::Cache cache_of(const noor_kv_cache* c) {
   return kv::Cache{static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->v_codes), c->k_scale, c->v_scale,
                    c->status, c->num_blocks, c->n_kv_heads, c->head_dim, c->block};
@@ -233,6 +240,7 @@ int noor_kv_append(const noor_kv_cache* c, const noor_kv_batch* b, const noor_he
   return guarded([&]() -> int {
     CKR(check_cache(c));
     CKR(check_batch(c, b));
+    CKR(check_touched(c, b));
     CKR(check_dtype(dtype));
     if (r) CKR(check_rotary(r, c->head_dim));
     if (!r) q = nullptr;
@@ -320,6 +328,7 @@ int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, const int32_t* 
   return guarded([&]() -> int {
     CKR(check_cache(c));
     CKR(check_batch(c, b, false));
+    CKR(check_touched(c, b));
     CKR(check_dtype(dtype));
     if (b->n_rows == 0) return NOOR_MOE_OK;
     if (!k_out || !v_out) return fail(NOOR_MOE_ERR_INVALID, "null output");

@@ -11,6 +11,7 @@ torch = pytest.importorskip("torch")
 
 P = 1 << 20  # a pointer that is aligned and never read
 INVALID, UNSUPPORTED = 1, 7
+NO_DEVICE = 1 << 20  # a device number that is refused before any launch
 
 
 def _cache(api, **kw):
@@ -105,9 +106,12 @@ def test_outputs_whose_heads_overlap_are_refused(pkg):
         assert _call(api, "attention", out=o) == INVALID and _call(api, "append", out=o) == INVALID
         assert _call(api, "rope", out=o) == INVALID and _call(api, "rope", rk=_heads(api), rk_out=o, k_heads=2) == INVALID
         assert b"overlap" in api.lib().noor_moe_last_error()
-    one = api.Heads(P, 0, 0)  # one token, one head: no stride is used
-    assert _call(api, "rope", out=one, tokens=1, q_heads=1) != INVALID
-    assert _call(api, "attention", out=api.Heads(P, 64, 10 ** 6)) != INVALID
+    # accepted (up to the device, which no machine has): one token and one head, whose strides are not used
+    one = api.Heads(P, 0, 0)
+    assert _call(api, "rope", out=one, tokens=1, q_heads=1, device=NO_DEVICE) != 0
+    assert b"overlap" not in api.lib().noor_moe_last_error()
+    assert _call(api, "attention", out=api.Heads(P, 64, 10 ** 6), cache=_cache(api, device=NO_DEVICE)) != 0
+    assert b"overlap" not in api.lib().noor_moe_last_error()
 
 
 def test_rows_past_32_bits_are_refused(pkg):
@@ -126,6 +130,17 @@ def test_rows_past_32_bits_are_refused(pkg):
         assert _call(api, "attention", cache=_cache(api, n_kv_heads=1), batch=_batch(api, n_rows=rows), q_heads=heads,
                      bytes=1 << 62) == INVALID
         assert b"32 bits" in api.lib().noor_moe_last_error()
+
+
+@pytest.mark.parametrize("name", ["append", "read"])
+def test_blocks_past_32_bits_are_refused(pkg, name):
+    """256 sequences that (by overlapping offsets) have all the rows each touch
+    fewer than 2^31 blocks."""
+    api = pkg.api
+    for rows, block, ok in ((1 << 28, 16, False), (1 << 28, 32, False), (1 << 28, 64, True), (1 << 26, 16, True)):
+        # (accepted up to the device, which no machine has)
+        assert _call(api, name, cache=_cache(api, block=block, device=NO_DEVICE), batch=_batch(api, n_rows=rows)) != 0
+        assert (b"n_rows" in api.lib().noor_moe_last_error()) != ok, (rows, block)
 
 
 def test_python_refuses_cpu_tensors(pkg):
