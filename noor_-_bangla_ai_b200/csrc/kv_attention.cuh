@@ -203,6 +203,8 @@ struct Shape {
                                             : (NB == 1 ? 3 : 2);
   static constexpr int kStages = 2;
   static constexpr int kQBytes = kQShared ? DP / 16 * NB * PARTS * 32 * 8 : 0;
+  // with four column groups, each warp's rows' v references
+  static constexpr int kRefBytes = NB > 2 ? 2 * kRows * 4 : 0;
   // v pages of 16 or 32 tokens lie 32 or 64 bytes apart, so that the quads'
   // reads of different pages fall into different banks
   static constexpr int kVPad = 128;
@@ -210,7 +212,7 @@ struct Shape {
   static constexpr int kJoin = (DP / 16 * NB * 4 + 6 * NB) * 32 * 4;
   static __host__ __device__ int pair_bytes(int D) {
     const int ring = kStages * (2 * kTile * D + kVPad);
-    return (ring > kJoin ? ring : kJoin) + kQBytes;
+    return (ring > kJoin ? ring : kJoin) + kQBytes + kRefBytes;
   }
   static constexpr int kBarBytes = (kPairs * 2 * kStages * 8 + 127) / 128 * 128;
   static __host__ __device__ int smem_bytes(int D) { return kBarBytes + kPairs * pair_bytes(D); }
@@ -230,7 +232,8 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   uint8_t* s_k = mine;
   uint8_t* s_v = mine + NST * kbytes;
   float* s_join = reinterpret_cast<float*>(mine);
-  uint2* s_q = reinterpret_cast<uint2*>(mine + Sh::pair_bytes(D) - Sh::kQBytes);  // [part][k step][nb][lane]
+  uint2* s_q = reinterpret_cast<uint2*>(mine + Sh::pair_bytes(D) - Sh::kQBytes - Sh::kRefBytes);  // [part][k step][nb][lane]
+  float* s_ref = reinterpret_cast<float*>(mine + Sh::pair_bytes(D) - Sh::kRefBytes) + half * R + 2 * qc;  // [half][row]
   if (half == 0 && lane < 2 * NST) tc::mbar_init(bars + lane, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -462,14 +465,24 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][nb][x] = 0.f;
     float m[NB][2], l[NB][2];
-    float vinv[NB][2];  // over each row's largest v scale so far, a power of two
+    // One over each row's largest v scale so far, up to a power of two: in
+    // registers, or with four column groups (whose sums leave none) in shared
+    // memory, where the eight lanes of a row write the same.
+    float vreg[NB][2];
+    auto vinv = [&](int nb, int x) -> float& {
+      if constexpr (NB <= 2)
+        return vreg[nb][x];
+      else
+        return s_ref[8 * nb + x];
+    };
+    float vlow = 1.17549435e-38f;  // the smallest of the rows' references, or less
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         m[nb][x] = -INFINITY;
         l[nb][x] = 0.f;
-        vinv[nb][x] = kv::kMostScale;  // (2^126)
+        vinv(nb, x) = kv::kMostScale;  // (2^126)
       }
 
     // Fixed parts of this lane's addresses: its score tokens' page and rows, its
@@ -533,11 +546,12 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
       // ---- scale, mask, running maximum
       float alpha[NB][2], mref[NB][2];
       const float vmax = fmaxf(fmaxf(vs, 0.f), __shfl_xor_sync(0xffffffffu, vs, 16));
+      const float vup = kv::power_up(vmax);
+      const bool vgrow = vup > vlow;
       bool moved = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float tm[2] = {-INFINITY, -INFINITY}, vseen[2] = {vmax, vmax};  // largest scale that the row sees here
-        if constexpr (!whole) vseen[0] = vseen[1] = 0.f;
+        float tm[2] = {-INFINITY, -INFINITY}, vseen[2] = {0.f, 0.f};  // (masked) largest scale that the row sees here
         const float f0 = qfac[nb][0] * ks, f1 = qfac[nb][1] * ks;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -569,17 +583,21 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             vseen[x] = fmaxf(vseen[x], __shfl_xor_sync(0xffffffffu, vseen[x], 8));
             vseen[x] = fmaxf(vseen[x], __shfl_xor_sync(0xffffffffu, vseen[x], 16));
           }
-          const float vnew = fminf(vinv[nb][x], kv::power_inverse(kv::power_up(vseen[x])));
-          alpha[nb][x] *= vnew * kv::power_inverse(vinv[nb][x]);
-          vinv[nb][x] = vnew;
+          if (!whole || vgrow) {
+            const float was = vinv(nb, x), now = fminf(was, kv::power_inverse(whole ? vup : kv::power_up(vseen[x])));
+            alpha[nb][x] *= now * kv::power_inverse(was);
+            vinv(nb, x) = now;
+          }
           moved |= alpha[nb][x] != 1.f;
         }
       }
+      if (whole && vgrow) vlow = vup;
       // ---- probabilities, transposed into the second operand's layout
       uint32_t pf[PARTS][NB][4];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float sum[2] = {0.f, 0.f};
+        const float vrel[2] = {vs * vinv(nb, 0), vs * vinv(nb, 1)};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -587,7 +605,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
             const float p = exp2_approx(sc[i][nb][x] - mref[nb][x & 1]);
             sum[x & 1] += p;
             // a masked token's p is zero whatever its block's scale
-            sc[i][nb][x] = !whole && sc[i][nb][x] == -INFINITY ? 0.f : p * (vs * vinv[nb][x & 1]);
+            sc[i][nb][x] = !whole && sc[i][nb][x] == -INFINITY ? 0.f : p * vrel[x & 1];
           }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -682,7 +700,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
         for (int x = 0; x < 2; ++x) {
           j[(4 * nb + 2 * x) * 32] = m[nb][x];
           j[(4 * nb + 2 * x + 1) * 32] = l[nb][x];
-          j[(4 * NB + 2 * nb + x) * 32] = kv::power_inverse(vinv[nb][x]);
+          j[(4 * NB + 2 * nb + x) * 32] = kv::power_inverse(vinv(nb, x));
         }
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
@@ -709,7 +727,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
           if (r >= nrows) continue;
           const int e = e0 + r, row = w.s.row0 + e / a.g, head = h * a.g + e % a.g;
           const float inv = !done ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
-          const float g0 = f0 * kv::power_inverse(vinv[nb][x]) * inv, g1 = f1 * j[(4 * NB + 2 * nb + x) * 32] * inv;
+          const float g0 = f0 * kv::power_inverse(vinv(nb, x)) * inv, g1 = f1 * j[(4 * NB + 2 * nb + x) * 32] * inv;
           if (gr == 0) {
             if (!done) {
               a.part_ml[(slot * R + r) * 2] = ll == 0.f ? -INFINITY : mm;
