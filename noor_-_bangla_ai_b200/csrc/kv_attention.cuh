@@ -203,8 +203,8 @@ struct Shape {
                                             : (NB == 1 ? 3 : 2);
   static constexpr int kStages = 2;
   static constexpr int kQBytes = kQShared ? DP / 16 * NB * PARTS * 32 * 8 : 0;
-  // with four column groups, each warp's rows' v references
-  static constexpr int kRefBytes = NB > 2 ? 2 * kRows * 4 : 0;
+  // with four column groups, each lane's rows' v references
+  static constexpr int kRefBytes = NB > 2 ? 64 * NB * 8 : 0;
   // v pages of 16 or 32 tokens lie 32 or 64 bytes apart, so that the quads'
   // reads of different pages fall into different banks
   static constexpr int kVPad = 128;
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
   uint8_t* s_v = mine + NST * kbytes;
   float* s_join = reinterpret_cast<float*>(mine);
   uint2* s_q = reinterpret_cast<uint2*>(mine + Sh::pair_bytes(D) - Sh::kQBytes - Sh::kRefBytes);  // [part][k step][nb][lane]
-  float* s_ref = reinterpret_cast<float*>(mine + Sh::pair_bytes(D) - Sh::kRefBytes) + half * R + 2 * qc;  // [half][row]
+  float* s_ref = reinterpret_cast<float*>(mine + Sh::pair_bytes(D) - Sh::kRefBytes) + 64 * half * NB + 2 * lane;  // [half][nb][lane][2]
   if (half == 0 && lane < 2 * NST) tc::mbar_init(bars + lane, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -467,13 +467,14 @@ __global__ void __launch_bounds__(Shape<DP, PARTS, NB>::kPairs * 64, 1) stream_k
     float m[NB][2], l[NB][2];
     // One over each row's largest v scale so far, up to a power of two: in
     // registers, or with four column groups (whose sums leave none) in shared
-    // memory, where the eight lanes of a row write the same.
+    // memory, a place of its own for each lane (one for the eight lanes of a row
+    // would need the warp to meet between its reads and writes: 6% of the time).
     float vreg[NB][2];
     auto vinv = [&](int nb, int x) -> float& {
       if constexpr (NB <= 2)
         return vreg[nb][x];
       else
-        return s_ref[8 * nb + x];
+        return s_ref[64 * nb + x];
     };
     float vlow = 1.17549435e-38f;  // the smallest of the rows' references, or less
 #pragma unroll
