@@ -390,7 +390,9 @@ typedef struct {
  * number of rows the row tensors hold; rows at or past cu_rows[batch] are
  * padding and are left as they were.  A sequence may have no rows.  One whose
  * offsets or length are wrong is skipped, and a page that cannot be read reads
- * as NaN; both set the status word. */
+ * as NaN; both set the status word.  n_rows is at most 2^28; n_rows / block stays
+ * below 2^23 - 2 for the write and the read back, and n_rows times the query heads of a
+ * kv head below 2^31 - 256 for attention. */
 typedef struct {
   const int32_t* block_table; /* [batch][max_blocks], entries past a sequence's pages are not read */
   int64_t table_stride;
@@ -426,12 +428,15 @@ NOOR_MOE_API int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, co
  * a query at position p = kv_lens[b] - rows(b) + i and sees the tokens j <= p
  * (window > 0: only p - j <= window, as attention.rs:133-136), query head h
  * over kv head h / (q_heads / n_kv_heads).  out = softmax(scale q.k) v; a row
- * that sees nothing gets zeros.  q, out [n_rows][q_heads] (they may be the
- * same); lse [n_rows][q_heads] f32 contiguous, nullable: the natural
- * logarithm of the sum of exponentials, -inf for a row that sees nothing.
+ * sees itself at least; one whose query is not finite is NaN.  q, out
+ * [n_rows][q_heads] (they may be the same); lse [n_rows][q_heads] f32
+ * contiguous, nullable: the natural logarithm of the sum of exponentials.
+ * Scores, maxima, sums and outputs are held in f32 until the output's own
+ * rounding; on the way to the tensor cores a weight is rounded to f16 (2^-11 of
+ * it) for BF16 calls, and F32 calls take queries and weights as two f16 parts (22 bits).
  * Values are held in f16 relative to the largest v scale among the tokens that
  * the row itself sees: blocks whose scale is below 2^-15 of it (int8: 2^-24) may
- * lose bits of their codes.  Tokens that a row does not see never matter to it.
+ * lose bits of their codes.  Blocks that a row sees no token of never matter to it.
  * max_rows: the most rows of any sequence, a hint that picks the kernels (a
  * wrong value costs time, not results).  The workspace, 16-byte aligned, of
  * at least noor_kv_attention_workspace bytes for the same arguments, is free

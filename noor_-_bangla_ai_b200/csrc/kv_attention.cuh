@@ -30,11 +30,11 @@
 // its bits alone.
 //
 // Measured at 32 / 8 heads of 128 dims: 64 ragged sequences of up to 8192
-// tokens, a row each, e4m3, 120-124 us = 5.5 TB/s of codes; 4 x 131072 tokens,
-// int8, 213-218 us = 5.0 TB/s.  int8 takes five instructions to widen a word, e4m3
-// two: e4m3 is bound by memory, int8 by its pairs' chains (0.47 instructions a
+// tokens, a row each, e4m3, 122-124 us = 5.5 TB/s of codes; 4 x 131072 tokens,
+// int8, 215-220 us = 4.9 TB/s.  int8 takes five instructions to widen a word, e4m3
+// two: e4m3 is bound by memory, int8 by its pairs' chains (0.50 instructions a
 // cycle and scheduler, between waits on shared loads and fixed latencies).  One stream of 1000 tokens
-// takes 14 us, the chain of its loads (lengths, page table, codes) and the join.
+// takes 13 us, the chain of its loads (lengths, page table, codes) and the join.
 //
 // The contraction index of an mma may be permuted at will if both operands
 // agree: thread c of a quad takes 16 consecutive bytes of a key row and feeds

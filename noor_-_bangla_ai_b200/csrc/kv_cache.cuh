@@ -320,9 +320,9 @@ __device__ __forceinline__ float4 toward4(const double (&x)[4]) {
 // that rounds alike, so the codes are those of the exact rotation.
 // Bound by memory once enough blocks run: the elements are read once into
 // registers.  Measured with the values' and q's launches: 8 ragged prompts of up
-// to 4096 tokens, 32 + 8 heads of 128 dims, BF16 to e4m3, 145 us = 3.6 TB/s (half
+// to 4096 tokens, 32 + 8 heads of 128 dims, BF16 to e4m3, 111 us = 3.7 TB/s (half
 // of it is q at 6.7 TB/s; the rest waits on f64 products and the block's
-// maximum); a decode step of 128 streams 20.5 us, the time of one block's chain
+// maximum); a decode step of 128 streams 8.6 us, the time of one block's chain
 // of loads: its place, its page, the old scale.
 template <typename T, int FMT, int TPT>
 __device__ void append_keys(const AppendArgs& a, const Task& k, int h0, int h1, Maxima& s_max) {
@@ -740,7 +740,7 @@ constexpr int kReadThreads = 256;
 // 16 tokens of 4 dims (four 16-byte loads), turns each 4 x 4 bytes over in
 // registers and writes 4 dims of each token, so a warp's stores are whole
 // rows.  Bound by memory: codes in, 2 or 4 bytes a code out.  32 ragged prefixes
-// of up to 4096 tokens, 8 heads of 128 dims, to BF16: 92 us, 5.2 TB/s.
+// of up to 4096 tokens, 8 heads of 128 dims, to BF16: 91 us, 5.2 TB/s.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const ReadArgs a) {
   const Cache& c = a.c;

@@ -24,7 +24,7 @@
 // p <= 2^15 then fits f16; shift 7 keeps p down to 2^-31 of the largest.
 //
 // Measured: 2 sequences of 2048 rows on 8192 tokens, 32 / 8 heads of 128 dims,
-// 547 us = 880 TFLOP/s of visible products.  Bound by the softmax warps: an
+// 549-558 us = 860-880 TFLOP/s of visible products.  Bound by the softmax warps: an
 // exponential, its scaling and the sums for each score, beside TMEM reads; the
 // tensor core waits for p.
 // V scales.  o of a row is held relative to the largest v scale (up to a power
@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
 
   // Registers: 128 a thread at launch (512 x 128, the whole file); the eight
   // softmax warps take 160, the other eight keep 96 (256 x 160 + 256 x 96 =
-  // 65536): neither spills.
+  // 65536).  Nothing spills with whole contexts at 128 dims; their cut form spills 12
+  // bytes (stores), the forms for 64 dims 64-76.
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     // ------------------------------------------------------- softmax

@@ -165,8 +165,8 @@ int64_t most_tasks(const noor_kv_cache* c, const noor_kv_batch* b) {
 // kv heads that one grid block takes in turn, so that finding its place and
 // (for keys) the angles is paid for once: as many as leave eight blocks for
 // every SM, at most 8.  Against one head, at 8 kv heads of 128
-// dims: 8 ragged prompts of up to 4096 tokens written in 145 us instead of 201,
-// 32 ragged prefixes of up to 4096 read back in 94 instead of 115.
+// dims: 8 ragged prompts of up to 4096 tokens written and read back in 145 us
+// instead of 201, 32 ragged prefixes of up to 4096 read back in 94 instead of 115.
 int heads_per_block(const noor_kv_cache* c, int64_t tasks, int32_t* heads) {
   int sms = 0;
   CKR(sm_count(c->device, &sms));
@@ -393,7 +393,7 @@ bool cut_pays(int units, int tiles, int sms) {
 // but a tile's chain is longer and less runs beside it.  16 sequences of 4096
 // tokens, 4 kv heads, one group / many: F32 at 128 dims 12 rows 41 / 69 us,
 // 48 rows 91 / 108, 64 rows 113 / 114; at 256 dims 12 rows 101 / 101, 32 rows
-// 177 / 154 (BF16 154 / 128).  BF16 up to 128 dims has the other kernel for
+// 177 / 154 (BF16 154 / 133).  BF16 up to 128 dims has the other kernel for
 // more rows.
 int stream_plan(const noor_kv_cache* c, const noor_kv_batch* b, int Hq, int max_rows, int window, int dtype, StreamPlan* p) {
   int sms = 0;

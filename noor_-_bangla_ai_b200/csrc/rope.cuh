@@ -150,7 +150,7 @@ __host__ __device__ __forceinline__ int head_units(int D, int rot, int layout) {
 // One block per `tok` tokens: the table of each token's angles is made once
 // in shared memory and used by every head of q and k.  Bound by memory: each
 // element is read and written once.  32768 tokens of 32 + 8 heads of 128 dims,
-// BF16, forward and gradient: 230 us, 5.8 TB/s; a decode step's 64 tokens 4.1 us, a launch's time.
+// BF16, forward and gradient: 230-240 us, 5.6-5.8 TB/s; a decode step's 64 tokens 3.1 us, a launch's time.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) rope_kernel(const Args a, int tok) {
   extern __shared__ float2 s_tab[];
