@@ -31,8 +31,8 @@
 // of two) among the tokens that the row has seen so far, and follows when that
 // grows; what a row does not see leaves its bits alone.
 //   A tile that every row of the unit sees whole is widened relative to its own
-//   largest scale (exact for powers of two, down to 2^-24 of it for int8 and
-//   2^-15 for e4m3), and its ratio to the row's, a power of two, goes into the
+//   largest scale (exact for powers of two down to 2^-24 of it for int8 and
+//   2^-15 for e4m3; below, to 2^-25 of the largest scale), and its ratio to the row's, a power of two, goes into the
 //   exponential: p comes out scaled, and its sum is scaled back.
 //   In the other tiles (the context's end, a window's start) values are codes
 //   alone, and each p is multiplied by its block's scale over the row's.
@@ -545,7 +545,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
       if (!ok) break;
       uint8_t* dv = s_v + slot * S::kK;
       const float vf = s_vf[i % kMeta][vq];
-      const __half2 hf = __float2half2_rn(vf);
+      // (a factor below f16's normal range is taken in two steps: as one it would
+      // lose the bits that its products still have, and be zero below 2^-24)
+      const bool low = vf < 6.1035156e-05f;  // 2^-14
+      const __half2 hf = __float2half2_rn(low ? vf * 16384.f : vf), h14 = __float2half2_rn(6.1035156e-05f);
       // codes past the last visible token, or of a page that cannot be read, count as zero
       const int nv = vf != 0.f ? min(max(hi_tok - ((tb + i) * kTok + 16 * vq), 0), 16) : 0;
       uint32_t keep[4];
@@ -572,7 +575,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const Args a) {
             uint32_t* w8[8] = {&u.x, &u.y, &u.z, &u.w, &v.x, &v.y, &v.z, &v.w};
 #pragma unroll
             for (int z = 0; z < 8; ++z) {
-              const __half2 m2 = __hmul2(*reinterpret_cast<__half2*>(w8[z]), hf);
+              __half2 m2 = __hmul2(*reinterpret_cast<__half2*>(w8[z]), hf);
+              if (low) m2 = __hmul2(m2, h14);
               *w8[z] = *reinterpret_cast<const uint32_t*>(&m2);
             }
           }

@@ -625,6 +625,32 @@ def test_hidden_value_scales_leave_a_row_alone(pkg, cuda_device, dtype, fmt, D, 
     c.check()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("down", [10, 16, 20, 24, 26, 28])
+@pytest.mark.parametrize("D,blk", [(64, 16), (128, 32)])
+def test_values_of_a_small_block_beside_large_ones(pkg, cuda_device, fmt, down, D, blk):
+    """All weight on a token whose block's scale is 2^-down of its neighbours', in
+    a tile that every row sees whole: its values are off by f16's last place
+    relative to the largest scale (2^-25 of it), not more."""
+    L, n, P = 240, 100, -(-240 // blk)
+    c, _, _ = make_cache(pkg, P, 1, blk, D, fmt)
+    rk, rv = fill(c, 53)
+    at = blk + 3  # the token, in the second block
+    rv.scale[:] = 1.0
+    rv.scale[1] = 2.0 ** -down
+    c.v_scale.copy_(rv.scale.float())
+    key = rk.tokens(range(P), L)[at, 0]
+    q = (key * (60.0 / float(key @ key) * D ** 0.5)).expand(n, 4, D).to(torch.bfloat16)  # its score: 60
+    tab = i32([list(range(P))])
+    got = c.attention(q.cuda(), tab, i32([L]), i32([0, n]), n).cpu().double()
+    k, v = rk.tokens(range(P), L), rv.tokens(range(P), L)
+    o, _, mag, smax, _ = ref.attend(q.double(), k, v, torch.arange(L - n, L), D ** -0.5, 0)
+    vsum = (v[:, 0].abs() / rv.scale[:, 0].repeat_interleave(blk)[:L, None]).sum(0)
+    tol = ref.attend_tolerance(torch.bfloat16, o, mag, smax, vsum, D, L) + 2.0 ** -25
+    assert bool(((got - o).abs() <= tol).all()), float(((got - o).abs() / tol).max())
+    c.check()
+
+
 @pytest.mark.parametrize("news", [1, 200])
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_attention_masked_blocks_may_hold_anything(pkg, cuda_device, news, fmt):
