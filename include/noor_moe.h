@@ -436,7 +436,7 @@ NOOR_MOE_API int noor_kv_read(const noor_kv_cache* c, const noor_kv_batch* b, co
  * it) for BF16 calls, and F32 calls take queries and weights as two f16 parts (22 bits).
  * Values are held in f16 relative to the largest v scale among the tokens that
  * the row itself sees: blocks whose scale is below 2^-15 of it (int8: 2^-24) may
- * lose bits of their codes.  Blocks that a row sees no token of never matter to it.
+ * lose bits of their codes, down to 2^-25 of that scale.  Blocks that a row sees no token of never matter to it.
  * max_rows: the most rows of any sequence, a hint that picks the kernels (a
  * wrong value costs time, not results).  The workspace, 16-byte aligned, of
  * at least noor_kv_attention_workspace bytes for the same arguments, is free
